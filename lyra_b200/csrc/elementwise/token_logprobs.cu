@@ -1,0 +1,534 @@
+// Scores of given tokens from logits: log probability, entropy and the k most likely alternatives of every row, and the
+// gradient of the first two.
+//
+//   lse = log sum_v e^{x_v}      logprob = x_t - lse      H = lse - sum_v p_v x_v
+//   dx_v = g_l ([v = t] - p_v) - g_H p_v (log p_v + H)
+//
+// Forward: one pass over a row with the running maximum m, s = sum e^{x-m} and u = sum e^{x-m} (x-m), from
+// which lse = m + log s and H = log s - u / s: no cancellation between two large numbers. The pass also leaves the maximum of
+// every run of loads in shared memory. The alternatives then need no second pass: the k-th largest of 64 disjoint subset maxima
+// is a bound that at least k elements reach and few exceed, and only the runs that reach it are read again (a few hundred
+// bytes, still in L2). The candidates are ranked by (value, lowest id), so the order in which they were found does not matter.
+//
+// Few rows are split over a cluster of up to eight CTAs (each SM streams a slice; partial results meet in the first CTA through
+// distributed shared memory): one row of 201088 fp32 logits would otherwise be read by one SM.
+#include <cooperative_groups.h>
+#include <cuda_bf16.h>
+#include <cuda_runtime.h>
+#include <math.h>
+#include <stdint.h>
+
+#include "../common/tmap.h"
+
+namespace lyra {
+namespace tlp {
+
+namespace cg = cooperative_groups;
+
+constexpr int THREADS = 512;
+constexpr int UNROLL = 4;            // 16-byte loads in flight per thread
+constexpr int MAX_TOP = 32;
+constexpr int CAP = 1024;            // candidate buffer; more candidates than this (long runs of equal logits) take the slow selection
+constexpr int MAX_RUNS = 10240;      // run maxima kept per CTA (40 KB)
+constexpr float L2E = 1.4426950408889634f;
+// Distances below the maximum are cut off here: e^{-1000} is 0 in fp32 as well, and 0 * y stays 0 for logits of -inf and for
+// masks of the type's lowest value, whose distance would overflow. The maximum itself is kept in the logits' own unit, so a row
+// that holds nothing but the lowest value is a uniform distribution.
+constexpr float FLOOR = -1000.f;
+
+struct Fwd {
+  const void* x;
+  const long long* target;           // [N], negative: the row has no target (logprob 0)
+  float* logprob;                    // [N]
+  float* entropy;                    // [N]
+  float* norm;                       // [2, N]: m and log s, for the gradient
+  float* top_lp;                     // [N, k]
+  long long* top_id;                 // [N, k]
+  long long stride;                  // elements between rows
+  int N, V, k, chunks_per_run;
+};
+
+// Order of the alternatives: larger value first (NaN above +inf, as a sort in torch has it; -0 equals 0), then lower id.
+__device__ __forceinline__ uint32_t order_key(float x) {
+  if (x != x) return 0xffffffffu;
+  const uint32_t b = __float_as_uint(x + 0.0f);
+  return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
+}
+__device__ __forceinline__ float key_value(uint32_t k) {
+  if (k == 0xffffffffu) return __uint_as_float(0x7fc00000u);
+  return __uint_as_float((k & 0x80000000u) ? (k & 0x7fffffffu) : ~k);
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
+template <typename T>
+struct Vec;
+template <>
+struct Vec<float> {
+  static constexpr int N = 4;
+  __device__ static void unpack(const uint4& v, float (&f)[4]) {
+    f[0] = __uint_as_float(v.x); f[1] = __uint_as_float(v.y); f[2] = __uint_as_float(v.z); f[3] = __uint_as_float(v.w);
+  }
+  __device__ static uint4 pack(const float (&f)[4]) {
+    return make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
+  }
+  __device__ static float load(const float* p) { return *p; }
+  __device__ static float largest(const uint4& v) {
+    return max_nan(max_nan(__uint_as_float(v.x), __uint_as_float(v.y)), max_nan(__uint_as_float(v.z), __uint_as_float(v.w)));
+  }
+  static constexpr uint32_t MINUS_INF = 0xff800000u;
+};
+template <>
+struct Vec<__nv_bfloat16> {
+  static constexpr int N = 8;
+  __device__ static void unpack(const uint4& v, float (&f)[8]) {
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      f[2 * i] = __uint_as_float(w[i] << 16);
+      f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    }
+  }
+  __device__ static uint4 pack(const float (&f)[8]) {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      __nv_bfloat162 t = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
+      w[i] = *reinterpret_cast<uint32_t*>(&t);
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+  }
+  __device__ static float load(const __nv_bfloat16* p) { return __bfloat162float(*p); }
+  __device__ static uint32_t max2(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+  }
+  __device__ static float largest(const uint4& v) {          // two values per instruction, unpacked once per 16 bytes
+    const uint32_t m = max2(max2(v.x, v.y), max2(v.z, v.w));
+    return max_nan(__uint_as_float(m << 16), __uint_as_float(m & 0xffff0000u));
+  }
+  static constexpr uint32_t MINUS_INF = 0xff80ff80u;
+};
+
+// A row is a list of 16-byte vectors on 16-byte boundaries: vector i holds elements i * VE - lead .. + VE - 1, where lead is the
+// row's distance from the boundary below it. The first and the last vector may reach over the row's ends: those are gathered
+// element by element and filled with -inf.
+template <typename T>
+struct Row {
+  static constexpr int VE = Vec<T>::N;
+  const T* p;
+  int V, lead, n_vec;
+  __device__ Row(const T* row, int v) : p(row), V(v) {
+    lead = int((reinterpret_cast<uintptr_t>(row) & 15) / sizeof(T));
+    n_vec = int(((long long)v + lead + VE - 1) / VE);
+  }
+  __device__ uint4 vec(int i) const {
+    const int e0 = i * VE - lead;
+    if (e0 >= 0 && e0 + VE <= V) return __ldg(reinterpret_cast<const uint4*>(p + e0));
+    uint32_t w[4];
+    if (sizeof(T) == 4) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) w[j] = (e0 + j >= 0 && e0 + j < V) ? reinterpret_cast<const uint32_t*>(p)[e0 + j] : 0xff800000u;
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int a = e0 + 2 * j, b = a + 1;
+        const uint32_t lo = (a >= 0 && a < V) ? reinterpret_cast<const uint16_t*>(p)[a] : 0xff80u;
+        const uint32_t hi = (b >= 0 && b < V) ? reinterpret_cast<const uint16_t*>(p)[b] : 0xff80u;
+        w[j] = lo | (hi << 16);
+      }
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+  }
+};
+
+struct Stat {      // running maximum (NaN once a NaN was seen), s = sum e^{x - m}, u = sum e^{x - m} (x - m)
+  float m, s, u;
+};
+__device__ __forceinline__ Stat merge(const Stat& a, const Stat& b) {
+  Stat r;
+  r.m = max_nan(a.m, b.m);
+  // an empty side has m = -inf, s = u = 0: its distance must not become inf * 0
+  const float da = a.m == -INFINITY ? 0.f : fmaxf(a.m - r.m, FLOOR), db = b.m == -INFINITY ? 0.f : fmaxf(b.m - r.m, FLOOR);
+  const float ea = exp2f(da * L2E), eb = exp2f(db * L2E);
+  r.s = a.s * ea + b.s * eb;
+  r.u = ea * (a.u + da * a.s) + eb * (b.u + db * b.s);
+  return r;
+}
+__device__ __forceinline__ Stat shfl_stat(const Stat& a, int o) {
+  return Stat{__shfl_xor_sync(0xffffffffu, a.m, o), __shfl_xor_sync(0xffffffffu, a.s, o), __shfl_xor_sync(0xffffffffu, a.u, o)};
+}
+
+struct Shared {
+  Stat part[THREADS / 32];
+  Stat total;
+  uint32_t tmax[THREADS];
+  uint32_t bound;
+  int n_cand;
+  unsigned long long cand[CAP];                     // (key << 32) | ~id : one unsigned comparison is the whole order
+  unsigned long long best[8 * MAX_TOP];             // the CTA's (then the cluster's) k best
+  unsigned long long red[THREADS / 32];
+};
+
+__device__ __forceinline__ unsigned long long entry(uint32_t key, int id) { return ((unsigned long long)key << 32) | (uint32_t)(~id); }
+
+// k best of list[0..n) into out[0..k): entries are distinct (their ids are), so an entry's rank is the number of larger ones.
+__device__ __forceinline__ void rank_select(const unsigned long long* list, int n, int k, unsigned long long* out) {
+  for (int i = threadIdx.x; i < n; i += THREADS) {
+    const unsigned long long mine = list[i];
+    int rank = 0;
+    for (int j = 0; j < n; ++j) rank += list[j] > mine;
+    if (rank < k) out[rank] = mine;
+  }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(THREADS, 2) token_logprobs_kernel(const Fwd p) {
+  constexpr int VE = Vec<T>::N;
+  extern __shared__ __align__(16) uint8_t dyn[];
+  Shared& sh = *reinterpret_cast<Shared*>(dyn);
+  uint32_t* run_key = reinterpret_cast<uint32_t*>(dyn + sizeof(Shared));
+  cg::cluster_group cluster = cg::this_cluster();
+  const int cs = int(cluster.num_blocks()), cr = int(cluster.block_rank());
+  const int row_id = int(blockIdx.x) / cs;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const T* rowp = reinterpret_cast<const T*>(p.x) + (long long)row_id * p.stride;
+  const Row<T> row(rowp, p.V);
+  const int v0 = int((long long)row.n_vec * cr / cs), v1 = int((long long)row.n_vec * (cr + 1) / cs);
+  constexpr int STEP = THREADS * UNROLL;
+  const int n_chunks = (v1 - v0 + STEP - 1) / STEP;
+
+  // ---- the pass over the slice
+  Stat st{-INFINITY, 0.f, 0.f};
+  uint32_t best_key = 0, this_run = 0;
+  int in_run = 0, run = 0;
+  for (int c = 0; c < n_chunks; ++c) {
+    uint4 v[UNROLL];
+    const int first = v0 + c * STEP + tid;
+#pragma unroll
+    for (int j = 0; j < UNROLL; ++j) {
+      const int i = first + j * THREADS;
+      v[j] = i < v1 ? row.vec(i) : make_uint4(Vec<T>::MINUS_INF, Vec<T>::MINUS_INF, Vec<T>::MINUS_INF, Vec<T>::MINUS_INF);
+    }
+    float g = Vec<T>::largest(v[0]);
+#pragma unroll
+    for (int j = 1; j < UNROLL; ++j) g = max_nan(g, Vec<T>::largest(v[j]));
+    if (p.k) {
+      if (first < v1) this_run = max(this_run, order_key(g));
+      if (++in_run == p.chunks_per_run) {
+        run_key[run++ * THREADS + tid] = this_run;
+        best_key = max(best_key, this_run);
+        this_run = 0;
+        in_run = 0;
+      }
+    }
+    const float m2 = max_nan(st.m, g);
+    if (!(m2 <= st.m)) {                            // moved up (or NaN)
+      if (st.m != -INFINITY) {
+        const float d = fmaxf(st.m - m2, FLOOR), e = exp2f(d * L2E);
+        st.u = e * (st.u + d * st.s);
+        st.s *= e;
+      }
+      st.m = m2;
+    }
+#pragma unroll
+    for (int j = 0; j < UNROLL; ++j) {
+      float f[VE];
+      Vec<T>::unpack(v[j], f);
+#pragma unroll
+      for (int i = 0; i < VE; ++i) {
+        const float y = fmaxf(f[i] - st.m, FLOOR);
+        const float e = exp2f(y * L2E);
+        st.s += e;
+        st.u = fmaf(e, y, st.u);
+      }
+    }
+  }
+  if (p.k && in_run) {
+    run_key[run++ * THREADS + tid] = this_run;
+    best_key = max(best_key, this_run);
+  }
+
+  // ---- statistics of the CTA, then of the cluster
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) st = merge(st, shfl_stat(st, o));
+  if (lane == 0) sh.part[warp] = st;
+  sh.tmax[tid] = best_key;
+  if (tid == 0) sh.n_cand = 0;
+  __syncthreads();
+  if (warp == 0) {
+    Stat t = lane < THREADS / 32 ? sh.part[lane] : Stat{-INFINITY, 0.f, 0.f};
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) t = merge(t, shfl_stat(t, o));
+    if (lane == 0) sh.total = t;
+  }
+
+  if (p.k) {
+    // ---- a bound that at least k elements reach: the k-th largest of 64 disjoint subset maxima
+    if (warp == 1) {
+      uint32_t a = 0, b = 0;
+#pragma unroll
+      for (int j = 0; j < THREADS / 64; ++j) {
+        a = max(a, sh.tmax[j * 64 + lane]);
+        b = max(b, sh.tmax[j * 64 + 32 + lane]);
+      }
+      int ra = 0, rb = 0;
+#pragma unroll 8
+      for (int s = 0; s < 32; ++s) {
+        const uint32_t oa = __shfl_sync(0xffffffffu, a, s), ob = __shfl_sync(0xffffffffu, b, s);
+        ra += (oa > a || (oa == a && s < lane)) + (ob > a);
+        rb += (oa >= b) + (ob > b || (ob == b && s < lane));
+      }
+      if (ra == p.k - 1) sh.bound = a;              // ranks 0..63 are all taken once; a subset without elements has key 0
+      if (rb == p.k - 1) sh.bound = b;
+    }
+    __syncthreads();
+    const uint32_t bound = max(sh.bound, 1u);       // key 0 marks "no element": every real key is larger (-inf has 0x007fffff)
+    for (int r = 0; r < run; ++r) {
+      if (run_key[r * THREADS + tid] < bound) continue;
+      for (int c = r * p.chunks_per_run; c < min((r + 1) * p.chunks_per_run, n_chunks); ++c) {
+        for (int j = 0; j < UNROLL; ++j) {
+          const int i = v0 + c * STEP + tid + j * THREADS;
+          if (i >= v1) continue;
+          const int e0 = i * VE - row.lead;
+          float f[VE];
+          Vec<T>::unpack(row.vec(i), f);
+#pragma unroll
+          for (int x = 0; x < VE; ++x) {
+            const uint32_t key = order_key(f[x]);
+            if (e0 + x >= 0 && e0 + x < p.V && key >= bound) {
+              const int at = atomicAdd(&sh.n_cand, 1);
+              if (at < CAP) sh.cand[at] = entry(key, e0 + x);
+            }
+          }
+        }
+      }
+    }
+    for (int i = tid; i < p.k; i += THREADS) sh.best[i] = 0;
+    __syncthreads();
+    if (sh.n_cand <= CAP) {
+      rank_select(sh.cand, sh.n_cand, p.k, sh.best);
+    } else {
+      // more than CAP elements reach the bound (long runs of equal logits): k passes, each takes the largest entry below the last
+      unsigned long long last = ~0ull;
+      for (int q = 0; q < p.k; ++q) {
+        unsigned long long mine = 0;
+        for (int i = v0 + tid; i < v1; i += THREADS) {
+          const int e0 = i * VE - row.lead;
+          float f[VE];
+          Vec<T>::unpack(row.vec(i), f);
+#pragma unroll
+          for (int x = 0; x < VE; ++x) {
+            if (e0 + x < 0 || e0 + x >= p.V) continue;
+            const unsigned long long en = entry(order_key(f[x]), e0 + x);
+            if (en < last && en > mine) mine = en;
+          }
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) mine = max(mine, __shfl_xor_sync(0xffffffffu, mine, o));
+        if (lane == 0) sh.red[warp] = mine;
+        __syncthreads();
+        mine = sh.red[0];
+        for (int w = 1; w < THREADS / 32; ++w) mine = max(mine, sh.red[w]);
+        if (tid == 0) sh.best[q] = mine;
+        last = mine;
+        __syncthreads();
+      }
+    }
+  }
+  __syncthreads();
+  if (cs > 1) {
+    cluster.sync();
+    if (cr == 0) {
+      if (tid == 0) {
+        Stat t = sh.total;
+        for (int r = 1; r < cs; ++r) t = merge(t, cluster.map_shared_rank(&sh, r)->total);
+        sh.total = t;
+      }
+      for (int i = tid; i < cs * p.k; i += THREADS) sh.cand[i] = cluster.map_shared_rank(&sh, i / p.k)->best[i % p.k];
+      __syncthreads();
+      // unfilled slots of small slices are 0: below every entry, but equal to one another, so they are dropped before ranking
+      if (p.k) {
+        for (int i = tid; i < cs * p.k; i += THREADS) {
+          const unsigned long long mine = sh.cand[i];
+          if (!mine) continue;
+          int rank = 0;
+          for (int j = 0; j < cs * p.k; ++j) rank += sh.cand[j] > mine;
+          if (rank < p.k) sh.best[MAX_TOP + rank] = mine;
+        }
+        __syncthreads();
+        for (int i = tid; i < p.k; i += THREADS) sh.best[i] = sh.best[MAX_TOP + i];
+      }
+      __syncthreads();
+    }
+    cluster.sync();                                 // no CTA leaves while its shared memory is read
+    if (cr != 0) return;
+  }
+
+  // ---- results
+  const Stat t = sh.total;
+  const bool bad = !(fabsf(t.m) < INFINITY);        // a NaN, a +inf, or nothing but -inf: no distribution
+  const float nan = __uint_as_float(0x7fc00000u);
+  const double log_s = log(double(t.s));
+  // (x - m) - log s, never x - lse: in a row of the type's lowest value m + log s would swallow log s
+  auto logp = [&](float x) { return float((double(x) - double(t.m)) - log_s); };
+  if (tid == 0) {
+    const long long tg = p.target[row_id];
+    float lp = nan;
+    if (tg < 0) lp = 0.f;
+    else if (tg < p.V && !bad) lp = logp(Vec<T>::load(rowp + tg));
+    p.logprob[row_id] = lp;
+    p.entropy[row_id] = bad ? nan : float(log_s - double(t.u) / double(t.s));
+    p.norm[row_id] = bad ? nan : t.m;
+    p.norm[p.N + row_id] = bad ? nan : float(log_s);
+  }
+  for (int i = tid; i < p.k; i += THREADS) {
+    const unsigned long long b = sh.best[i];
+    p.top_id[(long long)row_id * p.k + i] = (long long)(uint32_t)~(uint32_t)b;
+    p.top_lp[(long long)row_id * p.k + i] = bad ? nan : logp(key_value(uint32_t(b >> 32)));
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ gradient
+struct Bwd {
+  const void* x;
+  void* dx;                          // [N, W] contiguous
+  const long long* target;
+  const float *norm, *entropy, *g_lp, *g_h;     // g_lp / g_h may be null (no gradient from that output)
+  long long stride;
+  int N, V, W, blocks_per_row;       // columns V .. W - 1 (vocabulary padding) get zeros
+};
+
+constexpr int B_THREADS = 256, B_UNROLL = 4;
+
+// Bound by memory: every logit is read once and every gradient written once, in 16-byte pieces aligned to the gradient's row
+// (which a row of logits with the same distance from a 16-byte boundary shares; otherwise its elements are loaded one by one).
+template <typename T>
+__global__ void __launch_bounds__(B_THREADS) token_logprobs_bwd_kernel(const Bwd p) {
+  constexpr int VE = Vec<T>::N;
+  const long long r = blockIdx.x / p.blocks_per_row;
+  const int blk = int(blockIdx.x - r * p.blocks_per_row);
+  const T* x = reinterpret_cast<const T*>(p.x) + r * p.stride;
+  T* dx = reinterpret_cast<T*>(p.dx) + r * (long long)p.W;
+  const int lead = int((reinterpret_cast<uintptr_t>(dx) & 15) / sizeof(T));
+  const bool same = ((reinterpret_cast<uintptr_t>(x) ^ reinterpret_cast<uintptr_t>(dx)) & 15) == 0;
+  const int n_vec = int(((long long)p.W + lead + VE - 1) / VE);
+  const long long tg = p.target[r];
+  float gl = p.g_lp && tg >= 0 ? p.g_lp[r] : 0.f;
+  if (tg >= p.V) gl = __uint_as_float(0x7fc00000u);
+  const float gh = p.g_h ? p.g_h[r] : 0.f, m = p.norm[r], log_s = p.norm[p.N + r], H = p.entropy[r];
+  const float base = gl + gh * H;
+  uint4 v[B_UNROLL];
+  const int first = blk * B_THREADS * B_UNROLL + threadIdx.x;
+#pragma unroll
+  for (int j = 0; j < B_UNROLL; ++j) {
+    const int i = first + j * B_THREADS, e0 = i * VE - lead;
+    if (i < n_vec && same && e0 >= 0 && e0 + VE <= p.V) v[j] = __ldg(reinterpret_cast<const uint4*>(x + e0));
+  }
+#pragma unroll
+  for (int j = 0; j < B_UNROLL; ++j) {
+    const int i = first + j * B_THREADS, e0 = i * VE - lead;
+    if (i >= n_vec) continue;
+    const bool whole = e0 >= 0 && e0 + VE <= p.W;
+    float f[VE];
+    if (same && e0 >= 0 && e0 + VE <= p.V) {
+      Vec<T>::unpack(v[j], f);
+    } else {
+#pragma unroll
+      for (int q = 0; q < VE; ++q) f[q] = (e0 + q >= 0 && e0 + q < p.V) ? Vec<T>::load(x + e0 + q) : -INFINITY;
+    }
+#pragma unroll
+    for (int q = 0; q < VE; ++q) {
+      const float lp = fmaxf((f[q] - m) - log_s, FLOOR);        // a probability of 0 contributes 0, not 0 * inf
+      const float pr = exp2f(lp * L2E);
+      float g = -pr * fmaf(gh, lp, base);
+      if (e0 + q == tg) g += gl;
+      f[q] = e0 + q < p.V ? (m != m ? m : g) : 0.f;       // fmaxf drops a NaN: a row without a distribution has no gradient
+    }
+    if (whole) {
+      *reinterpret_cast<uint4*>(dx + e0) = Vec<T>::pack(f);
+    } else {
+#pragma unroll
+      for (int q = 0; q < VE; ++q)
+        if (e0 + q >= 0 && e0 + q < p.W) dx[e0 + q] = T(f[q]);
+    }
+  }
+}
+
+template <typename T>
+int launch_fwd(Fwd p, cudaStream_t stream) {
+  // Slices: as many CTAs per row (1, 2, 4, 8) as keep two CTAs on each of the 148 SMs, but at least 32 KB of logits each.
+  int cs = 1;
+  while (cs < 8 && (long long)p.N * cs * 2 <= 2 * sm_count() && (long long)p.V * int(sizeof(T)) >= (long long)cs * 2 * 32768) cs *= 2;
+  const long long n_vec = ((long long)p.V + 2 * Vec<T>::N) / Vec<T>::N + 1;
+  const long long chunks = (n_vec / cs + 1 + THREADS * UNROLL - 1) / (THREADS * UNROLL) + 1;
+  p.chunks_per_run = int((chunks * THREADS + MAX_RUNS - 1) / MAX_RUNS);
+  const long long runs = (chunks + p.chunks_per_run - 1) / p.chunks_per_run + 1;
+  const size_t smem = sizeof(Shared) + (p.k ? size_t(runs) * THREADS * 4 : 0);
+  static std::mutex lock;
+  static size_t configured[64] = {};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev >= 64) return -91;
+  {
+    std::lock_guard<std::mutex> guard(lock);
+    if (smem > configured[dev]) {
+      if (cudaFuncSetAttribute(token_logprobs_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem)) != cudaSuccess) return -92;
+      configured[dev] = smem;
+    }
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(unsigned(p.N) * cs);
+  cfg.blockDim = dim3(THREADS);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = cs;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if (cudaLaunchKernelEx(&cfg, token_logprobs_kernel<T>, p) != cudaSuccess) {
+    LYRA_CHECK_LAUNCH();
+    return -93;
+  }
+  return 0;
+}
+
+template <typename T>
+int launch_bwd(Bwd p, cudaStream_t stream) {
+  const long long n_vec = ((long long)p.W + 2 * Vec<T>::N - 2) / Vec<T>::N;        // the most any alignment of the row needs
+  p.blocks_per_row = int((n_vec + B_THREADS * B_UNROLL - 1) / (B_THREADS * B_UNROLL));
+  const long long blocks = (long long)p.N * p.blocks_per_row;
+  if (blocks > 0x7fffffffLL) return -94;
+  token_logprobs_bwd_kernel<T><<<unsigned(blocks), B_THREADS, 0, stream>>>(p);
+  LYRA_CHECK_LAUNCH();
+  return 0;
+}
+
+}  // namespace tlp
+}  // namespace lyra
+
+// x [N, *] (rows `stride` elements apart, columns 0 .. V - 1 are used), bf16 or fp32; target int64 [N].
+extern "C" int lyra_token_logprobs(const void* x, int is_bf16, const long long* target, float* logprob, float* entropy, float* norm, float* top_lp,
+                                   long long* top_id, int N, int V, int k, long long stride, cudaStream_t stream) {
+  using namespace lyra::tlp;
+  if (N < 1 || N > (1 << 28) || V < 1 || V > (1 << 30) || k < 0 || k > MAX_TOP || k > V || stride < V) return -90;
+  if (reinterpret_cast<uintptr_t>(x) % (is_bf16 ? 2 : 4)) return -90;
+  Fwd p{x, target, logprob, entropy, norm, top_lp, top_id, stride, N, V, k, 1};
+  return is_bf16 ? launch_fwd<__nv_bfloat16>(p, stream) : launch_fwd<float>(p, stream);
+}
+
+// dx [N, W] contiguous (W >= V): gradient of the logits from the gradients of logprob and entropy (either may be null).
+extern "C" int lyra_token_logprobs_bwd(const void* x, int is_bf16, void* dx, const long long* target, const float* norm, const float* entropy,
+                                       const float* g_lp, const float* g_h, int N, int V, int W, long long stride, cudaStream_t stream) {
+  using namespace lyra::tlp;
+  if (N < 1 || V < 1 || W < V || W > (1 << 30) || stride < V) return -90;
+  if (reinterpret_cast<uintptr_t>(x) % (is_bf16 ? 2 : 4) || reinterpret_cast<uintptr_t>(dx) % (is_bf16 ? 2 : 4)) return -90;
+  Bwd p{x, dx, target, norm, entropy, g_lp, g_h, stride, N, V, W, 1};
+  return is_bf16 ? launch_bwd<__nv_bfloat16>(p, stream) : launch_bwd<float>(p, stream);
+}

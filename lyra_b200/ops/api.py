@@ -144,6 +144,22 @@ def linear_cross_entropy(x, w, y, vocab_size: int, reduction: str = "sum", imple
     return ref.linear_cross_entropy(x, w, y, vocab_size, reduction)
 
 
+def token_logprobs(logits, targets, top_k: int = 0, vocab_size: int | None = None, implementation: str = "auto"):
+    """Scores of the tokens ``targets [...]`` (int32 / int64) under ``logits [..., V]`` (fp32 or bf16; columns from ``vocab_size``
+    on are vocabulary padding and take no part): a ``TokenLogprobs`` with the log probability of each target, the entropy of each
+    row, and the ``top_k`` (0..32) most likely tokens with their log probabilities, most likely first, equal logits by lower id.
+
+    ``logprob`` and ``entropy`` are differentiable with respect to ``logits`` (once); the alternatives are not. A negative target
+    marks a position without a token: its log probability is 0 and carries no gradient. A target from ``vocab_size`` on, a row
+    with a NaN or +inf, or one of nothing but -inf, has NaN scores and gradients. A logit of -inf is a token of probability 0."""
+    from lyra_b200.ops import logprobs
+
+    vocab = logprobs.check_arguments(logits, targets, top_k, vocab_size)
+    if use_kernels(logits, implementation):
+        return logprobs.token_logprobs(logits, targets, top_k, vocab)
+    return logprobs.TokenLogprobs(*ref.token_logprobs(logits, targets, top_k, vocab))
+
+
 def embedding(emb, tokens, implementation: str = "auto", presorted: bool = True):
     """Row gather with a deterministic (sorted segment-sum, fp32) gradient (lyra/kernels/embs.py)."""
     if use_kernels(emb, implementation):

@@ -7,6 +7,7 @@ machine ``kernels_available()`` is False and callers use the PyTorch reference i
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import functools
 from pathlib import Path
@@ -69,6 +70,14 @@ def ptr(t: torch.Tensor | None) -> c_void_p:
 
 def stream_ptr() -> c_void_p:
     return c_void_p(torch._C._cuda_getCurrentRawStream(torch.cuda.current_device()))
+
+
+def on_device(t: torch.Tensor):
+    """Context in which ``t``'s GPU is the current one: a launch goes to the current device's stream, which for a tensor of
+    another GPU would be the wrong stream. Free of cost where the device is current already."""
+    if t.device.index == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(t.device)
 
 
 _status: dict[int, torch.Tensor] = {}

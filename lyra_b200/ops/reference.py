@@ -83,6 +83,23 @@ def linear_cross_entropy(x: torch.Tensor, w: torch.Tensor, y: torch.Tensor, voca
     return loss, torch.cat(lses)
 
 
+def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, top_k: int, vocab: int):
+    """``(logprob, entropy, top_logprobs, top_ids)`` of every row of ``logits[..., :vocab]``; see ``ops.api.token_logprobs``."""
+    x = logits[..., :vocab]
+    x = x if x.dtype == torch.float64 else x.float()
+    bad = ~torch.isfinite(x.amax(dim=-1))                      # a NaN, a +inf, or nothing but -inf: no distribution
+    nan = torch.full((), float("nan"), dtype=x.dtype, device=x.device)
+    logp = torch.log_softmax(x, dim=-1)
+    at = targets.long()
+    picked = logp.gather(-1, at.clamp(0, vocab - 1)[..., None])[..., 0]
+    picked = torch.where(at < 0, torch.zeros_like(picked), torch.where(bad | (at >= vocab), nan, picked))
+    entropy = torch.where(bad, nan, -(logp.exp() * logp.clamp(min=-1000.0)).sum(-1))
+    order = torch.sort(x.detach(), dim=-1, descending=True, stable=True).indices[..., :top_k]
+    top = torch.where(bad[..., None], nan, logp.detach().gather(-1, order))
+    out = torch.float64 if x.dtype == torch.float64 else torch.float32
+    return picked.to(out), entropy.to(out), top.to(out), order
+
+
 def grouped_gemm(lhs: torch.Tensor, rhs: torch.Tensor, group_sizes: torch.Tensor, bias: torch.Tensor | None = None) -> torch.Tensor:
     """``out[m] = lhs[m] @ rhs[g(m)]`` for rows sorted by group (lyra/kernels/gemm.py:477-499)."""
     out = lhs.new_empty(lhs.shape[0], rhs.shape[-1])
