@@ -1,0 +1,813 @@
+// A whole pre-norm mixture-of-experts block for the few tokens (1..64) of a decode step, in one persistent cooperative launch:
+//
+//   xn = rms_norm(x) * norm;  logits = xn R + r;  e_1..e_k = top-k of logits, s = softmax over the chosen logits
+//   out = x + rs * sum_j s_j (W_down[e_j]^T a_j + b_down),  a_j = swiglu(W_up[e_j]^T xn + b_up)     (shared experts: s = 1)
+//
+// The work is reading the chosen experts' weights once; every expert is a product with a handful of columns. So the design is
+// about bytes in flight. Each SM holds one CTA; the weights of a phase are cut into equal units (64 x 128 bf16 or 128 x 128
+// e4m3 values: 16 KB), the units are numbered through all chosen experts and dealt to the CTAs in contiguous runs of equal length
+// (experts x column panels rarely divide by 148). A producer warp streams a run through a ring of 16 KB stages (two TMA boxes
+// plus the matching piece of the activations by cp.async, 100-200 KB in flight); eight consumer warps multiply with m16n8k16 MMAs
+// in which the weight columns are the 16 rows and the tokens the 8 columns, 16 columns of the panel per warp. A tcgen05 tile has
+// 128 rows of one operand and its accumulator in TMEM: with one to eight tokens per expert it would wait for the same bytes.
+// Panels that a run boundary cuts are summed through a small fp32 slot per CTA by whichever CTA arrives last, always in CTA order,
+// so the result does not depend on timing.
+//
+//   phase 1  router: logits and row norms from the unrounded input in fp32, split over experts, tokens and input columns
+//   grid barrier; every CTA derives the same choice and row lists on its own
+//   phase 2  up-projection + SwiGLU -> act (bf16);   grid barrier (the first stages of phase 3 are already loading)
+//   phase 3  down-projection; a panel of output columns passes through all experts, scaled by their scores in an fp32 tile
+//
+// Roundings: x * norm is rounded to bf16 for the product (its 1/rms factor is applied to the fp32 sum), the SwiGLU result is
+// rounded to bf16 (both are the operands of bf16 MMAs), the output once at the end. The router sees neither rounding.
+#include <cooperative_groups.h>
+#include <cuda_fp8.h>
+
+#include "../common/sm100.cuh"
+#include "../common/tmap.h"
+
+namespace lyra {
+namespace moeblk {
+
+namespace cg = cooperative_groups;
+
+constexpr int CONSUMERS = 256, THREADS = CONSUMERS + 32;
+constexpr int MAX_F = 64, MAX_N = 256, MAX_ROWS = 512;   // tokens, experts (shared ones included), assignments
+constexpr int W_STAGE = 16384, HALF = 8192;              // bytes of weights per stage; each TMA box fills one half
+constexpr int MAX_STAGES = 12;
+constexpr float L2E = 1.4426950408889634f;
+
+struct Params {
+  const __nv_bfloat16* x;      // [F, C]
+  const float* norm;           // [C]
+  const float* router;         // [C, E]
+  const float* router_bias;    // [E] or null
+  const float* up_scale;       // e4m3: [n, C / up_bk, 2H / up_bn]
+  const float* down_scale;     // e4m3: [n, H / dn_bk, C / dn_bn]
+  const float* up_bias;        // [n, 2H] or null
+  const float* down_bias;      // [n, C] or null
+  __nv_bfloat16* out;          // [F, C]
+  float* scores;               // [F, k]
+  long long* idx;              // [F, k]
+  // workspace
+  float* part_logits;          // [csplit, F, E]
+  float* part_sq;              // [csplit, F]
+  __nv_bfloat16* xs;           // [F, C]  x * norm
+  __nv_bfloat16* act;          // [rows, H]
+  float* slots;                // [grid, 2, F, 128]
+  int* counters;               // [n * up_panels + down_panels]
+  int* status;
+  int F, C, H, E, shared, k, csplit, stages, x_stage, up_bk, up_bn, dn_bk, dn_bn;
+  float eps, beta, limit, residual_scale;
+};
+
+struct Lists {                                    // derived by every CTA from the logits; the same everywhere
+  unsigned long long mask[MAX_N];                 // tokens of each expert
+  float rstd[MAX_F];
+  float score[MAX_ROWS];                          // by row
+  short chosen[MAX_F * 8];
+  float chosen_score[MAX_F * 8];
+  unsigned char tok[MAX_ROWS];                    // token of each row; rows are grouped by expert
+  short expert[MAX_N];                            // active experts in ascending order
+  short base[MAX_N + 1];                          // first row of each active expert
+  int n_active;
+  int last;
+  int abort;
+};
+
+__device__ __forceinline__ void consumer_sync() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src, int bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void cp_arrive(uint32_t bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
+}
+__device__ __forceinline__ void ldsm4t(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
+}
+__device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t e4m3x2_to_bf16x2(uint16_t two) {      // exact: e4m3 has 3 bits of mantissa
+  const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(two, __NV_E4M3);
+  const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h));
+  return pack_bf16(f.x, f.y);
+}
+// Order of the logits: larger first, NaN above +inf (as torch.topk has it), -0 equal to 0; 0 is below every logit.
+__device__ __forceinline__ uint32_t order_key(float v) {
+  if (v != v) return 0xffffffffu;
+  const uint32_t b = __float_as_uint(v + 0.0f);
+  return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
+}
+__device__ __forceinline__ float key_value(uint32_t k) {
+  if (k == 0xffffffffu) return __uint_as_float(0x7fc00000u);
+  return __uint_as_float((k & 0x80000000u) ? (k & 0x7fffffffu) : ~k);
+}
+
+// ------------------------------------------------------------------------------------------------ unit runs
+// U units over G CTAs: CTA c has [U c / G, U (c + 1) / G).
+__device__ __forceinline__ int run_begin(long long U, int c, int G) { return int(U * c / G); }
+__device__ __forceinline__ int owner(long long U, int u, int G) { return int(((long long)(u + 1) * G - 1) / U); }
+
+// ------------------------------------------------------------------------------------------------ phase 1
+constexpr int RT = 4, RE = 8;      // tokens and experts of one router task
+
+__device__ void router_task(const Params& p, int task, float* red) {
+  const int n_es = (p.E + RE - 1) / RE, n_tg = (p.F + RT - 1) / RT;
+  const int es = task % n_es, tg = (task / n_es) % n_tg, cs = task / (n_es * n_tg);
+  const int e0 = es * RE, t0 = tg * RT;
+  const int c0 = int((long long)p.C * cs / p.csplit), c1 = int((long long)p.C * (cs + 1) / p.csplit);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const bool whole = e0 + RE <= p.E && p.E % 4 == 0 && (reinterpret_cast<uintptr_t>(p.router) & 15) == 0;
+  float acc[RT][RE], sq[RT];
+#pragma unroll
+  for (int t = 0; t < RT; ++t) {
+    sq[t] = 0.f;
+#pragma unroll
+    for (int e = 0; e < RE; ++e) acc[t][e] = 0.f;
+  }
+#pragma unroll 2
+  for (int c = c0 + threadIdx.x; c < c1; c += CONSUMERS) {
+    float r[RE];
+    const float* rp = p.router + (long long)c * p.E + e0;
+    if (whole) {
+      const float4 a = __ldg(reinterpret_cast<const float4*>(rp)), b = __ldg(reinterpret_cast<const float4*>(rp) + 1);
+      r[0] = a.x; r[1] = a.y; r[2] = a.z; r[3] = a.w; r[4] = b.x; r[5] = b.y; r[6] = b.z; r[7] = b.w;
+    } else {
+#pragma unroll
+      for (int e = 0; e < RE; ++e) r[e] = e0 + e < p.E ? __ldg(rp + e) : 0.f;
+    }
+    const float w = __ldg(p.norm + c);
+#pragma unroll
+    for (int t = 0; t < RT; ++t) {
+      if (t0 + t < p.F) {
+        const long long at = (long long)(t0 + t) * p.C + c;
+        const float v = __bfloat162float(p.x[at]), s = v * w;
+        sq[t] = fmaf(v, v, sq[t]);
+        if (es == 0) p.xs[at] = __float2bfloat16(s);
+#pragma unroll
+        for (int e = 0; e < RE; ++e) acc[t][e] = fmaf(s, r[e], acc[t][e]);
+      }
+    }
+  }
+  constexpr int NV = RT * RE + RT;
+#pragma unroll
+  for (int t = 0; t < RT; ++t) {
+#pragma unroll
+    for (int e = 0; e <= RE; ++e) {
+      float v = e < RE ? acc[t][e < RE ? e : 0] : sq[t];
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+      if (lane == 0) red[warp * NV + t * (RE + 1) + e] = v;
+    }
+  }
+  consumer_sync();
+  if (threadIdx.x < NV) {
+    float v = 0.f;
+#pragma unroll
+    for (int w = 0; w < CONSUMERS / 32; ++w) v += red[w * NV + threadIdx.x];
+    const int t = threadIdx.x / (RE + 1), e = threadIdx.x % (RE + 1);
+    if (t0 + t < p.F) {
+      if (e < RE) {
+        if (e0 + e < p.E) p.part_logits[((long long)cs * p.F + t0 + t) * p.E + e0 + e] = v;
+      } else if (es == 0) {
+        p.part_sq[cs * p.F + t0 + t] = v;
+      }
+    }
+  }
+  consumer_sync();
+}
+
+// Choice of every token and the experts' row lists, in shared memory.
+__device__ void route(const Params& p, Lists& L) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int n = p.E + p.shared;
+  for (int e = threadIdx.x; e < n; e += CONSUMERS)
+    L.mask[e] = e < p.E ? 0ull : (p.F == 64 ? ~0ull : (1ull << p.F) - 1ull);
+  consumer_sync();
+  for (int f = warp; f < p.F; f += CONSUMERS / 32) {
+    float sq = 0.f;
+    for (int s = 0; s < p.csplit; ++s) sq += __ldcg(p.part_sq + s * p.F + f);
+    const float rstd = rsqrtf(sq / float(p.C) + p.eps);
+    uint32_t key[MAX_N / 32];
+#pragma unroll
+    for (int i = 0; i < MAX_N / 32; ++i) {
+      const int e = i * 32 + lane;
+      key[i] = 0;
+      if (e < p.E) {
+        float v = 0.f;
+        for (int s = 0; s < p.csplit; ++s) v += __ldcg(p.part_logits + ((long long)s * p.F + f) * p.E + e);
+        key[i] = order_key(fmaf(v, rstd, p.router_bias ? __ldg(p.router_bias + e) : 0.f));
+      }
+    }
+    float top = 0.f, den = 0.f, mine = 0.f;
+    int my_e = 0;
+    for (int j = 0; j < p.k; ++j) {
+      uint32_t bk = 0;
+      int be = 0;
+#pragma unroll
+      for (int i = 0; i < MAX_N / 32; ++i)
+        if (key[i] > bk) { bk = key[i]; be = i * 32 + lane; }       // ascending e: the first of equals stays
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) {
+        const uint32_t ok = __shfl_xor_sync(0xffffffffu, bk, o);
+        const int oe = __shfl_xor_sync(0xffffffffu, be, o);
+        if (ok > bk || (ok == bk && oe < be)) { bk = ok; be = oe; }
+      }
+#pragma unroll
+      for (int i = 0; i < MAX_N / 32; ++i)
+        if (i * 32 + lane == be) key[i] = 0;
+      const float v = key_value(bk);
+      if (j == 0) top = v;
+      const float w = exp2f((v - top) * L2E);
+      den += w;
+      if (lane == j) { mine = w; my_e = be; }
+    }
+    if (lane == 0) L.rstd[f] = rstd;
+    if (lane < p.k) {
+      const float s = mine / den;
+      L.chosen[f * 8 + lane] = short(my_e);
+      L.chosen_score[f * 8 + lane] = s;
+      atomicOr(&L.mask[my_e], 1ull << f);
+      if (blockIdx.x == 0) {
+        p.scores[(long long)f * p.k + lane] = s;
+        p.idx[(long long)f * p.k + lane] = my_e;
+      }
+    }
+  }
+  consumer_sync();
+  if (warp == 0) {
+    int active = 0, rows = 0;
+    for (int e0 = 0; e0 < n; e0 += 32) {
+      const int e = e0 + lane;
+      const int c = e < n ? __popcll(L.mask[e]) : 0;
+      const uint32_t have = __ballot_sync(0xffffffffu, c > 0);
+      int incl = c;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int v = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += v;
+      }
+      if (c > 0) {
+        const int a = active + __popc(have & ((1u << lane) - 1u));
+        L.expert[a] = short(e);
+        L.base[a] = short(rows + incl - c);
+      }
+      active += __popc(have);
+      rows += __shfl_sync(0xffffffffu, incl, 31);
+    }
+    if (lane == 0) {
+      L.n_active = active;
+      L.base[active] = short(rows);
+    }
+  }
+  consumer_sync();
+  for (int a = threadIdx.x; a < L.n_active; a += CONSUMERS) {
+    const int e = L.expert[a];
+    unsigned long long m = L.mask[e];
+    for (int r = L.base[a]; m; ++r, m &= m - 1) {
+      const int f = __ffsll(m) - 1;
+      float s = 1.f;
+      if (e < p.E)
+        for (int j = 0; j < p.k; ++j)
+          if (L.chosen[f * 8 + j] == e) s = L.chosen_score[f * 8 + j];
+      L.tok[r] = (unsigned char)f;
+      L.score[r] = s;
+    }
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ the ring
+struct Ring {
+  uint32_t stages_addr;            // shared address of stage 0: [weights 16 KB | activations]
+  uint32_t full, empty;            // barrier arrays
+  int stage_bytes, n;
+  int s = 0;
+  uint32_t ph = 0;
+  __device__ void next() {
+    if (++s == n) { s = 0; ph ^= 1; }
+  }
+};
+
+// A bounded wait ran out: record it and go on. Every later wait of the CTA then returns at once, no copy is started any more, and
+// all warps keep walking the same sequence of barriers to the end of the kernel (its outputs are void, the status word says so).
+struct Giveup {
+  volatile int* flag;
+  int* status;
+  __device__ void operator()(int code) const {
+    if ((threadIdx.x & 31) == 0) {
+      *flag = 1;
+      atomicCAS(status, 0, code);
+    }
+  }
+};
+
+template <bool FP8>
+struct Geo {
+  static constexpr int KT = FP8 ? 128 : 64;       // input rows per unit
+};
+
+// Rows [0, rows) of the activation piece of a unit (KT values each, as KT / 64 tiles of 128-byte rows, 128B swizzle).
+template <bool FP8, class RowPtr>
+__device__ __forceinline__ void load_acts(uint32_t dst, int lane, int rows, int rows_pad, int k0, int K, RowPtr row_ptr) {
+  constexpr int CH = Geo<FP8>::KT / 8;             // 16-byte chunks per row
+  for (int i = lane; i < rows * CH; i += 32) {
+    const int r = i / CH, c = i % CH;
+    const __nv_bfloat16* src = row_ptr(r);
+    const int kk = k0 + c * 8;
+    const bool in = kk < K;                        // K is a multiple of 8; the rest of the last unit is zero, like the weights there
+    cp16(dst + (c >> 3) * rows_pad * 128 + swz128(r, c & 7), src + (in ? kk : 0), in ? 16 : 0);
+  }
+}
+
+// n_units units of one expert through the ring: this warp's 16 weight columns times NT * 8 tokens, in fp32.
+template <bool FP8, int NT>
+__device__ void multiply(Ring& ring, int n_units, int k0, int rows_pad, const float* scale, int scale_step, int bk, int n_kb, Giveup give, float (&tot)[NT][4]) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int half = warp >> 2, wc = warp & 3;
+  float acc[NT][4];
+#pragma unroll
+  for (int i = 0; i < NT; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) tot[i][j] = acc[i][j] = 0.f;
+  float sc = 0.f, sc_next = 0.f;
+  int kb = 0, left = 0;                            // k-16 steps left in the current scale block
+  if (FP8) {
+    kb = k0 / bk;
+    left = (bk - (k0 - kb * bk)) / 16;
+    sc = __ldg(scale + (long long)kb * scale_step);
+    if (kb + 1 < n_kb) sc_next = __ldg(scale + (long long)(kb + 1) * scale_step);
+  }
+  for (int u = 0; u < n_units; ++u) {
+    if (!mbar_wait(ring.full + ring.s * 8, ring.ph, give.flag)) give(STATUS_TIMEOUT_FULL);
+    const uint32_t w = ring.stages_addr + ring.s * ring.stage_bytes + half * HALF;
+    const uint32_t xa = ring.stages_addr + ring.s * ring.stage_bytes + W_STAGE;
+    constexpr int STEPS = Geo<FP8>::KT / 32;       // two k-16 MMAs per step
+#pragma unroll
+    for (int st = 0; st < STEPS; ++st) {
+      uint32_t a[2][4];
+      if (FP8) {
+        uint32_t raw[4];
+        const int k = st * 32 + lane;
+        ldsm4t(raw, w + k * 64 + ((wc ^ ((k >> 1) & 3)) << 4));
+        // raw[j]: k = 8j + 2 (lane % 4) in the low half, k + 1 in the high half; columns 2 (lane / 4) and + 1 as the two bytes
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const uint32_t t = __byte_perm(raw[j], 0, 0x3120);
+          a[j >> 1][(j & 1) * 2] = e4m3x2_to_bf16x2(uint16_t(t & 0xffffu));
+          a[j >> 1][(j & 1) * 2 + 1] = e4m3x2_to_bf16x2(uint16_t(t >> 16));
+        }
+      } else {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int k = st * 32 + h * 16 + ((lane >> 4) << 3) + (lane & 7);
+          ldsm4t(a[h], w + swz128(k, wc * 2 + ((lane >> 3) & 1)));
+        }
+      }
+      const uint32_t xt = xa + (st >> 1) * rows_pad * 128;
+      uint32_t b[NT][4];
+#pragma unroll
+      for (int i = 0; i < NT; ++i) ldsm4(b[i], xt + i * 1024 + swz128(lane & 7, (st & 1) * 4 + (lane >> 3)));
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        if (FP8 && left == 0) {                    // a new scale block begins here
+#pragma unroll
+          for (int i = 0; i < NT; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              tot[i][j] = fmaf(acc[i][j], sc, tot[i][j]);
+              acc[i][j] = 0.f;
+            }
+          sc = sc_next;
+          ++kb;
+          left = bk / 16;
+          if (kb + 1 < n_kb) sc_next = __ldg(scale + (long long)(kb + 1) * scale_step);
+        }
+        if (FP8) --left;
+#pragma unroll
+        for (int i = 0; i < NT; ++i) mma16816(FP8 ? acc[i] : tot[i], a[h], b[i][2 * h], b[i][2 * h + 1]);
+      }
+    }
+    __syncwarp();
+    if (lane == 0) mbar_arrive(ring.empty + ring.s * 8);
+    ring.next();
+  }
+  if (FP8) {
+#pragma unroll
+    for (int i = 0; i < NT; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) tot[i][j] = fmaf(acc[i][j], sc, tot[i][j]);
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ the kernel
+template <bool FP8>
+struct Block {
+  static constexpr int KT = Geo<FP8>::KT;
+  const Params& p;
+  Lists& L;
+  Ring ring;
+  float* buf;                       // [F][128] fp32: rows of an expert (phase 2) or tokens (phase 3) times the panel's columns
+  Giveup give;
+  int G, c, rows_pad;
+  int up_panels, up_units, dn_panels, dn_units;    // column panels per matrix, units along the input per panel
+
+  // columns of this thread's accumulators inside the panel (the e4m3 path pairs neighbouring columns, see multiply())
+  __device__ int col(int second) const {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    return warp * 16 + (FP8 ? 2 * (lane >> 2) + second : (lane >> 2) + 8 * second);
+  }
+
+  template <int NT, bool DOWN>
+  __device__ void segment(int a, int panel, int k_unit, int n_units) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int e = L.expert[a], base = L.base[a], cnt = L.base[a + 1] - base;
+    const float* scale = nullptr;
+    int step = 0, bk = 16, n_kb = 0;
+    if (FP8) {
+      const int N = DOWN ? p.C : 2 * p.H, K = DOWN ? p.H : p.C, bn = DOWN ? p.dn_bn : p.up_bn;
+      bk = DOWN ? p.dn_bk : p.up_bk;
+      n_kb = K / bk;
+      step = N / bn;
+      const int first = DOWN ? panel * 128 + warp * 16 : (warp >> 2) * p.H + panel * 64 + (warp & 3) * 16;
+      scale = (DOWN ? p.down_scale : p.up_scale) + (long long)e * n_kb * step + min(first, N - 16) / bn;
+    }
+    float tot[NT][4];
+    multiply<FP8, NT>(ring, n_units, k_unit * KT, rows_pad, scale, step, bk, n_kb, give, tot);
+    const int c0 = col(0), c1 = col(1);
+    float b0 = 0.f, b1 = 0.f;
+    if (DOWN && k_unit == 0 && p.down_bias) {      // the run that holds the expert's first unit of this panel adds its bias
+      const int g0 = panel * 128 + c0, g1 = panel * 128 + c1;
+      if (g0 < p.C) b0 = __ldg(p.down_bias + (long long)e * p.C + g0);
+      if (g1 < p.C) b1 = __ldg(p.down_bias + (long long)e * p.C + g1);
+    }
+#pragma unroll
+    for (int i = 0; i < NT; ++i) {
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int r = i * 8 + (lane & 3) * 2 + j;
+        if (r < cnt) {
+          if (DOWN) {
+            const int t = L.tok[base + r];
+            const float s = L.score[base + r];
+            buf[t * 128 + c0] += s * (tot[i][j] + b0);
+            buf[t * 128 + c1] += s * (tot[i][2 + j] + b1);
+          } else {
+            buf[r * 128 + c0] = tot[i][j];
+            buf[r * 128 + c1] = tot[i][2 + j];
+          }
+        }
+      }
+    }
+    __syncwarp();                                  // another lane adds to the same token for the next expert
+  }
+  template <bool DOWN>
+  __device__ void run_segment(int a, int panel, int k_unit, int n_units) {
+    const int cnt = L.base[a + 1] - L.base[a];
+    if (cnt <= 8) segment<1, DOWN>(a, panel, k_unit, n_units);
+    else if (cnt <= 16) segment<2, DOWN>(a, panel, k_unit, n_units);
+    else if (cnt <= 32) segment<4, DOWN>(a, panel, k_unit, n_units);
+    else segment<8, DOWN>(a, panel, k_unit, n_units);
+  }
+
+  // The panel's units [q0, q0 + per) of a phase with U units were shared by several CTAs: publish this CTA's part; true in the
+  // CTA that arrives last, which then adds the parts up in CTA order.
+  __device__ bool publish(long long U, int q, int per, int rows, int* counter, int& first, int& last) {
+    first = owner(U, q * per, G);
+    last = owner(U, q * per + per - 1, G);
+    const int expected = U >= G ? last - first + 1 : per;      // with fewer units than CTAs every unit has a CTA of its own
+    float* slot = slot_of(U, q, per, c);
+    for (int i = threadIdx.x; i < rows * 128; i += CONSUMERS) __stcg(slot + i, buf[i]);
+    __threadfence();
+    consumer_sync();
+    if (threadIdx.x == 0) L.last = atomicAdd(counter, 1) == expected - 1;
+    consumer_sync();
+    if (!L.last) return false;
+    __threadfence();
+    return true;
+  }
+  __device__ float* slot_of(long long U, int q, int per, int cta) const {
+    const int which = run_begin(U, cta, G) / per == q ? 0 : 1;  // a cut panel is the first or the last of a run
+    return p.slots + ((long long)cta * 2 + which) * p.F * 128;
+  }
+  __device__ float collect(long long U, int q, int per, int first, int last, int at) const {
+    float v = 0.f;
+    for (int i = first; i <= last; ++i)
+      if (run_begin(U, i, G) != run_begin(U, i + 1, G)) v += __ldcg(slot_of(U, q, per, i) + at);
+    return v;
+  }
+
+  __device__ void consume_up() {
+    const long long U = (long long)L.n_active * up_panels * up_units;
+    int u = run_begin(U, c, G);
+    const int end = run_begin(U, c + 1, G);
+    while (u < end) {
+      const int q = u / up_units, stop = min(end, (q + 1) * up_units), a = q / up_panels, panel = q % up_panels;
+      run_segment<false>(a, panel, u - q * up_units, stop - u);
+      consumer_sync();
+      const int e = L.expert[a], base = L.base[a], cnt = L.base[a + 1] - base, h0 = panel * 64;
+      const bool whole = stop - u == up_units;
+      int first = 0, last = 0;
+      if (whole || publish(U, q, up_units, cnt, p.counters + e * up_panels + panel, first, last)) {
+        for (int i = threadIdx.x; i < cnt * 64; i += CONSUMERS) {
+          const int r = i >> 6, j = i & 63, h = h0 + j;
+          if (h >= p.H) continue;
+          const float rstd = L.rstd[L.tok[base + r]];
+          float g = rstd * (whole ? buf[r * 128 + j] : collect(U, q, up_units, first, last, r * 128 + j));
+          float l = rstd * (whole ? buf[r * 128 + 64 + j] : collect(U, q, up_units, first, last, r * 128 + 64 + j));
+          if (p.up_bias) {
+            g += __ldg(p.up_bias + (long long)e * 2 * p.H + h);
+            l += __ldg(p.up_bias + (long long)e * 2 * p.H + p.H + h);
+          }
+          // comparisons keep a NaN where fminf / fmaxf would drop it
+          g = g > p.limit ? p.limit : g;
+          l = l > p.limit ? p.limit : (l < -p.limit ? -p.limit : l);
+          const float act = (l + 1.f) * g / (1.f + exp2f(-p.beta * L2E * g));
+          p.act[(long long)(base + r) * p.H + h] = __float2bfloat16(act);
+        }
+      }
+      consumer_sync();
+      u = stop;
+    }
+  }
+
+  __device__ void consume_down() {
+    const int per = L.n_active * dn_units;
+    const long long U = (long long)dn_panels * per;
+    int u = run_begin(U, c, G);
+    const int end = run_begin(U, c + 1, G);
+    while (u < end) {
+      const int q = u / per, stop = min(end, (q + 1) * per);
+      const bool whole = stop - u == per;
+      for (int i = threadIdx.x; i < p.F * 128; i += CONSUMERS) buf[i] = 0.f;
+      consumer_sync();
+      while (u < stop) {
+        const int v = u - q * per, a = v / dn_units, k_unit = v % dn_units;
+        const int n = min(stop - u, dn_units - k_unit);
+        run_segment<true>(a, q, k_unit, n);
+        u += n;
+      }
+      consumer_sync();
+      int first = 0, last = 0;
+      if (whole || publish(U, q, per, p.F, p.counters + (p.E + p.shared) * up_panels + q, first, last)) {
+        for (int i = threadIdx.x; i < p.F * 128; i += CONSUMERS) {
+          const int t = i >> 7, g = q * 128 + (i & 127);
+          if (g >= p.C) continue;
+          const float v = whole ? buf[i] : collect(U, q, per, first, last, i);
+          const long long at = (long long)t * p.C + g;
+          p.out[at] = __float2bfloat16(fmaf(p.residual_scale, v, __bfloat162float(p.x[at])));
+        }
+      }
+      consumer_sync();
+    }
+  }
+
+  // ---- producer side: weights and activations of one unit into the stage of `r`
+  __device__ void load_weights(const Ring& r, const CUtensorMap* map, bool down, int u) const {
+    int e, x0, x1, k;
+    if (down) {
+      const int per = L.n_active * dn_units, q = u / per, v = u % per;
+      e = L.expert[v / dn_units];
+      k = (v % dn_units) * KT;
+      x0 = q * 128;
+      x1 = x0 + 64;
+    } else {
+      const int q = u / up_units;
+      e = L.expert[q / up_panels];
+      k = (u % up_units) * KT;
+      x0 = (q % up_panels) * 64;
+      x1 = p.H + x0;
+    }
+    const uint32_t bar = r.full + r.s * 8, dst = r.stages_addr + r.s * r.stage_bytes;
+    mbar_expect_tx(bar, W_STAGE);
+    tma_load_3d(dst, map, bar, x0, k, e);
+    tma_load_3d(dst + HALF, map, bar, x1, k, e);
+  }
+  __device__ void load_rows(const Ring& r, bool down, int u) const {
+    const int lane = threadIdx.x & 31;
+    const uint32_t dst = r.stages_addr + r.s * r.stage_bytes + W_STAGE;
+    if (down) {
+      const int v = u % (L.n_active * dn_units), a = v / dn_units, base = L.base[a];
+      load_acts<FP8>(dst, lane, L.base[a + 1] - base, rows_pad, (v % dn_units) * KT, p.H, [&](int i) { return p.act + (long long)(base + i) * p.H; });
+    } else {
+      const int a = u / up_units / up_panels, base = L.base[a];
+      load_acts<FP8>(dst, lane, L.base[a + 1] - base, rows_pad, (u % up_units) * KT, p.C, [&](int i) { return p.xs + (long long)L.tok[base + i] * p.C; });
+    }
+    cp_arrive(r.full + r.s * 8);
+  }
+};
+
+template <bool FP8>
+__global__ void __launch_bounds__(THREADS, 1)
+moe_block_kernel(const __grid_constant__ CUtensorMap up_map, const __grid_constant__ CUtensorMap down_map, const Params p) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  const int stage_bytes = W_STAGE + p.x_stage;
+  uint8_t* after = smem + p.stages * stage_bytes;
+  float* buf = reinterpret_cast<float*>(after);
+  Lists& L = *reinterpret_cast<Lists*>(after + p.F * 512);
+  __shared__ uint64_t full[MAX_STAGES], empty[MAX_STAGES];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int G = int(gridDim.x), c = int(blockIdx.x);
+  constexpr int KT = Geo<FP8>::KT;
+  cg::grid_group grid = cg::this_grid();
+
+  Block<FP8> blk{p, L, Ring{smem_u32(smem), smem_u32(full), smem_u32(empty), stage_bytes, p.stages}, buf, Giveup{&L.abort, p.status}, G, c, (p.F + 7) / 8 * 8,
+                 (p.H + 63) / 64, (p.C + KT - 1) / KT, (p.C + 127) / 128, (p.H + KT - 1) / KT};
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < p.stages; ++s) {
+      mbar_init(smem_u32(&full[s]), 1 + 32);       // the weights' expect_tx and one arrival per lane for its copies of activations
+      mbar_init(smem_u32(&empty[s]), CONSUMERS / 32);
+    }
+    L.abort = 0;
+    fence_mbar_init();
+  }
+  __syncthreads();
+
+  // ---- phase 1
+  if (warp < CONSUMERS / 32) {
+    const int n_counters = (p.E + p.shared) * blk.up_panels + blk.dn_panels;
+    for (int i = c * CONSUMERS + threadIdx.x; i < n_counters; i += G * CONSUMERS) p.counters[i] = 0;
+    const int tasks = (p.E + RE - 1) / RE * ((p.F + RT - 1) / RT) * p.csplit;
+    for (int t = c; t < tasks; t += G) router_task(p, t, reinterpret_cast<float*>(smem));
+  } else if (lane == 0) {
+    tma_prefetch_desc(&up_map);
+    tma_prefetch_desc(&down_map);
+  }
+  grid.sync();
+  if (warp < CONSUMERS / 32) route(p, L);
+  // the router's reduction used the stages through the generic proxy; the TMA writes there next
+  fence_proxy_async_smem();
+  __syncthreads();
+
+  // ---- phases 2 and 3
+  if (warp == CONSUMERS / 32) {
+    const long long U2 = (long long)L.n_active * blk.up_panels * blk.up_units, U3 = (long long)blk.dn_panels * L.n_active * blk.dn_units;
+    Ring r = blk.ring;
+    auto load = [&](const CUtensorMap* map, bool down, int u, bool weights, bool rows) {
+      if (weights && !mbar_wait(r.empty + r.s * 8, r.ph ^ 1, blk.give.flag)) blk.give(STATUS_TIMEOUT_EMPTY);
+      __syncwarp();
+      if (!*blk.give.flag) {
+        if (weights && lane == 0) blk.load_weights(r, map, down, u);
+        if (rows) blk.load_rows(r, down, u);
+      }
+      r.next();
+    };
+    for (int u = run_begin(U2, c, G); u < run_begin(U2, c + 1, G); ++u) load(&up_map, false, u, true, true);
+    // the weights of the first units of phase 3 need no barrier: they cross it in flight
+    const int b3 = run_begin(U3, c, G), e3 = run_begin(U3, c + 1, G), early = min(b3 + p.stages, e3);
+    const Ring mark = r;
+    for (int u = b3; u < early; ++u) load(&down_map, true, u, true, false);
+    __syncwarp();
+    grid.sync();
+    const Ring ahead = r;
+    r = mark;
+    for (int u = b3; u < early; ++u) load(&down_map, true, u, false, true);
+    r = ahead;
+    for (int u = early; u < e3; ++u) load(&down_map, true, u, true, true);
+  } else {
+    blk.consume_up();
+    grid.sync();
+    blk.consume_down();
+  }
+  asm volatile("cp.async.wait_all;" ::: "memory");
+  __syncthreads();
+  if (L.abort)
+    for (int i = 0; i < 64; ++i) __nanosleep(1000);   // copies still in flight land before the shared memory is given back
+}
+
+template <bool FP8>
+int launch(const CUtensorMap& up, const CUtensorMap& down, const Params& p, int grid, int smem, cudaStream_t stream) {
+  static std::mutex lock;
+  static int configured[64] = {};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev >= 64) return -101;
+  {
+    std::lock_guard<std::mutex> guard(lock);
+    if (smem > configured[dev]) {
+      if (cudaFuncSetAttribute(moe_block_kernel<FP8>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return -102;
+      configured[dev] = smem;
+    }
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(THREADS);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeCooperative;
+  attr[0].val.cooperative = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if (cudaLaunchKernelEx(&cfg, moe_block_kernel<FP8>, up, down, p) != cudaSuccess) {
+    LYRA_CHECK_LAUNCH();
+    return -103;
+  }
+  return 0;
+}
+
+struct Plan {
+  int grid, csplit, stages, x_stage, smem;
+  long long logits, sq, xs, act, slots, counters, total;      // byte offsets into the workspace
+};
+
+// Grid, ring depth and workspace of a call: functions of the sizes alone.
+inline Plan make_plan(int F, int C, int H, int E, int shared, int k, bool fp8) {
+  Plan q;
+  const int KT = fp8 ? 128 : 64, sms = sm_count();
+  const long long chosen = (long long)(E < F * k ? E : F * k) + shared;
+  const long long up_panels = (H + 63) / 64, dn_panels = (C + 127) / 128;
+  const long long u2 = chosen * up_panels * ((C + KT - 1) / KT), u3 = chosen * dn_panels * ((H + KT - 1) / KT);
+  const long long want = ((u2 > u3 ? u2 : u3) + 1) / 2;        // two units per CTA at least: below that a barrier of more CTAs costs more
+  q.grid = int(want < sms ? (want > 1 ? want : 1) : sms);
+  const int tasks = (E + RE - 1) / RE * ((F + RT - 1) / RT);
+  q.csplit = q.grid / tasks;
+  if (q.csplit > 8) q.csplit = 8;
+  if (q.csplit > C / 128) q.csplit = C / 128;
+  if (q.csplit < 1) q.csplit = 1;
+  q.x_stage = (F + 7) / 8 * 8 * 128 * (KT / 64);
+  const int fixed = 1024 + F * 512 + int(sizeof(Lists));
+  q.stages = (232448 - 1024 - fixed) / (W_STAGE + q.x_stage);  // 227 KB per CTA; the barriers are static
+  if (q.stages > MAX_STAGES) q.stages = MAX_STAGES;
+  q.smem = fixed + q.stages * (W_STAGE + q.x_stage);
+  long long at = 0;
+  auto take = [&](long long bytes) { const long long here = at; at += (bytes + 255) / 256 * 256; return here; };
+  q.logits = take(4LL * q.csplit * F * E);
+  q.sq = take(4LL * q.csplit * F);
+  q.xs = take(2LL * F * C);
+  q.act = take(2LL * F * (k + shared) * H);
+  q.slots = take(4LL * q.grid * 2 * F * 128);
+  q.counters = take(4LL * ((E + shared) * up_panels + dn_panels));
+  q.total = at;
+  return q;
+}
+
+}  // namespace moeblk
+}  // namespace lyra
+
+// Bytes of workspace a call needs (its contents need no initialisation), or a negative code for sizes the kernel does not take.
+extern "C" long long lyra_moe_block_workspace(int F, int C, int H, int E, int shared, int k, int fp8) {
+  using namespace lyra::moeblk;
+  if (F < 1 || F > MAX_F || E < 1 || shared < 0 || E + shared > MAX_N || k < 1 || k > E || k + shared > 8) return -100;
+  const int unit = fp8 ? 16 : 8;
+  if (C < unit || H < unit || C % unit || H % unit || C > (1 << 20) || H > (1 << 20)) return -100;
+  const long long chosen = (long long)(E < F * k ? E : F * k) + shared;
+  if (chosen * ((H + 63) / 64) * ((C + 63) / 64) > (1LL << 30)) return -100;
+  return make_plan(F, C, H, E, shared, k, fp8 != 0).total;
+}
+
+// x, out [F, C] bf16; up [n, C, 2H], down [n, H, C] bf16 or e4m3 with fp32 scales per (bk x bn) block; n = E + shared.
+extern "C" int lyra_moe_block(const void* x, const float* norm, float eps, const float* router, const float* router_bias, const void* up, const float* up_scale,
+                              int up_bk, int up_bn, const float* up_bias, const void* down, const float* down_scale, int dn_bk, int dn_bn,
+                              const float* down_bias, void* out, float* scores, long long* idx, void* workspace, int F, int C, int H, int E, int shared,
+                              int k, int fp8, float beta, float limit, float residual_scale, int* status, cudaStream_t stream) {
+  using namespace lyra;
+  using namespace lyra::moeblk;
+  if (lyra_moe_block_workspace(F, C, H, E, shared, k, fp8) < 0) return -100;
+  if (fp8 && (!up_scale || !down_scale || up_bk % 16 || up_bn % 16 || dn_bk % 16 || dn_bn % 16 || up_bk < 16 || up_bn < 16 || dn_bk < 16 || dn_bn < 16 ||
+              C % up_bk || (2 * H) % up_bn || H % dn_bk || C % dn_bn))
+    return -100;
+  const uintptr_t aligned = reinterpret_cast<uintptr_t>(up) | reinterpret_cast<uintptr_t>(down) | reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(out) |
+                            reinterpret_cast<uintptr_t>(workspace);
+  if (aligned & 15) return -100;
+  const Plan q = make_plan(F, C, H, E, shared, k, fp8 != 0);
+  const uint64_t n = uint64_t(E + shared), esz = fp8 ? 1 : 2;
+  const CUtensorMapDataType dt = fp8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  const CUtensorMapSwizzle swz = fp8 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B;
+  const uint32_t box[3] = {64, uint32_t(fp8 ? 128 : 64), 1};
+  CUtensorMap um, dm;
+  const uint64_t ud[3] = {uint64_t(2 * H), uint64_t(C), n}, us[2] = {uint64_t(2 * H) * esz, uint64_t(2 * H) * C * esz};
+  const uint64_t dd[3] = {uint64_t(C), uint64_t(H), n}, ds[2] = {uint64_t(C) * esz, uint64_t(C) * H * esz};
+  if (make_tmap_cached(&um, up, dt, 3, ud, us, box, swz)) return -104;
+  if (make_tmap_cached(&dm, down, dt, 3, dd, ds, box, swz)) return -104;
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  Params p;
+  p.x = static_cast<const __nv_bfloat16*>(x);
+  p.norm = norm;
+  p.router = router;
+  p.router_bias = router_bias;
+  p.up_scale = up_scale;
+  p.down_scale = down_scale;
+  p.up_bias = up_bias;
+  p.down_bias = down_bias;
+  p.out = static_cast<__nv_bfloat16*>(out);
+  p.scores = scores;
+  p.idx = idx;
+  p.part_logits = reinterpret_cast<float*>(ws + q.logits);
+  p.part_sq = reinterpret_cast<float*>(ws + q.sq);
+  p.xs = reinterpret_cast<__nv_bfloat16*>(ws + q.xs);
+  p.act = reinterpret_cast<__nv_bfloat16*>(ws + q.act);
+  p.slots = reinterpret_cast<float*>(ws + q.slots);
+  p.counters = reinterpret_cast<int*>(ws + q.counters);
+  p.status = status;
+  p.F = F; p.C = C; p.H = H; p.E = E; p.shared = shared; p.k = k;
+  p.csplit = q.csplit; p.stages = q.stages; p.x_stage = q.x_stage;
+  p.up_bk = up_bk; p.up_bn = up_bn; p.dn_bk = dn_bk; p.dn_bn = dn_bn;
+  p.eps = eps; p.beta = beta; p.limit = limit; p.residual_scale = residual_scale;
+  return fp8 ? launch<true>(um, dm, p, q.grid, q.smem, stream) : launch<false>(um, dm, p, q.grid, q.smem, stream);
+}

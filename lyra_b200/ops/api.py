@@ -203,3 +203,29 @@ def moe_experts(xn, scores, indices, w_up, up_bias, w_down, down_bias, beta: flo
     unpermute[order] = torch.arange(order.numel(), device=order.device)
     rows = t[unpermute].reshape(F_, K, C)
     return torch.einsum("fkc,fk->fc", rows.float(), scores.float()).to(xn.dtype)
+
+
+def moe_block(x, norm_scale, eps: float, router, router_bias, w_up, up_bias, w_down, down_bias, k: int, n_shared: int, beta: float, limit: float,
+              residual_scale: float = 1.0, implementation: str = "auto"):
+    """The whole pre-norm mixture-of-experts block for the few tokens of a decode step, without a gradient:
+    ``x + residual_scale * sum_j s_j expert_{e_j}(rms_norm(x))`` over the ``k`` experts with the largest router logits (equal logits:
+    lower index first; scores are the softmax over the chosen logits) and the ``n_shared`` last experts with score 1.
+
+    ``x [F, C]``, ``norm_scale [C]``, ``router [C, E]``, ``router_bias [E]`` or None, ``w_up [E + n_shared, C, 2, H]``, ``w_down [E + n_shared,
+    H, C]`` - tensors, or e4m3 ``QArray``s with 2-D block scales (``w_up`` then ``[E + n_shared, C, 2H]``) - and biases ``[E + n_shared, 2, H]`` /
+    ``[E + n_shared, C]`` or None. Returns ``(out [F, C] in x's dtype, scores [F, k] fp32, indices [F, k] int64)``.
+
+    The router works on the unrounded normalised input in fp32. On a GPU: one kernel for 1..64 tokens of bf16 (``ops.decode.
+    moe_block_supported`` names the shapes), which reads the chosen experts' weights once."""
+    from lyra_b200.nn.quant import QArray, dequantize
+    from lyra_b200.ops import decode
+
+    n, C, H = decode.check_moe_block(x, norm_scale, router, router_bias, w_up, up_bias, w_down, down_bias, k, n_shared)
+    if use_kernels(x, implementation):
+        return decode.moe_block(x, norm_scale, eps, router, router_bias, w_up, up_bias, w_down, down_bias, k, n_shared, beta, limit, residual_scale)
+
+    def expert(e):
+        pick = lambda w: dequantize(QArray(w.qval[e], w.scale[e], w.block), torch.float32) if isinstance(w, QArray) else w[e]
+        return pick(w_up).reshape(C, 2 * H), pick(w_down)
+
+    return ref.moe_block(x, norm_scale, eps, router, router_bias, expert, up_bias, down_bias, n, k, n_shared, beta, limit, residual_scale)

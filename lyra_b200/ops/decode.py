@@ -249,3 +249,101 @@ def decode_moe(xn, scores, indices, w_up, up_bias, w_down, down_bias, beta, limi
     if down_q:
         w_down = dequantize(w_down, BF16)
     return cuda_ops.moe_experts(xn, scores, indices, w_up, up_bias, w_down, down_bias, beta, limit)
+
+
+MOE_BLOCK_MAX_TOKENS = 64
+
+
+def check_moe_block(x, norm_scale, router, router_bias, w_up, up_bias, w_down, down_bias, k: int, n_shared: int) -> tuple[int, int, int]:
+    """Refuses arguments that do not describe a block; returns ``(experts, C, H)``."""
+    if x.ndim != 2 or not x.is_floating_point():
+        raise ValueError(f"x must be a floating-point [tokens, C], got {tuple(x.shape)} {x.dtype}")
+    up, down = (w.qval if isinstance(w, QArray) else w for w in (w_up, w_down))
+    C, n = x.shape[1], up.shape[0]
+    if down.ndim != 3 or down.shape[0] != n or down.shape[2] != C:
+        raise ValueError(f"w_down {tuple(down.shape)} must be [{n}, H, {C}]")
+    H = down.shape[1]
+    want = (n, C, 2 * H) if isinstance(w_up, QArray) else (n, C, 2, H)
+    if tuple(up.shape) != want:
+        raise ValueError(f"w_up {tuple(up.shape)} must be {want}")
+    E = n - n_shared
+    if n_shared < 0 or not 1 <= k <= E:
+        raise ValueError(f"{k} routed choices and {n_shared} shared of {n} experts: k must lie in 1..{E}")
+    for name, t, shape in (("norm_scale", norm_scale, (C,)), ("router", router, (C, E)), ("router_bias", router_bias, (E,)),
+                           ("up_bias", up_bias, (n, 2, H)), ("down_bias", down_bias, (n, C))):
+        if t is not None and tuple(t.shape) != shape:
+            raise ValueError(f"{name} {tuple(t.shape)} must be {shape}")
+    for w in (w_up, w_down):
+        if isinstance(w, QArray):
+            r, c = w.qval.shape[-2:]
+            if len(w.block) != 2 or r % w.block[0] or c % w.block[1] or tuple(w.scale.shape) != (n, r // w.block[0], c // w.block[1]):
+                raise ValueError(f"quantised weights need 2-D blocks that divide them: block {w.block}, scale {tuple(w.scale.shape)}, values {tuple(w.qval.shape)}")
+    tensors = [t for t in (x, norm_scale, router, router_bias, up, up_bias, down, down_bias) if t is not None]
+    if any(t.device != x.device for t in tensors):
+        raise ValueError(f"all arguments must be on {x.device}")
+    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
+        raise ValueError("moe_block has no backward pass: call it under torch.no_grad()")
+    return n, C, H
+
+
+def moe_block_supported(F_: int, C: int, H: int, E: int, n_shared: int, k: int, w_up, w_down) -> bool:
+    """Shapes of the one-kernel block: 1..64 tokens, up to 256 experts, at most 8 experts per token (shared ones included); bf16 (or
+    fp32 masters, through their bf16 copies) with widths that are multiples of 8, or e4m3 for both matrices with widths and blocks
+    that are multiples of 16."""
+    quant = isinstance(w_up, QArray)
+    if quant != isinstance(w_down, QArray):
+        return False
+    if quant and any(w.qval.dtype != torch.float8_e4m3fn or w.block[0] % 16 or w.block[1] % 16 for w in (w_up, w_down)):
+        return False
+    lib = native.kernels()
+    lib.lyra_moe_block_workspace.restype = c_ll
+    return F_ >= 1 and lib.lyra_moe_block_workspace(F_, C, H, E, n_shared, k, int(quant)) >= 0
+
+
+def moe_block(x, norm_scale, eps, router, router_bias, w_up, up_bias, w_down, down_bias, k, n_shared, beta, limit, residual_scale):
+    """CUDA path (``csrc/moe/moe_block.cu``); the arguments have passed :func:`check_moe_block`. The workspace is allocated per call, so
+    calls on several streams and captured graphs never share one."""
+    from lyra_b200.ops import cuda_ops
+
+    F_, C = x.shape
+    n = (w_up.qval if isinstance(w_up, QArray) else w_up).shape[0]
+    H = (w_down.qval if isinstance(w_down, QArray) else w_down).shape[1]
+    E, dev = n - n_shared, x.device
+    scores = torch.empty(F_, k, dtype=torch.float32, device=dev)
+    idx = torch.empty(F_, k, dtype=torch.int64, device=dev)
+    if F_ == 0:
+        return torch.empty_like(x), scores, idx
+    if x.dtype != BF16:
+        raise ValueError(f"moe_block takes bf16 tokens on a GPU, got {x.dtype}")
+    if not moe_block_supported(F_, C, H, E, n_shared, k, w_up, w_down):
+        raise ValueError(f"moe_block does not take {F_} tokens, C {C}, H {H}, {E} + {n_shared} experts, k {k}, weights "
+                         f"{type(w_up).__name__} / {type(w_down).__name__} on a GPU (ops.decode.moe_block_supported)")
+    quant = isinstance(w_up, QArray)
+    with native.on_device(x):
+        if quant:
+            wu, wd = w_up.qval.contiguous(), w_down.qval.contiguous()
+            us, ds = w_up.scale.float().contiguous(), w_down.scale.float().contiguous()
+            blocks = (*w_up.block, *w_down.block)
+        else:
+            wu, wd = cuda_ops.bf16_weight(w_up).contiguous(), cuda_ops.bf16_weight(w_down).contiguous()
+            us = ds = None
+            blocks = (16, 16, 16, 16)
+        f32 = lambda p: None if p is None else cuda_ops.fp32_param(p).contiguous()
+        xc, ns, rw, rb, ub, db = _aligned(x), f32(norm_scale), f32(router), f32(router_bias), f32(up_bias), f32(down_bias)
+        wu, wd = _aligned(wu), _aligned(wd)
+        out = torch.empty(F_, C, dtype=BF16, device=dev)
+        lib = native.kernels()
+        ws = torch.empty(lib.lyra_moe_block_workspace(F_, C, H, E, n_shared, k, int(quant)), dtype=torch.uint8, device=dev)
+        rc = lib.lyra_moe_block(ptr(xc), ptr(ns), c_float(eps), ptr(rw), ptr(rb), ptr(wu), ptr(us), c_int(blocks[0]), c_int(blocks[1]), ptr(ub), ptr(wd),
+                                ptr(ds), c_int(blocks[2]), c_int(blocks[3]), ptr(db), ptr(out), ptr(scores), ptr(idx), ptr(ws), c_int(F_), c_int(C), c_int(H),
+                                c_int(E), c_int(n_shared), c_int(k), c_int(int(quant)), c_float(beta), c_float(limit), c_float(residual_scale),
+                                ptr(native.status_word()), native.stream_ptr())
+    native.check(rc, "lyra_moe_block")
+    native.count_launch()
+    return out, scores, idx
+
+
+def _aligned(t: torch.Tensor) -> torch.Tensor:
+    """Contiguous on a 16-byte boundary (a slice may start off one)."""
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()

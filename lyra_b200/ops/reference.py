@@ -137,6 +137,35 @@ def combine(experts_out: torch.Tensor, scores: torch.Tensor, unpermute_map: torc
     return torch.einsum("fkc,fk->fc", rows.float(), scores.float()).to(experts_out.dtype)
 
 
+def moe_block(x, norm_scale, eps: float, router, router_bias, expert, up_bias, down_bias, n_experts: int, k: int, n_shared: int, beta: float, limit: float,
+              residual_scale: float):
+    """Whole pre-norm mixture-of-experts block over ``x [F, C]`` in fp32 (fp64 for fp64 inputs), rounded once at the end; see
+    ``ops.api.moe_block``. ``expert(e)`` gives the two weight matrices ``[C, 2H]`` and ``[H, C]`` of expert ``e``."""
+    dt = torch.float64 if x.dtype == torch.float64 else torch.float32
+    F_, E = x.shape[0], n_experts - n_shared
+    xf = x.to(dt)
+    xn = xf * torch.rsqrt(xf.pow(2).mean(-1, keepdim=True) + eps) * norm_scale.to(dt)
+    logits = xn @ router.to(dt)
+    if router_bias is not None:
+        logits = logits + router_bias.to(dt)
+    vals, idx = softcap_free_topk(logits, k)
+    scores = torch.softmax(vals, dim=-1)
+    mixed = torch.zeros_like(xf)
+    for e in [*torch.unique(idx).tolist(), *range(E, n_experts)]:
+        hit = idx == e
+        rows = hit.any(-1).nonzero()[:, 0] if e < E else torch.arange(F_, device=x.device)
+        weight = (scores * hit).sum(-1)[rows] if e < E else scores.new_ones(F_)
+        w_up, w_down = expert(e)
+        t = xn[rows] @ w_up.to(dt)
+        if up_bias is not None:
+            t = t + up_bias[e].reshape(-1).to(dt)
+        y = swiglu(t.reshape(t.shape[0], 2, -1), beta, limit) @ w_down.to(dt)
+        if down_bias is not None:
+            y = y + down_bias[e].to(dt)
+        mixed[rows] += weight[:, None] * y
+    return (xf + residual_scale * mixed).to(x.dtype), scores, idx
+
+
 def embedding_grad(tokens: torch.Tensor, grad: torch.Tensor, vocab: int) -> torch.Tensor:
     """Deterministic embedding gradient: sort token ids, segment-sum in fp32 (lyra/kernels/embs.py:22-29)."""
     flat = tokens.reshape(-1).long()
