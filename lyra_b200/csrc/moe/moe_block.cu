@@ -31,10 +31,11 @@ namespace moeblk {
 
 namespace cg = cooperative_groups;
 
-constexpr int CONSUMERS = 256, THREADS = CONSUMERS + 32;
+constexpr int CONSUMERS = 256, THREADS = CONSUMERS + 64;   // + a warp that copies weights and one that copies activations
 constexpr int MAX_F = 64, MAX_N = 256, MAX_ROWS = 512;   // tokens, experts (shared ones included), assignments
 constexpr int W_STAGE = 16384, HALF = 8192;              // bytes of weights per stage; each TMA box fills one half
 constexpr int MAX_STAGES = 12;
+constexpr int MAX_CSPLIT = 8;                            // pieces of the input width in the router
 constexpr float L2E = 1.4426950408889634f;
 
 struct Params {
@@ -110,17 +111,54 @@ __device__ __forceinline__ float key_value(uint32_t k) {
 }
 
 // ------------------------------------------------------------------------------------------------ unit runs
-// U units over G CTAs: CTA c has [U c / G, U (c + 1) / G).
-__device__ __forceinline__ int run_begin(long long U, int c, int G) { return int(U * c / G); }
-__device__ __forceinline__ int owner(long long U, int u, int G) { return int(((long long)(u + 1) * G - 1) / U); }
+// U units over G CTAs in contiguous runs: the first U % G CTAs take one unit more (with U < G the first U CTAs take one each).
+struct Runs {
+  int per, rem;
+  __device__ Runs(int U, int G) : per(U / G), rem(U % G) {}
+  __device__ int begin(int c) const { return c * per + min(c, rem); }
+  __device__ int owner(int u) const {
+    const int wide = rem * (per + 1);
+    return u < wide ? u / (per + 1) : rem + (u - wide) / per;
+  }
+};
 
 // ------------------------------------------------------------------------------------------------ phase 1
-constexpr int RT = 4, RE = 8;      // tokens and experts of one router task
+constexpr int RT = 8, RE = 8;      // tokens and experts of one router task
+constexpr int NV = RT * (RE + 1);  // sums of a task: logits and squares
+
+template <int T, bool WHOLE>
+__device__ __forceinline__ void router_dots(const Params& p, int e0, int t0, int c0, int c1, float (&acc)[RT][RE], float (&sq)[RT]) {
+  const __nv_bfloat16* __restrict__ x = p.x + (long long)t0 * p.C;
+  const float* __restrict__ router = p.router + e0;
+  const float* __restrict__ norm = p.norm;
+#pragma unroll 2
+  for (int c = c0 + threadIdx.x; c < c1; c += CONSUMERS) {
+    float r[RE], v[T];
+    const float* rp = router + (long long)c * p.E;
+    if (WHOLE) {
+      const float4 a = __ldg(reinterpret_cast<const float4*>(rp)), b = __ldg(reinterpret_cast<const float4*>(rp) + 1);
+      r[0] = a.x; r[1] = a.y; r[2] = a.z; r[3] = a.w; r[4] = b.x; r[5] = b.y; r[6] = b.z; r[7] = b.w;
+    } else {
+#pragma unroll
+      for (int e = 0; e < RE; ++e) r[e] = e0 + e < p.E ? __ldg(rp + e) : 0.f;
+    }
+#pragma unroll
+    for (int t = 0; t < T; ++t) v[t] = t0 + t < p.F ? __bfloat162float(__ldg(x + (long long)t * p.C + c)) : 0.f;
+    const float w = __ldg(norm + c);
+#pragma unroll
+    for (int t = 0; t < T; ++t) {
+      sq[t] = fmaf(v[t], v[t], sq[t]);
+      const float s = v[t] * w;
+#pragma unroll
+      for (int e = 0; e < RE; ++e) acc[t][e] = fmaf(s, r[e], acc[t][e]);
+    }
+  }
+}
 
 __device__ void router_task(const Params& p, int task, float* red) {
   const int n_es = (p.E + RE - 1) / RE, n_tg = (p.F + RT - 1) / RT;
   const int es = task % n_es, tg = (task / n_es) % n_tg, cs = task / (n_es * n_tg);
-  const int e0 = es * RE, t0 = tg * RT;
+  const int e0 = es * RE, t0 = tg * RT, n_t = min(RT, p.F - t0);
   const int c0 = int((long long)p.C * cs / p.csplit), c1 = int((long long)p.C * (cs + 1) / p.csplit);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const bool whole = e0 + RE <= p.E && p.E % 4 == 0 && (reinterpret_cast<uintptr_t>(p.router) & 15) == 0;
@@ -131,79 +169,66 @@ __device__ void router_task(const Params& p, int task, float* red) {
 #pragma unroll
     for (int e = 0; e < RE; ++e) acc[t][e] = 0.f;
   }
-#pragma unroll 2
-  for (int c = c0 + threadIdx.x; c < c1; c += CONSUMERS) {
-    float r[RE];
-    const float* rp = p.router + (long long)c * p.E + e0;
-    if (whole) {
-      const float4 a = __ldg(reinterpret_cast<const float4*>(rp)), b = __ldg(reinterpret_cast<const float4*>(rp) + 1);
-      r[0] = a.x; r[1] = a.y; r[2] = a.z; r[3] = a.w; r[4] = b.x; r[5] = b.y; r[6] = b.z; r[7] = b.w;
-    } else {
+  if (n_t == 1) {                                  // one token: four rows of the router in flight per thread instead of eight tokens
+    whole ? router_dots<1, true>(p, e0, t0, c0, c1, acc, sq) : router_dots<1, false>(p, e0, t0, c0, c1, acc, sq);
+  } else {
+    whole ? router_dots<RT, true>(p, e0, t0, c0, c1, acc, sq) : router_dots<RT, false>(p, e0, t0, c0, c1, acc, sq);
+  }
 #pragma unroll
-      for (int e = 0; e < RE; ++e) r[e] = e0 + e < p.E ? __ldg(rp + e) : 0.f;
-    }
-    const float w = __ldg(p.norm + c);
+  for (int t = 0; t < RT; ++t) {
+    if (t < n_t) {
 #pragma unroll
-    for (int t = 0; t < RT; ++t) {
-      if (t0 + t < p.F) {
-        const long long at = (long long)(t0 + t) * p.C + c;
-        const float v = __bfloat162float(p.x[at]), s = v * w;
-        sq[t] = fmaf(v, v, sq[t]);
-        if (es == 0) p.xs[at] = __float2bfloat16(s);
+      for (int e = 0; e <= RE; ++e) {
+        float v = e < RE ? acc[t][e < RE ? e : 0] : sq[t];
 #pragma unroll
-        for (int e = 0; e < RE; ++e) acc[t][e] = fmaf(s, r[e], acc[t][e]);
+        for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+        if (lane == 0) red[warp * NV + t * (RE + 1) + e] = v;
       }
     }
   }
-  constexpr int NV = RT * RE + RT;
-#pragma unroll
-  for (int t = 0; t < RT; ++t) {
-#pragma unroll
-    for (int e = 0; e <= RE; ++e) {
-      float v = e < RE ? acc[t][e < RE ? e : 0] : sq[t];
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-      if (lane == 0) red[warp * NV + t * (RE + 1) + e] = v;
-    }
-  }
   consumer_sync();
-  if (threadIdx.x < NV) {
+  if (threadIdx.x < n_t * (RE + 1)) {
     float v = 0.f;
 #pragma unroll
     for (int w = 0; w < CONSUMERS / 32; ++w) v += red[w * NV + threadIdx.x];
     const int t = threadIdx.x / (RE + 1), e = threadIdx.x % (RE + 1);
-    if (t0 + t < p.F) {
-      if (e < RE) {
-        if (e0 + e < p.E) p.part_logits[((long long)cs * p.F + t0 + t) * p.E + e0 + e] = v;
-      } else if (es == 0) {
-        p.part_sq[cs * p.F + t0 + t] = v;
-      }
+    if (e < RE) {
+      if (e0 + e < p.E) p.part_logits[((long long)cs * p.F + t0 + t) * p.E + e0 + e] = v;
+    } else if (es == 0) {
+      p.part_sq[cs * p.F + t0 + t] = v;
     }
   }
   consumer_sync();
 }
 
 // Choice of every token and the experts' row lists, in shared memory.
-__device__ void route(const Params& p, Lists& L) {
+__device__ void route(const Params& p, Lists& L, float* logits) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int n = p.E + p.shared;
   for (int e = threadIdx.x; e < n; e += CONSUMERS)
     L.mask[e] = e < p.E ? 0ull : (p.F == 64 ? ~0ull : (1ull << p.F) - 1ull);
+  // all partial sums of the router are fetched at once (eight independent loads per thread and round), summed in a fixed order
+  const int cells = p.F * p.E;
+  for (int i = threadIdx.x; i < cells + p.F; i += CONSUMERS) {
+    const float* from = i < cells ? p.part_logits + i : p.part_sq + (i - cells);
+    const int step = i < cells ? cells : p.F;
+    float part[MAX_CSPLIT];
+#pragma unroll
+    for (int s = 0; s < MAX_CSPLIT; ++s) part[s] = s < p.csplit ? __ldcg(from + (long long)s * step) : 0.f;
+    float v = 0.f;
+#pragma unroll
+    for (int s = 0; s < MAX_CSPLIT; ++s) v += part[s];
+    if (i < cells) logits[i] = v;
+    else L.rstd[i - cells] = rsqrtf(v / float(p.C) + p.eps);
+  }
   consumer_sync();
   for (int f = warp; f < p.F; f += CONSUMERS / 32) {
-    float sq = 0.f;
-    for (int s = 0; s < p.csplit; ++s) sq += __ldcg(p.part_sq + s * p.F + f);
-    const float rstd = rsqrtf(sq / float(p.C) + p.eps);
+    const float rstd = L.rstd[f];
     uint32_t key[MAX_N / 32];
 #pragma unroll
     for (int i = 0; i < MAX_N / 32; ++i) {
       const int e = i * 32 + lane;
-      key[i] = 0;
-      if (e < p.E) {
-        float v = 0.f;
-        for (int s = 0; s < p.csplit; ++s) v += __ldcg(p.part_logits + ((long long)s * p.F + f) * p.E + e);
-        key[i] = order_key(fmaf(v, rstd, p.router_bias ? __ldg(p.router_bias + e) : 0.f));
-      }
+      key[i] = e < p.E ? order_key(fmaf(logits[f * p.E + e], rstd, p.router_bias ? __ldg(p.router_bias + e) : 0.f)) : 0u;
     }
     float top = 0.f, den = 0.f, mine = 0.f;
     int my_e = 0;
@@ -228,7 +253,6 @@ __device__ void route(const Params& p, Lists& L) {
       den += w;
       if (lane == j) { mine = w; my_e = be; }
     }
-    if (lane == 0) L.rstd[f] = rstd;
     if (lane < p.k) {
       const float s = mine / den;
       L.chosen[f * 8 + lane] = short(my_e);
@@ -475,37 +499,35 @@ struct Block {
     else segment<8, DOWN>(a, panel, k_unit, n_units);
   }
 
-  // The panel's units [q0, q0 + per) of a phase with U units were shared by several CTAs: publish this CTA's part; true in the
-  // CTA that arrives last, which then adds the parts up in CTA order.
-  __device__ bool publish(long long U, int q, int per, int rows, int* counter, int& first, int& last) {
-    first = owner(U, q * per, G);
-    last = owner(U, q * per + per - 1, G);
-    const int expected = U >= G ? last - first + 1 : per;      // with fewer units than CTAs every unit has a CTA of its own
-    float* slot = slot_of(U, q, per, c);
+  // The units [q per, (q + 1) per) of panel q were shared by the CTAs first .. last: publish this CTA's part; true in the CTA
+  // that arrives last, which then adds the parts up in CTA order. A cut panel is the first or the last of a CTA's run: slot 0 or 1.
+  __device__ bool publish(const Runs& runs, int q, int per, int rows, int* counter, int& first, int& last) {
+    first = runs.owner(q * per);
+    last = runs.owner(q * per + per - 1);
+    float* slot = slot_of(runs, q * per, c);
     for (int i = threadIdx.x; i < rows * 128; i += CONSUMERS) __stcg(slot + i, buf[i]);
     __threadfence();
     consumer_sync();
-    if (threadIdx.x == 0) L.last = atomicAdd(counter, 1) == expected - 1;
+    if (threadIdx.x == 0) L.last = atomicAdd(counter, 1) == last - first;
     consumer_sync();
     if (!L.last) return false;
     __threadfence();
     return true;
   }
-  __device__ float* slot_of(long long U, int q, int per, int cta) const {
-    const int which = run_begin(U, cta, G) / per == q ? 0 : 1;  // a cut panel is the first or the last of a run
-    return p.slots + ((long long)cta * 2 + which) * p.F * 128;
+  __device__ float* slot_of(const Runs& runs, int q0, int cta) const {
+    return p.slots + ((long long)cta * 2 + (runs.begin(cta) >= q0 ? 0 : 1)) * p.F * 128;
   }
-  __device__ float collect(long long U, int q, int per, int first, int last, int at) const {
-    float v = 0.f;
-    for (int i = first; i <= last; ++i)
-      if (run_begin(U, i, G) != run_begin(U, i + 1, G)) v += __ldcg(slot_of(U, q, per, i) + at);
+  __device__ float collect(const Runs& runs, int q0, int first, int last, int at) const {
+    float v = __ldcg(slot_of(runs, q0, first) + at);
+#pragma unroll 4
+    for (int i = first + 1; i <= last; ++i) v += __ldcg(slot_of(runs, q0, i) + at);
     return v;
   }
 
   __device__ void consume_up() {
-    const long long U = (long long)L.n_active * up_panels * up_units;
-    int u = run_begin(U, c, G);
-    const int end = run_begin(U, c + 1, G);
+    const Runs runs(L.n_active * up_panels * up_units, G);
+    int u = runs.begin(c);
+    const int end = runs.begin(c + 1);
     while (u < end) {
       const int q = u / up_units, stop = min(end, (q + 1) * up_units), a = q / up_panels, panel = q % up_panels;
       run_segment<false>(a, panel, u - q * up_units, stop - u);
@@ -513,13 +535,13 @@ struct Block {
       const int e = L.expert[a], base = L.base[a], cnt = L.base[a + 1] - base, h0 = panel * 64;
       const bool whole = stop - u == up_units;
       int first = 0, last = 0;
-      if (whole || publish(U, q, up_units, cnt, p.counters + e * up_panels + panel, first, last)) {
+      if (whole || publish(runs, q, up_units, cnt, p.counters + e * up_panels + panel, first, last)) {
         for (int i = threadIdx.x; i < cnt * 64; i += CONSUMERS) {
           const int r = i >> 6, j = i & 63, h = h0 + j;
           if (h >= p.H) continue;
           const float rstd = L.rstd[L.tok[base + r]];
-          float g = rstd * (whole ? buf[r * 128 + j] : collect(U, q, up_units, first, last, r * 128 + j));
-          float l = rstd * (whole ? buf[r * 128 + 64 + j] : collect(U, q, up_units, first, last, r * 128 + 64 + j));
+          float g = rstd * (whole ? buf[r * 128 + j] : collect(runs, q * up_units, first, last, r * 128 + j));
+          float l = rstd * (whole ? buf[r * 128 + 64 + j] : collect(runs, q * up_units, first, last, r * 128 + 64 + j));
           if (p.up_bias) {
             g += __ldg(p.up_bias + (long long)e * 2 * p.H + h);
             l += __ldg(p.up_bias + (long long)e * 2 * p.H + p.H + h);
@@ -538,9 +560,9 @@ struct Block {
 
   __device__ void consume_down() {
     const int per = L.n_active * dn_units;
-    const long long U = (long long)dn_panels * per;
-    int u = run_begin(U, c, G);
-    const int end = run_begin(U, c + 1, G);
+    const Runs runs(dn_panels * per, G);
+    int u = runs.begin(c);
+    const int end = runs.begin(c + 1);
     while (u < end) {
       const int q = u / per, stop = min(end, (q + 1) * per);
       const bool whole = stop - u == per;
@@ -554,11 +576,11 @@ struct Block {
       }
       consumer_sync();
       int first = 0, last = 0;
-      if (whole || publish(U, q, per, p.F, p.counters + (p.E + p.shared) * up_panels + q, first, last)) {
+      if (whole || publish(runs, q, per, p.F, p.counters + (p.E + p.shared) * up_panels + q, first, last)) {
         for (int i = threadIdx.x; i < p.F * 128; i += CONSUMERS) {
           const int t = i >> 7, g = q * 128 + (i & 127);
           if (g >= p.C) continue;
-          const float v = whole ? buf[i] : collect(U, q, per, first, last, i);
+          const float v = whole ? buf[i] : collect(runs, q * per, first, last, i);
           const long long at = (long long)t * p.C + g;
           p.out[at] = __float2bfloat16(fmaf(p.residual_scale, v, __bfloat162float(p.x[at])));
         }
@@ -567,38 +589,61 @@ struct Block {
     }
   }
 
-  // ---- producer side: weights and activations of one unit into the stage of `r`
-  __device__ void load_weights(const Ring& r, const CUtensorMap* map, bool down, int u) const {
-    int e, x0, x1, k;
-    if (down) {
-      const int per = L.n_active * dn_units, q = u / per, v = u % per;
-      e = L.expert[v / dn_units];
-      k = (v % dn_units) * KT;
-      x0 = q * 128;
-      x1 = x0 + 64;
-    } else {
-      const int q = u / up_units;
-      e = L.expert[q / up_panels];
-      k = (u % up_units) * KT;
-      x0 = (q % up_panels) * 64;
-      x1 = p.H + x0;
-    }
-    const uint32_t bar = r.full + r.s * 8, dst = r.stages_addr + r.s * r.stage_bytes;
-    mbar_expect_tx(bar, W_STAGE);
-    tma_load_3d(dst, map, bar, x0, k, e);
-    tma_load_3d(dst + HALF, map, bar, x1, k, e);
+  // ---- producer side. A cursor walks a run without divisions: a warp that issues a unit every few hundred cycles has no time for
+  // them (with the divisions the producer, not the memory, set the pace: 98 us instead of XX us for one token).
+  struct Cursor {
+    int a, panel, k;
+  };
+  __device__ Cursor at_up(int u) const { return Cursor{u / up_units / up_panels, u / up_units % up_panels, u % up_units}; }
+  __device__ Cursor at_down(int u) const {
+    const int per = L.n_active * dn_units;
+    return Cursor{u % per / dn_units, u / per, u % dn_units};
   }
-  __device__ void load_rows(const Ring& r, bool down, int u) const {
-    const int lane = threadIdx.x & 31;
-    const uint32_t dst = r.stages_addr + r.s * r.stage_bytes + W_STAGE;
+  __device__ void advance(Cursor& w, bool down) const {
     if (down) {
-      const int v = u % (L.n_active * dn_units), a = v / dn_units, base = L.base[a];
-      load_acts<FP8>(dst, lane, L.base[a + 1] - base, rows_pad, (v % dn_units) * KT, p.H, [&](int i) { return p.act + (long long)(base + i) * p.H; });
-    } else {
-      const int a = u / up_units / up_panels, base = L.base[a];
-      load_acts<FP8>(dst, lane, L.base[a + 1] - base, rows_pad, (u % up_units) * KT, p.C, [&](int i) { return p.xs + (long long)L.tok[base + i] * p.C; });
+      if (++w.k == dn_units) {
+        w.k = 0;
+        if (++w.a == L.n_active) { w.a = 0; ++w.panel; }
+      }
+    } else if (++w.k == up_units) {
+      w.k = 0;
+      if (++w.panel == up_panels) { w.panel = 0; ++w.a; }
     }
-    cp_arrive(r.full + r.s * 8);
+  }
+  // `n` units from `w` on: the weights (one lane) or the activations (a warp) of each into the next stage
+  template <bool DOWN>
+  __device__ void feed_weights(Ring& r, const CUtensorMap* map, Cursor& w, int n) const {
+    for (int i = 0; i < n; ++i) {
+      if (!mbar_wait(r.empty + r.s * 8, r.ph ^ 1, give.flag)) give(STATUS_TIMEOUT_EMPTY);
+      if (!*give.flag) {
+        const uint32_t bar = r.full + r.s * 8, dst = r.stages_addr + r.s * r.stage_bytes;
+        const int e = L.expert[w.a], x0 = w.panel * (DOWN ? 128 : 64), x1 = DOWN ? x0 + 64 : p.H + x0;
+        mbar_expect_tx(bar, W_STAGE);
+        tma_load_3d(dst, map, bar, x0, w.k * KT, e);
+        tma_load_3d(dst + HALF, map, bar, x1, w.k * KT, e);
+      }
+      advance(w, DOWN);
+      r.next();
+    }
+  }
+  template <bool DOWN>
+  __device__ void feed_rows(Ring& r, Cursor& w, int n) const {
+    const int lane = threadIdx.x & 31;
+    for (int i = 0; i < n; ++i) {
+      if (!mbar_wait(r.empty + r.s * 8, r.ph ^ 1, give.flag)) give(STATUS_TIMEOUT_EMPTY);
+      __syncwarp();
+      if (!*give.flag) {
+        const uint32_t dst = r.stages_addr + r.s * r.stage_bytes + W_STAGE;
+        const int base = L.base[w.a], cnt = L.base[w.a + 1] - base;
+        if (DOWN)
+          load_acts<FP8>(dst, lane, cnt, rows_pad, w.k * KT, p.H, [&](int j) { return p.act + (long long)(base + j) * p.H; });
+        else
+          load_acts<FP8>(dst, lane, cnt, rows_pad, w.k * KT, p.C, [&](int j) { return p.xs + (long long)L.tok[base + j] * p.C; });
+        cp_arrive(r.full + r.s * 8);
+      }
+      advance(w, DOWN);
+      r.next();
+    }
   }
 };
 
@@ -633,6 +678,7 @@ moe_block_kernel(const __grid_constant__ CUtensorMap up_map, const __grid_consta
   if (warp < CONSUMERS / 32) {
     const int n_counters = (p.E + p.shared) * blk.up_panels + blk.dn_panels;
     for (int i = c * CONSUMERS + threadIdx.x; i < n_counters; i += G * CONSUMERS) p.counters[i] = 0;
+    for (int i = c * CONSUMERS + threadIdx.x; i < p.F * p.C; i += G * CONSUMERS) p.xs[i] = __float2bfloat16(__bfloat162float(p.x[i]) * __ldg(p.norm + i % p.C));
     const int tasks = (p.E + RE - 1) / RE * ((p.F + RT - 1) / RT) * p.csplit;
     for (int t = c; t < tasks; t += G) router_task(p, t, reinterpret_cast<float*>(smem));
   } else if (lane == 0) {
@@ -640,36 +686,33 @@ moe_block_kernel(const __grid_constant__ CUtensorMap up_map, const __grid_consta
     tma_prefetch_desc(&down_map);
   }
   grid.sync();
-  if (warp < CONSUMERS / 32) route(p, L);
+  if (warp < CONSUMERS / 32) route(p, L, reinterpret_cast<float*>(smem));
   // the router's reduction used the stages through the generic proxy; the TMA writes there next
   fence_proxy_async_smem();
   __syncthreads();
 
   // ---- phases 2 and 3
+  const Runs up_runs(L.n_active * blk.up_panels * blk.up_units, G), down_runs(blk.dn_panels * L.n_active * blk.dn_units, G);
+  const int b2 = up_runs.begin(c), n2 = up_runs.begin(c + 1) - b2, b3 = down_runs.begin(c), n3 = down_runs.begin(c + 1) - b3;
   if (warp == CONSUMERS / 32) {
-    const long long U2 = (long long)L.n_active * blk.up_panels * blk.up_units, U3 = (long long)blk.dn_panels * L.n_active * blk.dn_units;
+    // weights: those of the first units of phase 3 need no barrier, they cross it in flight
     Ring r = blk.ring;
-    auto load = [&](const CUtensorMap* map, bool down, int u, bool weights, bool rows) {
-      if (weights && !mbar_wait(r.empty + r.s * 8, r.ph ^ 1, blk.give.flag)) blk.give(STATUS_TIMEOUT_EMPTY);
-      __syncwarp();
-      if (!*blk.give.flag) {
-        if (weights && lane == 0) blk.load_weights(r, map, down, u);
-        if (rows) blk.load_rows(r, down, u);
-      }
-      r.next();
-    };
-    for (int u = run_begin(U2, c, G); u < run_begin(U2, c + 1, G); ++u) load(&up_map, false, u, true, true);
-    // the weights of the first units of phase 3 need no barrier: they cross it in flight
-    const int b3 = run_begin(U3, c, G), e3 = run_begin(U3, c + 1, G), early = min(b3 + p.stages, e3);
-    const Ring mark = r;
-    for (int u = b3; u < early; ++u) load(&down_map, true, u, true, false);
+    const int early = min(p.stages, n3);
+    auto w2 = blk.at_up(b2), w3 = blk.at_down(b3);
+    if (lane == 0) {
+      blk.template feed_weights<false>(r, &up_map, w2, n2);
+      blk.template feed_weights<true>(r, &down_map, w3, early);
+    }
     __syncwarp();
     grid.sync();
-    const Ring ahead = r;
-    r = mark;
-    for (int u = b3; u < early; ++u) load(&down_map, true, u, false, true);
-    r = ahead;
-    for (int u = early; u < e3; ++u) load(&down_map, true, u, true, true);
+    if (lane == 0) blk.template feed_weights<true>(r, &down_map, w3, n3 - early);
+    __syncwarp();
+  } else if (warp == CONSUMERS / 32 + 1) {
+    Ring r = blk.ring;
+    auto w2 = blk.at_up(b2), w3 = blk.at_down(b3);
+    blk.template feed_rows<false>(r, w2, n2);
+    grid.sync();
+    blk.template feed_rows<true>(r, w3, n3);
   } else {
     blk.consume_up();
     grid.sync();
@@ -727,7 +770,7 @@ inline Plan make_plan(int F, int C, int H, int E, int shared, int k, bool fp8) {
   q.grid = int(want < sms ? (want > 1 ? want : 1) : sms);
   const int tasks = (E + RE - 1) / RE * ((F + RT - 1) / RT);
   q.csplit = q.grid / tasks;
-  if (q.csplit > 8) q.csplit = 8;
+  if (q.csplit > MAX_CSPLIT) q.csplit = MAX_CSPLIT;
   if (q.csplit > C / 128) q.csplit = C / 128;
   if (q.csplit < 1) q.csplit = 1;
   q.x_stage = (F + 7) / 8 * 8 * 128 * (KT / 64);

@@ -124,23 +124,24 @@ def test_refusals():
 @pytest.mark.parametrize("G", [1, 2, 5, 64, 148])
 @pytest.mark.parametrize("per", [1, 3, 45])
 def test_unit_runs(U, G, per):
-    """The kernel's bookkeeping restated: contiguous runs cover every unit once, ``owner`` finds them, the CTAs that share a panel are
-    as many as the last arriver waits for, and no CTA needs a third slot for a cut panel."""
+    """The kernel's bookkeeping restated: contiguous runs cover every unit once, ``owner`` finds them, the CTAs ``first .. last`` that the
+    last arriver of a panel waits for all have a part of it, and no CTA needs a third slot for a cut panel."""
     U = U * per
-    begin = [U * c // G for c in range(G + 1)]
-    owner = lambda u: ((u + 1) * G - 1) // U
+    size, rem = U // G, U % G
+    begin = [c * size + min(c, rem) for c in range(G + 1)]
+    wide = rem * (size + 1)
+    owner = lambda u: u // (size + 1) if u < wide else rem + (u - wide) // size
     assert begin[0] == 0 and begin[G] == U
     for u in range(0, U, max(1, U // 997)):
         c = owner(u)
         assert begin[c] <= u < begin[c + 1]
     cut = {c: [] for c in range(G)}
     for q in range(0, U // per, max(1, U // per // 499)):
-        first, last = owner(q * per), owner(q * per + per - 1)
-        sharing = [c for c in range(first, last + 1) if begin[c] != begin[c + 1]]
-        assert len(sharing) == (last - first + 1 if U >= G else per)
-        for c in sharing:
+        for c in range(owner(q * per), owner(q * per + per - 1) + 1):
+            assert begin[c] < (q + 1) * per and q * per < begin[c + 1] and begin[c] != begin[c + 1]
             if not (begin[c] <= q * per and (q + 1) * per <= begin[c + 1]):
-                cut[c].append(0 if begin[c] // per == q else 1)
+                cut[c].append(0 if begin[c] >= q * per else 1)
+                assert (begin[c] // per == q) == (cut[c][-1] == 0)
     assert all(len(slots) == len(set(slots)) <= 2 for slots in cut.values())
 
 
