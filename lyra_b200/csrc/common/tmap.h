@@ -31,7 +31,8 @@ inline EncodeTiledFn get_encode_fn() {
 // rank-N tiled map over a row-major tensor. dims[0] is the innermost (contiguous) extent.
 // strides_bytes[i] is the byte stride of dims[i+1]. Returns 0 on success.
 inline int make_tmap(CUtensorMap* out, const void* base, CUtensorMapDataType dt, int rank, const uint64_t* dims,
-                     const uint64_t* strides_bytes, const uint32_t* box, CUtensorMapSwizzle swz) {
+                     const uint64_t* strides_bytes, const uint32_t* box, CUtensorMapSwizzle swz,
+                     CUtensorMapL2promotion promotion = CU_TENSOR_MAP_L2_PROMOTION_L2_256B) {
   EncodeTiledFn fn = get_encode_fn();
   if (!fn) return -1;
   cuuint64_t d[5];
@@ -44,7 +45,7 @@ inline int make_tmap(CUtensorMap* out, const void* base, CUtensorMapDataType dt,
   }
   for (int i = 0; i + 1 < rank; ++i) s[i] = strides_bytes[i];
   CUresult r = fn(out, dt, rank, const_cast<void*>(base), d, s, b, e, CU_TENSOR_MAP_INTERLEAVE_NONE, swz,
-                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+                  promotion, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) {
     fprintf(stderr, "[lyra_b200] cuTensorMapEncodeTiled failed: %d (rank %d dims %llu,%llu box %u,%u stride %llu)\n", int(r), rank,
             (unsigned long long)dims[0], (unsigned long long)(rank > 1 ? dims[1] : 0), box[0], rank > 1 ? box[1] : 0,
@@ -61,7 +62,7 @@ struct TmapKey {
   const void* base;
   uint64_t dims[5], strides[4];
   uint32_t box[5];
-  int dt, rank, swz;
+  int dt, rank, swz, promotion;
   bool operator==(const TmapKey& o) const { return memcmp(this, &o, sizeof(TmapKey)) == 0; }
 };
 struct TmapKeyHash {
@@ -74,7 +75,8 @@ struct TmapKeyHash {
 };
 
 inline int make_tmap_cached(CUtensorMap* out, const void* base, CUtensorMapDataType dt, int rank, const uint64_t* dims,
-                            const uint64_t* strides_bytes, const uint32_t* box, CUtensorMapSwizzle swz) {
+                            const uint64_t* strides_bytes, const uint32_t* box, CUtensorMapSwizzle swz,
+                            CUtensorMapL2promotion promotion = CU_TENSOR_MAP_L2_PROMOTION_L2_256B) {
   static std::unordered_map<TmapKey, CUtensorMap, TmapKeyHash> cache;
   static std::mutex lock;
   TmapKey key;
@@ -83,6 +85,7 @@ inline int make_tmap_cached(CUtensorMap* out, const void* base, CUtensorMapDataT
   key.dt = int(dt);
   key.rank = rank;
   key.swz = int(swz);
+  key.promotion = int(promotion);
   for (int i = 0; i < rank; ++i) {
     key.dims[i] = dims[i];
     key.box[i] = box[i];
@@ -94,7 +97,7 @@ inline int make_tmap_cached(CUtensorMap* out, const void* base, CUtensorMapDataT
     *out = it->second;
     return 0;
   }
-  const int rc = make_tmap(out, base, dt, rank, dims, strides_bytes, box, swz);
+  const int rc = make_tmap(out, base, dt, rank, dims, strides_bytes, box, swz, promotion);
   if (rc == 0) {
     if (cache.size() > (1u << 16)) cache.clear();
     cache.emplace(key, *out);
