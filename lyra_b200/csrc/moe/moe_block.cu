@@ -5,8 +5,9 @@
 //
 // The work is reading the chosen experts' weights once; every expert is a product with a handful of columns. So the design is
 // about bytes in flight and about the order in which memory sees them. Each SM holds one CTA; the weights of a phase are cut into
-// equal units (32 x 256 bf16 or 64 x 256 e4m3 values: 16 KB), the units are numbered through all chosen experts and dealt to the CTAs
-// in contiguous runs of equal length (experts x column panels rarely divide by 148). Two producer warps stream a run through a ring
+// equal units (64 x 256 bf16 or 128 x 256 e4m3 values: 32 KB), the units are numbered through all chosen experts and dealt to the CTAs
+// in contiguous runs of equal length (experts x column panels rarely divide by 148); teams of up to four neighbouring CTAs walk
+// neighbouring panels side by side, so that memory sees longer pieces of each row (a CTA's own piece of a W_up row is 2 x 128 bytes). Two producer warps stream a run through a ring
 // of stages (weights by TMA, the matching piece of the activations by cp.async; 100-190 KB in flight); eight consumer warps multiply
 // with m16n8k16 MMAs in which the weight columns are the 16 rows and the tokens the 8 columns, two tiles of 16 columns per warp - in
 // the up-projection the gate and the linear column of the same hidden units, so SwiGLU happens in registers. A tcgen05 tile has 128
@@ -34,8 +35,8 @@ namespace cg = cooperative_groups;
 
 constexpr int CONSUMERS = 256, THREADS = CONSUMERS + 64;   // + a warp that copies weights and one that copies activations
 constexpr int MAX_F = 64, MAX_N = 256, MAX_ROWS = 512;   // tokens, experts (shared ones included), assignments
-constexpr int W_STAGE = 16384, PANEL = 256;              // bytes of weights per stage, columns per panel
-constexpr int MAX_STAGES = 12;
+constexpr int W_STAGE = 32768, PANEL = 256;              // bytes of weights per stage, columns per panel
+constexpr int MAX_STAGES = 6;
 constexpr int MAX_CSPLIT = 8;                            // pieces of the input width in the router
 constexpr float L2E = 1.4426950408889634f;
 
@@ -60,15 +61,16 @@ struct Params {
   __nv_bfloat16* xs;           // [F, C]  x * norm
   __nv_bfloat16* act;          // [rows, H]
   float* slots;                // [grid, 2, slot_rows(F), 256]
-  int* counters;               // [n * up_panels + down_panels]
+  int* counters;               // [n, up panels]
   int* status;
-  int F, C, H, E, shared, k, csplit, stages, x_stage, up_bk, up_bn, dn_bk, dn_bn;
+  int F, C, H, E, shared, k, csplit, stages, x_stage, up_team, dn_team, up_bk, up_bn, dn_bk, dn_bn;
   float eps, beta, limit, residual_scale;
 };
 
 struct Lists {                                    // derived by every CTA from the logits; the same everywhere
   unsigned long long mask[MAX_N];                 // tokens of each expert
   float rstd[MAX_F];
+  float bias[MAX_N];                              // of the router, fetched before the barrier that the logits wait for
   float score[MAX_ROWS];                          // by row
   short chosen[MAX_F * 8];
   float chosen_score[MAX_F * 8];
@@ -242,7 +244,7 @@ __device__ void route(const Params& p, Lists& L, float* logits) {
 #pragma unroll
     for (int i = 0; i < MAX_N / 32; ++i) {
       const int e = i * 32 + lane;
-      key[i] = e < p.E ? order_key(fmaf(logits[f * p.E + e], rstd, p.router_bias ? __ldg(p.router_bias + e) : 0.f)) : 0u;
+      key[i] = e < p.E ? order_key(fmaf(logits[f * p.E + e], rstd, L.bias[e])) : 0u;
     }
     float top = 0.f, den = 0.f, mine = 0.f;
     int my_e = 0;
@@ -349,20 +351,20 @@ struct Giveup {
 // Tile j of warp w (16 columns): bf16 box 2j + w / 4, columns 16 (w % 4); e4m3 box j, columns 16 w.
 template <bool FP8>
 struct Geo {
-  static constexpr int KT = FP8 ? 64 : 32;         // input rows per unit
+  static constexpr int KT = FP8 ? 128 : 64;        // input rows per unit
   static constexpr int BOX = KT * 128;             // bytes of a box
 };
 
-// Rows [0, rows) of the activation piece of a unit: KT values each, in 128-byte rows with the 128B swizzle (bf16: half of each used).
+// Rows [0, rows) of the activation piece of a unit: KT values each, in KT / 64 tiles of 128-byte rows with the 128B swizzle.
 template <bool FP8, class RowPtr>
-__device__ __forceinline__ void load_acts(uint32_t dst, int lane, int rows, int k0, int K, RowPtr row_ptr) {
+__device__ __forceinline__ void load_acts(uint32_t dst, int lane, int rows, int rows_pad, int k0, int K, RowPtr row_ptr) {
   constexpr int CH = Geo<FP8>::KT / 8;             // 16-byte chunks per row
   for (int i = lane; i < rows * CH; i += 32) {
     const int r = i / CH, c = i % CH;
     const __nv_bfloat16* src = row_ptr(r);
     const int kk = k0 + c * 8;
     const bool in = kk < K;                        // K is a multiple of 8; the rest of the last unit is zero, like the weights there
-    cp16(dst + swz128(r, c), src + (in ? kk : 0), in ? 16 : 0);
+    cp16(dst + (c >> 3) * rows_pad * 128 + swz128(r, c & 7), src + (in ? kk : 0), in ? 16 : 0);
   }
 }
 
@@ -374,7 +376,7 @@ struct Scales {
 
 // n_units units of one expert through the ring: two tiles of 16 weight columns times NT * 8 tokens, in fp32.
 template <bool FP8, int NT>
-__device__ __forceinline__ void multiply(Ring& ring, int n_units, int k0, const Scales& sc, const Giveup& give, float (&tot)[2][NT][4]) {
+__device__ __forceinline__ void multiply(Ring& ring, int n_units, int k0, int rows_pad, const Scales& sc, const Giveup& give, float (&tot)[2][NT][4]) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   float acc[2][NT][4];
 #pragma unroll
@@ -429,7 +431,7 @@ __device__ __forceinline__ void multiply(Ring& ring, int n_units, int k0, const 
         }
       }
 #pragma unroll
-      for (int i = 0; i < NT; ++i) ldsm4(b[i], xa + i * 1024 + swz128(lane & 7, st * 4 + (lane >> 3)));
+      for (int i = 0; i < NT; ++i) ldsm4(b[i], xa + (st >> 1) * rows_pad * 128 + i * 1024 + swz128(lane & 7, (st & 1) * 4 + (lane >> 3)));
       uint32_t a[2][2][4];                         // [tile][k-16 step]
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
@@ -484,8 +486,12 @@ struct Block {
   Ring ring;
   float* buf;                       // [F][256] fp32: the tokens' sums of one panel of output columns (phase 3)
   Giveup give;
-  int G, c;
-  int up_panels, up_units, dn_panels, dn_units;    // column panels per matrix, units along the input per panel
+  int c, rows_pad;
+  // A team of up_team (dn_team) CTAs has one run; its members take neighbouring panels of the same units. up_groups (dn_groups):
+  // panels per matrix in teams; up_units (dn_units): units along the input.
+  int G, up_team, up_groups, up_units, dn_team, dn_groups, dn_units;
+  __device__ Runs up_runs() const { return Runs(L.n_active * up_groups * up_units, G / up_team); }
+  __device__ Runs down_runs() const { return Runs(dn_groups * L.n_active * dn_units, G / dn_team); }
 
   // column of accumulator pair `second` of tile `t` inside the panel (the e4m3 path pairs neighbouring columns, see multiply())
   __device__ static int col(int t, int second) {
@@ -501,9 +507,9 @@ struct Block {
     return Scales{base + min(first, N - 16) / bn, base + min(second, N - 16) / bn, N / bn, bk, K / bk};
   }
 
-  // A cut panel (units [q0, q0 + per)) is the first or the last of a CTA's run: slot 0 or 1 of the CTA.
-  __device__ float* slot_of(const Runs& runs, int q0, int cta) const {
-    return p.slots + ((long long)cta * 2 + (runs.begin(cta) >= q0 ? 0 : 1)) * slot_rows(p.F) * PANEL;
+  // A cut panel (units [q0, q0 + per)) is the first or the last of a team's run: slot 0 or 1 of the team's member.
+  __device__ float* slot_of(const Runs& runs, int q0, int team, int size, int member) const {
+    return p.slots + ((long long)(team * size + member) * 2 + (runs.begin(team) >= q0 ? 0 : 1)) * slot_rows(p.F) * PANEL;
   }
   // After this CTA's part is in its slot: true in the CTA that arrives last of the n that share the panel.
   __device__ bool arrive(int* counter, int n) {
@@ -522,17 +528,17 @@ struct Block {
     const int lane = threadIdx.x & 31;
     const int e = L.expert[a], base = L.base[a], cnt = L.base[a + 1] - base;
     float tot[2][NT][4];
-    multiply<FP8, NT>(ring, n, (u - q0) * KT, scales<false>(e, panel), give, tot);
+    multiply<FP8, NT>(ring, n, (u - q0) * KT, rows_pad, scales<false>(e, panel), give, tot);
     if (n < up_units) {                            // cut: every thread leaves its registers in the slot and picks up the same ones
-      const int first = runs.owner(q0), last = runs.owner(q0 + up_units - 1);
-      float* slot = slot_of(runs, q0, c) + threadIdx.x;
+      const int first = runs.owner(q0), last = runs.owner(q0 + up_units - 1), member = c % up_team;
+      float* slot = slot_of(runs, q0, c / up_team, up_team, member) + threadIdx.x;
 #pragma unroll
       for (int i = 0; i < 2 * NT * 4; ++i) __stcg(slot + i * CONSUMERS, tot[i / (NT * 4)][i / 4 % NT][i % 4]);
-      if (!arrive(p.counters + e * up_panels + panel, last - first + 1)) return;
+      if (!arrive(p.counters + e * up_groups * up_team + panel, last - first + 1)) return;
 #pragma unroll
       for (int i = 0; i < 2 * NT * 4; ++i) tot[i / (NT * 4)][i / 4 % NT][i % 4] = 0.f;
       for (int k = first; k <= last; ++k) {
-        const float* from = slot_of(runs, q0, k) + threadIdx.x;
+        const float* from = slot_of(runs, q0, k, up_team, member) + threadIdx.x;
 #pragma unroll
         for (int i = 0; i < 2 * NT * 4; ++i) tot[i / (NT * 4)][i / 4 % NT][i % 4] += __ldcg(from + i * CONSUMERS);
       }
@@ -570,7 +576,7 @@ struct Block {
     const int lane = threadIdx.x & 31;
     const int e = L.expert[a], base = L.base[a], cnt = L.base[a + 1] - base;
     float tot[2][NT][4];
-    multiply<FP8, NT>(ring, n, k_unit * KT, scales<true>(e, panel), give, tot);
+    multiply<FP8, NT>(ring, n, k_unit * KT, rows_pad, scales<true>(e, panel), give, tot);
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
 #pragma unroll
@@ -592,11 +598,12 @@ struct Block {
   }
 
   __device__ void consume_up() {
-    const Runs runs(L.n_active * up_panels * up_units, G);
-    int u = runs.begin(c);
-    const int end = runs.begin(c + 1);
+    const Runs runs = up_runs();
+    int u = runs.begin(c / up_team);
+    const int end = runs.begin(c / up_team + 1);
     while (u < end) {
-      const int q = u / up_units, q0 = q * up_units, n = min(end, q0 + up_units) - u, a = q / up_panels, panel = q - a * up_panels;
+      const int q = u / up_units, q0 = q * up_units, n = min(end, q0 + up_units) - u, a = q / up_groups;
+      const int panel = (q - a * up_groups) * up_team + c % up_team;
       const int cnt = L.base[a + 1] - L.base[a];
       if (cnt <= 8) up_segment<1>(runs, a, panel, q0, u, n);
       else if (cnt <= 16) up_segment<2>(runs, a, panel, q0, u, n);
@@ -607,12 +614,12 @@ struct Block {
   }
 
   __device__ void consume_down() {
-    const int per = L.n_active * dn_units;
-    const Runs runs(dn_panels * per, G);
-    int u = runs.begin(c);
-    const int end = runs.begin(c + 1);
+    const int per = L.n_active * dn_units, team = c / dn_team, member = c % dn_team;
+    const Runs runs = down_runs();
+    int u = runs.begin(team);
+    const int end = runs.begin(team + 1);
     while (u < end) {
-      const int q = u / per, q0 = q * per, stop = min(end, q0 + per);
+      const int group = u / per, q0 = group * per, stop = min(end, q0 + per), q = group * dn_team + member;
       const bool whole = stop - u == per;
       for (int i = threadIdx.x; i < p.F * PANEL; i += CONSUMERS) buf[i] = 0.f;
       consumer_sync();
@@ -626,53 +633,43 @@ struct Block {
         u += n;
       }
       consumer_sync();
-      bool mine = whole;
-      int first = 0, last = 0;
-      if (!whole) {
-        first = runs.owner(q0);
-        last = runs.owner(q0 + per - 1);
-        float* slot = slot_of(runs, q0, c);
-        for (int i = threadIdx.x; i < p.F * PANEL; i += CONSUMERS) __stcg(slot + i, buf[i]);
-        mine = arrive(p.counters + (p.E + p.shared) * up_panels + q, last - first + 1);
-      }
-      if (mine) {
-        const int g = q * PANEL + int(threadIdx.x);              // 256 threads, 256 columns: thread and column go together
-        if (g < p.C) {
-          for (int t0 = 0; t0 < p.F; t0 += 4) {
-            float v[4] = {0.f, 0.f, 0.f, 0.f};
-            if (whole) {
-#pragma unroll
-              for (int t = 0; t < 4; ++t)
-                if (t0 + t < p.F) v[t] = buf[(t0 + t) * PANEL + threadIdx.x];
-            } else {
-#pragma unroll 4
-              for (int k = first; k <= last; ++k) {
-                const float* from = slot_of(runs, q0, k) + t0 * PANEL + threadIdx.x;
-#pragma unroll
-                for (int t = 0; t < 4; ++t)
-                  if (t0 + t < p.F) v[t] += __ldcg(from + t * PANEL);
-              }
-            }
-#pragma unroll
-            for (int t = 0; t < 4; ++t) {
-              if (t0 + t < p.F) {
-                const long long at = (long long)(t0 + t) * p.C + g;
-                p.out[at] = __float2bfloat16(fmaf(p.residual_scale, v[t], __bfloat162float(p.x[at])));
-              }
-            }
-          }
+      const int g = q * PANEL + int(threadIdx.x);                // 256 threads, 256 columns: thread and column go together
+      if (g < p.C) {
+        float* slot = slot_of(runs, q0, team, dn_team, member) + threadIdx.x;
+        for (int t = 0; t < p.F; ++t) {
+          if (whole) store_out((long long)t * p.C + g, buf[t * PANEL + threadIdx.x]);
+          else __stcg(slot + t * PANEL, buf[t * PANEL + threadIdx.x]);
         }
       }
       consumer_sync();
+    }
+  }
+  __device__ void store_out(long long at, float v) const {
+    p.out[at] = __float2bfloat16(fmaf(p.residual_scale, v, __bfloat162float(p.x[at])));
+  }
+  // After the last barrier: the outputs of cut panels, summed in team order by all CTAs together (the CTA that happened to come
+  // last took 75 us for it at 64 tokens).
+  __device__ void join() const {
+    const int per = L.n_active * dn_units;
+    const Runs runs = down_runs();
+    for (int i = c * THREADS + int(threadIdx.x); i < p.F * p.C; i += G * THREADS) {
+      const int t = i / p.C, g = i - t * p.C, q = g / PANEL, group = q / dn_team, q0 = group * per;
+      const int first = runs.owner(q0), last = runs.owner(q0 + per - 1);
+      if (first == last) continue;
+      const int at = t * PANEL + g % PANEL, member = q % dn_team;
+      float v = 0.f;
+#pragma unroll 8
+      for (int k = first; k <= last; ++k) v += __ldcg(slot_of(runs, q0, k, dn_team, member) + at);
+      store_out(i, v);
     }
   }
 
   // ---- producer side. A cursor walks a run without divisions: a warp that issues a unit every few hundred cycles has no time for
   // them (with the divisions the producer, not the memory, set the pace: 98 us instead of XX us for one token).
   struct Cursor {
-    int a, panel, k;
+    int a, group, k;
   };
-  __device__ Cursor at_up(int u) const { return Cursor{u / up_units / up_panels, u / up_units % up_panels, u % up_units}; }
+  __device__ Cursor at_up(int u) const { return Cursor{u / up_units / up_groups, u / up_units % up_groups, u % up_units}; }
   __device__ Cursor at_down(int u) const {
     const int per = L.n_active * dn_units;
     return Cursor{u % per / dn_units, u / per, u % dn_units};
@@ -681,21 +678,24 @@ struct Block {
     if (down) {
       if (++w.k == dn_units) {
         w.k = 0;
-        if (++w.a == L.n_active) { w.a = 0; ++w.panel; }
+        if (++w.a == L.n_active) { w.a = 0; ++w.group; }
       }
     } else if (++w.k == up_units) {
       w.k = 0;
-      if (++w.panel == up_panels) { w.panel = 0; ++w.a; }
+      if (++w.group == up_groups) { w.group = 0; ++w.a; }
     }
   }
   // `n` units from `w` on: the weights (one lane) or the activations (a warp) of each into the next stage
   template <bool DOWN>
   __device__ void feed_weights(Ring& r, const CUtensorMap* map, Cursor& w, int n) const {
+    const int up_cols = (2 * p.H + 15) / 16 * 16;  // a first column past the matrix, on a 16-byte boundary
     for (int i = 0; i < n; ++i) {
       if (!mbar_wait(r.empty + r.s * 8, r.ph ^ 1, give.flag)) give(STATUS_TIMEOUT_EMPTY);
       if (!*give.flag) {
         const uint32_t bar = r.full + r.s * 8, dst = r.stages_addr + r.s * r.stage_bytes;
-        const int e = L.expert[w.a], x0 = w.panel * (DOWN ? PANEL : 128), x1 = DOWN ? x0 + 128 : p.H + x0;
+        // columns past the matrix (the last panel, a team's surplus member) are out of bounds for the map: zeros without traffic
+        const int e = L.expert[w.a], member = c % (DOWN ? dn_team : up_team), panel = w.group * (DOWN ? dn_team : up_team) + member;
+        const int at = panel * (DOWN ? PANEL : 128), x0 = !DOWN && at >= p.H ? up_cols : at, x1 = DOWN ? x0 + 128 : p.H + at;
         mbar_expect_tx(bar, W_STAGE);
         tma_load_3d(dst, map, bar, x0, w.k * KT, e);
         if (!FP8) tma_load_3d(dst + Geo<FP8>::BOX, map, bar, x0 + 64, w.k * KT, e);
@@ -716,9 +716,9 @@ struct Block {
         const uint32_t dst = r.stages_addr + r.s * r.stage_bytes + W_STAGE;
         const int base = L.base[w.a], cnt = L.base[w.a + 1] - base;
         if (DOWN)
-          load_acts<FP8>(dst, lane, cnt, w.k * KT, p.H, [&](int j) { return p.act + (long long)(base + j) * p.H; });
+          load_acts<FP8>(dst, lane, cnt, rows_pad, w.k * KT, p.H, [&](int j) { return p.act + (long long)(base + j) * p.H; });
         else
-          load_acts<FP8>(dst, lane, cnt, w.k * KT, p.C, [&](int j) { return p.xs + (long long)L.tok[base + j] * p.C; });
+          load_acts<FP8>(dst, lane, cnt, rows_pad, w.k * KT, p.C, [&](int j) { return p.xs + (long long)L.tok[base + j] * p.C; });
         cp_arrive(r.full + r.s * 8);
       }
       advance(w, DOWN);
@@ -742,8 +742,9 @@ moe_block_kernel(const __grid_constant__ CUtensorMap up_map, const __grid_consta
   constexpr int KT = Geo<FP8>::KT;
   cg::grid_group grid = cg::this_grid();
 
-  Block<FP8> blk{p, L, Ring{smem_u32(smem), smem_u32(full), smem_u32(empty), stage_bytes, p.stages}, buf, Giveup{&L.abort, p.status}, G, c,
-                 (p.H + 127) / 128, (p.C + KT - 1) / KT, (p.C + PANEL - 1) / PANEL, (p.H + KT - 1) / KT};
+  Block<FP8> blk{p, L, Ring{smem_u32(smem), smem_u32(full), smem_u32(empty), stage_bytes, p.stages}, buf, Giveup{&L.abort, p.status}, c, (p.F + 7) / 8 * 8,
+                 G, p.up_team, ((p.H + 127) / 128 + p.up_team - 1) / p.up_team, (p.C + KT - 1) / KT,
+                 p.dn_team, ((p.C + PANEL - 1) / PANEL + p.dn_team - 1) / p.dn_team, (p.H + KT - 1) / KT};
   if (threadIdx.x == 0) {
     for (int s = 0; s < p.stages; ++s) {
       mbar_init(smem_u32(&full[s]), 1 + 32);       // the weights' expect_tx and one arrival per lane for its copies of activations
@@ -756,7 +757,8 @@ moe_block_kernel(const __grid_constant__ CUtensorMap up_map, const __grid_consta
 
   // ---- phase 1
   if (warp < CONSUMERS / 32) {
-    const int n_counters = (p.E + p.shared) * blk.up_panels + blk.dn_panels;
+    for (int e = threadIdx.x; e < p.E; e += CONSUMERS) L.bias[e] = p.router_bias ? __ldg(p.router_bias + e) : 0.f;
+    const int n_counters = (p.E + p.shared) * blk.up_groups * blk.up_team;
     for (int i = c * CONSUMERS + threadIdx.x; i < n_counters; i += G * CONSUMERS) p.counters[i] = 0;
     for (int i = c * CONSUMERS + threadIdx.x; i < p.F * p.C; i += G * CONSUMERS) p.xs[i] = __float2bfloat16(__bfloat162float(p.x[i]) * __ldg(p.norm + i % p.C));
     const int tasks = (p.E + RE - 1) / RE * ((p.F + RT - 1) / RT) * p.csplit;
@@ -772,8 +774,9 @@ moe_block_kernel(const __grid_constant__ CUtensorMap up_map, const __grid_consta
   __syncthreads();
 
   // ---- phases 2 and 3
-  const Runs up_runs(L.n_active * blk.up_panels * blk.up_units, G), down_runs(blk.dn_panels * L.n_active * blk.dn_units, G);
-  const int b2 = up_runs.begin(c), n2 = up_runs.begin(c + 1) - b2, b3 = down_runs.begin(c), n3 = down_runs.begin(c + 1) - b3;
+  const Runs up_runs = blk.up_runs(), down_runs = blk.down_runs();
+  const int b2 = up_runs.begin(c / p.up_team), n2 = up_runs.begin(c / p.up_team + 1) - b2;
+  const int b3 = down_runs.begin(c / p.dn_team), n3 = down_runs.begin(c / p.dn_team + 1) - b3;
   if (warp == CONSUMERS / 32) {
     // weights: those of the first units of phase 3 need no barrier, they cross it in flight
     Ring r = blk.ring;
@@ -799,7 +802,8 @@ moe_block_kernel(const __grid_constant__ CUtensorMap up_map, const __grid_consta
     blk.consume_down();
   }
   asm volatile("cp.async.wait_all;" ::: "memory");
-  __syncthreads();
+  grid.sync();
+  blk.join();
   if (L.abort)
     for (int i = 0; i < 64; ++i) __nanosleep(1000);   // copies still in flight land before the shared memory is given back
 }
@@ -835,25 +839,34 @@ int launch(const CUtensorMap& up, const CUtensorMap& down, const Params& p, int 
 }
 
 struct Plan {
-  int grid, csplit, stages, x_stage, smem;
+  int grid, csplit, stages, x_stage, smem, up_team, dn_team;
   long long logits, sq, xs, act, slots, counters, total;      // byte offsets into the workspace
 };
 
 // Grid, ring depth and workspace of a call: functions of the sizes alone.
 inline Plan make_plan(int F, int C, int H, int E, int shared, int k, bool fp8) {
   Plan q;
-  const int KT = fp8 ? 64 : 32, sms = sm_count();
+  const int KT = fp8 ? 128 : 64, sms = sm_count();
   const long long chosen = (long long)(E < F * k ? E : F * k) + shared;
   const long long up_panels = (H + 127) / 128, dn_panels = (C + PANEL - 1) / PANEL;
   const long long u2 = chosen * up_panels * ((C + KT - 1) / KT), u3 = chosen * dn_panels * ((H + KT - 1) / KT);
   const long long want = ((u2 > u3 ? u2 : u3) + 1) / 2;        // two units per CTA at least: below that a barrier of more CTAs costs more
   q.grid = int(want < sms ? (want > 1 ? want : 1) : sms);
+  if (q.grid > 4) q.grid = q.grid / 4 * 4;
+  // Members per team: as many of 4, 2, 1 as divide the grid and leave at most a tenth of the members without a panel.
+  auto team = [&](long long panels) {
+    for (int t = 4; t > 1; t /= 2)
+      if (q.grid % t == 0 && (panels + t - 1) / t * t * 10 <= panels * 11) return t;
+    return 1;
+  };
+  q.up_team = team(up_panels);
+  q.dn_team = team(dn_panels);
   const int tasks = (E + RE - 1) / RE * ((F + RT - 1) / RT);
   q.csplit = q.grid / tasks;
   if (q.csplit > MAX_CSPLIT) q.csplit = MAX_CSPLIT;
   if (q.csplit > C / 128) q.csplit = C / 128;
   if (q.csplit < 1) q.csplit = 1;
-  q.x_stage = (F + 7) / 8 * 8 * 128;
+  q.x_stage = (F + 7) / 8 * 8 * 128 * (KT / 64);
   const int fixed = 1024 + F * PANEL * 4 + int(sizeof(Lists));
   q.stages = (232448 - 1024 - fixed) / (W_STAGE + q.x_stage);  // 227 KB per CTA; the barriers are static
   if (q.stages > MAX_STAGES) q.stages = MAX_STAGES;
@@ -865,7 +878,7 @@ inline Plan make_plan(int F, int C, int H, int E, int shared, int k, bool fp8) {
   q.xs = take(2LL * F * C);
   q.act = take(2LL * F * (k + shared) * H);
   q.slots = take(4LL * q.grid * 2 * slot_rows(F) * PANEL);
-  q.counters = take(4LL * ((E + shared) * up_panels + dn_panels));
+  q.counters = take(4LL * (E + shared) * ((up_panels + q.up_team - 1) / q.up_team * q.up_team));
   q.total = at;
   return q;
 }
@@ -880,7 +893,7 @@ extern "C" long long lyra_moe_block_workspace(int F, int C, int H, int E, int sh
   const int unit = fp8 ? 16 : 8;
   if (C < unit || H < unit || C % unit || H % unit || C > (1 << 20) || H > (1 << 20)) return -100;
   const long long chosen = (long long)(E < F * k ? E : F * k) + shared;
-  if (chosen * ((H + 127) / 128) * ((C + 31) / 32) > (1LL << 30) || chosen * ((C + 255) / 256) * ((H + 31) / 32) > (1LL << 30)) return -100;
+  if (chosen * ((H + 511) / 128) * ((C + 63) / 64) > (1LL << 30) || chosen * ((C + 1023) / 256) * ((H + 63) / 64) > (1LL << 30)) return -100;
   return make_plan(F, C, H, E, shared, k, fp8 != 0).total;
 }
 
@@ -902,7 +915,7 @@ extern "C" int lyra_moe_block(const void* x, const float* norm, float eps, const
   const uint64_t n = uint64_t(E + shared), esz = fp8 ? 1 : 2;
   const CUtensorMapDataType dt = fp8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
   const CUtensorMapSwizzle swz = CU_TENSOR_MAP_SWIZZLE_128B;
-  const uint32_t box[3] = {uint32_t(fp8 ? 128 : 64), uint32_t(fp8 ? 64 : 32), 1};
+  const uint32_t box[3] = {uint32_t(fp8 ? 128 : 64), uint32_t(fp8 ? 128 : 64), 1};
   // 256 bytes of a bf16 row are asked for together; of an e4m3 row of W_up it is 128, and fetching the other half of a 256-byte
   // block early pushes as much out of L2 before it is used (2.9 instead of 3.7 TB/s with narrower boxes)
   const CUtensorMapL2promotion promo = fp8 ? CU_TENSOR_MAP_L2_PROMOTION_L2_128B : CU_TENSOR_MAP_L2_PROMOTION_L2_256B;
@@ -932,7 +945,7 @@ extern "C" int lyra_moe_block(const void* x, const float* norm, float eps, const
   p.counters = reinterpret_cast<int*>(ws + q.counters);
   p.status = status;
   p.F = F; p.C = C; p.H = H; p.E = E; p.shared = shared; p.k = k;
-  p.csplit = q.csplit; p.stages = q.stages; p.x_stage = q.x_stage;
+  p.csplit = q.csplit; p.stages = q.stages; p.x_stage = q.x_stage; p.up_team = q.up_team; p.dn_team = q.dn_team;
   p.up_bk = up_bk; p.up_bn = up_bn; p.dn_bk = dn_bk; p.dn_bn = dn_bn;
   p.eps = eps; p.beta = beta; p.limit = limit; p.residual_scale = residual_scale;
   return fp8 ? launch<true>(um, dm, p, q.grid, q.smem, stream) : launch<false>(um, dm, p, q.grid, q.smem, stream);
