@@ -20,9 +20,13 @@
 //   phase 2  up-projection + SwiGLU -> act (bf16);   grid barrier (the first stages of phase 3 are already loading)
 //   phase 3  down-projection; a panel of output columns passes through all experts, scaled by their scores in an fp32 tile
 //
-// Roundings: x * norm is rounded to bf16 for the product (its 1/rms factor is applied to the fp32 sum), the SwiGLU result is
-// rounded to bf16 (both are the operands of bf16 MMAs), the output once at the end. The router sees neither rounding.
+// Roundings: x * norm is rounded to the MMA's operand type (its 1/rms factor is applied to the fp32 sum), so is the SwiGLU result;
+// the output is rounded once at the end. The router sees neither rounding. The operand type is bf16 for bf16 weights. For e4m3
+// weights it is fp16, into which e4m3 converts in one instruction per pair (by way of bf16 it is four, and the conversions then set
+// the pace: 3.8 instead of XX TB/s); fp16 has three more bits of mantissa and a smaller range, so each token's x * norm is scaled by
+// a power of two that puts its largest value below 2^10, and the SwiGLU result by one that makes its bound (limit + 1) * limit fit.
 #include <cooperative_groups.h>
+#include <cuda_fp16.h>
 #include <cuda_fp8.h>
 
 #include "../common/sm100.cuh"
@@ -37,11 +41,15 @@ constexpr int CONSUMERS = 256, THREADS = CONSUMERS + 64;   // + a warp that copi
 constexpr int MAX_F = 64, MAX_N = 256, MAX_ROWS = 512;   // tokens, experts (shared ones included), assignments
 constexpr int W_STAGE = 32768, PANEL = 256;              // bytes of weights per stage, columns per panel
 constexpr int MAX_STAGES = 6;
+constexpr int SCALE_STAGE = 1024;                        // end of an e4m3 stage: 16 column groups x 8 k-16 steps of fp32 (512 bytes used)
 constexpr int MAX_CSPLIT = 8;                            // pieces of the input width in the router
 constexpr float L2E = 1.4426950408889634f;
 
 // Rows a slot has room for: the accumulators of an expert hold 8, 16, 32 or 64 rows.
 __host__ __device__ inline int slot_rows(int F) { return F <= 8 ? 8 : F <= 16 ? 16 : F <= 32 ? 32 : 64; }
+
+// fp32 tile of a CTA: [F][256] sums in phase 3; before that the router's logits [F][E <= 256] and the reductions of its tasks
+__host__ __device__ inline int buf_bytes(int F) { return (F < 4 ? 4 : F) * PANEL * 4; }
 
 struct Params {
   const __nv_bfloat16* x;      // [F, C]
@@ -58,18 +66,20 @@ struct Params {
   // workspace
   float* part_logits;          // [csplit, F, E]
   float* part_sq;              // [csplit, F]
-  __nv_bfloat16* xs;           // [F, C]  x * norm
-  __nv_bfloat16* act;          // [rows, H]
+  float* gain;                 // [F]  e4m3: what a token's x * norm was divided by
+  uint16_t* xs;                // [F, C]  x * norm in the operand type
+  uint16_t* act;               // [rows, H]
   float* slots;                // [grid, 2, slot_rows(F), 256]
   int* counters;               // [n, up panels]
   int* status;
   int F, C, H, E, shared, k, csplit, stages, x_stage, up_team, dn_team, up_bk, up_bn, dn_bk, dn_bn;
-  float eps, beta, limit, residual_scale;
+  float eps, beta, limit, residual_scale, act_scale, act_gain;     // act_scale: power of two, act_gain its inverse
 };
 
 struct Lists {                                    // derived by every CTA from the logits; the same everywhere
   unsigned long long mask[MAX_N];                 // tokens of each expert
   float rstd[MAX_F];
+  float gain[MAX_F];                              // of the tokens' sums in the up-projection: rstd and the operand's own factor
   float bias[MAX_N];                              // of the router, fetched before the barrier that the logits wait for
   float score[MAX_ROWS];                          // by row
   short chosen[MAX_F * 8];
@@ -86,6 +96,12 @@ __device__ __forceinline__ void consumer_sync() { asm volatile("bar.sync 1, 256;
 __device__ __forceinline__ void cp16(uint32_t dst, const void* src, int bytes) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
+__device__ __forceinline__ void cp4(uint32_t dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void lds128(uint32_t addr, float& a, float& b, float& c, float& d) {
+  asm volatile("ld.shared.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(a), "=f"(b), "=f"(c), "=f"(d) : "r"(addr));
+}
 __device__ __forceinline__ void cp_arrive(uint32_t bar) {
   asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
 }
@@ -100,10 +116,15 @@ __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], 
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ uint32_t e4m3x2_to_bf16x2(uint16_t two) {      // exact: e4m3 has 3 bits of mantissa
+// the same with fp16 operands, into a fresh accumulator
+__device__ __forceinline__ void mma16816_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
+}
+__device__ __forceinline__ uint32_t e4m3x2_to_f16x2(uint16_t two) {       // exact, NaN included
   const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(two, __NV_E4M3);
-  const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h));
-  return pack_bf16(f.x, f.y);
+  return *reinterpret_cast<const uint32_t*>(&h);
 }
 // Order of the logits: larger first, NaN above +inf (as torch.topk has it), -0 equal to 0; 0 is below every logit.
 __device__ __forceinline__ uint32_t order_key(float v) {
@@ -207,6 +228,72 @@ __device__ void router_task(const Params& p, int task, float* red) {
   consumer_sync();
 }
 
+// x * norm of token t in fp16, scaled by a power of two so that its largest value lies in [2^9, 2^10).
+__device__ void operand_row_f16(const Params& p, int t, float* red) {
+  const __nv_bfloat16* x = p.x + (long long)t * p.C;
+  float m = 0.f;
+  for (int c = threadIdx.x; c < p.C; c += CONSUMERS) m = fmaxf(m, fabsf(__bfloat162float(__ldg(x + c)) * __ldg(p.norm + c)));
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = m;
+  consumer_sync();
+  m = red[0];
+#pragma unroll
+  for (int w = 1; w < CONSUMERS / 32; ++w) m = fmaxf(m, red[w]);
+  // exponent arithmetic: 2^(9 - floor(log2 m)); zeros, subnormal sizes and infinities are left as they are
+  const int e = int(__float_as_uint(m) >> 23);
+  const bool usual = e > 30 && e < 254;
+  const float to = usual ? __uint_as_float(uint32_t(254 + 9 - e) << 23) : 1.f, back = usual ? __uint_as_float(uint32_t(e - 9) << 23) : 1.f;
+  for (int c = threadIdx.x; c < p.C; c += CONSUMERS)
+    p.xs[(long long)t * p.C + c] = __half_as_ushort(__float2half_rn(__bfloat162float(__ldg(x + c)) * __ldg(p.norm + c) * to));
+  if (threadIdx.x == 0) p.gain[t] = back;
+  consumer_sync();
+}
+
+// The k experts of every token, a token per warp; NE * 32 >= E.
+template <int NE>
+__device__ __forceinline__ void choose(const Params& p, Lists& L, const float* logits) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  for (int f = warp; f < p.F; f += CONSUMERS / 32) {
+    const float rstd = L.rstd[f];
+    uint32_t key[NE];
+#pragma unroll
+    for (int i = 0; i < NE; ++i) {
+      const int e = i * 32 + lane;
+      key[i] = e < p.E ? order_key(fmaf(logits[f * p.E + e], rstd, L.bias[e])) : 0u;
+    }
+    float top = 0.f, den = 0.f, mine = 0.f;
+    int my_e = 0;
+    for (int j = 0; j < p.k; ++j) {
+      uint32_t bk = key[0];
+      int be = lane;
+#pragma unroll
+      for (int i = 1; i < NE; ++i)
+        if (key[i] > bk) { bk = key[i]; be = i * 32 + lane; }       // ascending e: the first of equals stays
+      const uint32_t best = __reduce_max_sync(0xffffffffu, bk);
+      be = int(__reduce_min_sync(0xffffffffu, bk == best ? uint32_t(be) : 0xffffffffu));
+#pragma unroll
+      for (int i = 0; i < NE; ++i)
+        if (i * 32 + lane == be) key[i] = 0;
+      const float v = key_value(best);
+      if (j == 0) top = v;
+      const float w = exp2f((v - top) * L2E);
+      den += w;
+      if (lane == j) { mine = w; my_e = be; }
+    }
+    if (lane < p.k) {
+      const float s = mine / den;
+      L.chosen[f * 8 + lane] = short(my_e);
+      L.chosen_score[f * 8 + lane] = s;
+      atomicOr(&L.mask[my_e], 1ull << f);
+      if (blockIdx.x == 0) {
+        p.scores[(long long)f * p.k + lane] = s;
+        p.idx[(long long)f * p.k + lane] = my_e;
+      }
+    }
+  }
+}
+
 // Choice of every token and the experts' row lists, in shared memory.
 __device__ void route(const Params& p, Lists& L, float* logits) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -235,51 +322,17 @@ __device__ void route(const Params& p, Lists& L, float* logits) {
 #pragma unroll
     for (int s = 0; s < MAX_CSPLIT; ++s) v += part[s];
     if (i < cells) logits[i] = v;
-    else L.rstd[i - cells] = rsqrtf(v / float(p.C) + p.eps);
+    else {
+      const float rstd = rsqrtf(v / float(p.C) + p.eps);
+      L.rstd[i - cells] = rstd;
+      L.gain[i - cells] = p.up_scale ? rstd * __ldcg(p.gain + i - cells) : rstd;
+    }
   }
   consumer_sync();
-  for (int f = warp; f < p.F; f += CONSUMERS / 32) {
-    const float rstd = L.rstd[f];
-    uint32_t key[MAX_N / 32];
-#pragma unroll
-    for (int i = 0; i < MAX_N / 32; ++i) {
-      const int e = i * 32 + lane;
-      key[i] = e < p.E ? order_key(fmaf(logits[f * p.E + e], rstd, L.bias[e])) : 0u;
-    }
-    float top = 0.f, den = 0.f, mine = 0.f;
-    int my_e = 0;
-    for (int j = 0; j < p.k; ++j) {
-      uint32_t bk = 0;
-      int be = 0;
-#pragma unroll
-      for (int i = 0; i < MAX_N / 32; ++i)
-        if (key[i] > bk) { bk = key[i]; be = i * 32 + lane; }       // ascending e: the first of equals stays
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) {
-        const uint32_t ok = __shfl_xor_sync(0xffffffffu, bk, o);
-        const int oe = __shfl_xor_sync(0xffffffffu, be, o);
-        if (ok > bk || (ok == bk && oe < be)) { bk = ok; be = oe; }
-      }
-#pragma unroll
-      for (int i = 0; i < MAX_N / 32; ++i)
-        if (i * 32 + lane == be) key[i] = 0;
-      const float v = key_value(bk);
-      if (j == 0) top = v;
-      const float w = exp2f((v - top) * L2E);
-      den += w;
-      if (lane == j) { mine = w; my_e = be; }
-    }
-    if (lane < p.k) {
-      const float s = mine / den;
-      L.chosen[f * 8 + lane] = short(my_e);
-      L.chosen_score[f * 8 + lane] = s;
-      atomicOr(&L.mask[my_e], 1ull << f);
-      if (blockIdx.x == 0) {
-        p.scores[(long long)f * p.k + lane] = s;
-        p.idx[(long long)f * p.k + lane] = my_e;
-      }
-    }
-  }
+  if (p.E <= 32) choose<1>(p, L, logits);
+  else if (p.E <= 64) choose<2>(p, L, logits);
+  else if (p.E <= 128) choose<4>(p, L, logits);
+  else choose<8>(p, L, logits);
   consumer_sync();
   if (warp == 0) {
     int active = 0, rows = 0;
@@ -361,77 +414,60 @@ __device__ __forceinline__ void load_acts(uint32_t dst, int lane, int rows, int 
   constexpr int CH = Geo<FP8>::KT / 8;             // 16-byte chunks per row
   for (int i = lane; i < rows * CH; i += 32) {
     const int r = i / CH, c = i % CH;
-    const __nv_bfloat16* src = row_ptr(r);
+    const uint16_t* src = row_ptr(r);
     const int kk = k0 + c * 8;
     const bool in = kk < K;                        // K is a multiple of 8; the rest of the last unit is zero, like the weights there
     cp16(dst + (c >> 3) * rows_pad * 128 + swz128(r, c & 7), src + (in ? kk : 0), in ? 16 : 0);
   }
 }
 
-// Scales of a warp's two column tiles along the input.
-struct Scales {
-  const float *col0, *col1;        // of k block 0
-  int step, bk, n_kb;
-};
-
-// n_units units of one expert through the ring: two tiles of 16 weight columns times NT * 8 tokens, in fp32.
+// n_units units of one expert through the ring: two tiles of 16 weight columns times NT * 8 tokens, in fp32. e4m3: every k-16 product
+// gets a fresh accumulator and joins the total with the scale of its block (a table in the stage, [column group of 16][k-16 step]), so
+// the loop has no branches at the block borders; such a branch after every MMA kept the conversions of neighbouring steps apart.
 template <bool FP8, int NT>
-__device__ __forceinline__ void multiply(Ring& ring, int n_units, int k0, int rows_pad, const Scales& sc, const Giveup& give, float (&tot)[2][NT][4]) {
+__device__ __forceinline__ void multiply(Ring& ring, int n_units, int rows_pad, const Giveup& give, float (&tot)[2][NT][4]) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  float acc[2][NT][4];
 #pragma unroll
   for (int t = 0; t < 2; ++t)
 #pragma unroll
     for (int i = 0; i < NT; ++i)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) tot[t][i][j] = acc[t][i][j] = 0.f;
-  float s0 = 0.f, s1 = 0.f, next0 = 0.f, next1 = 0.f;
-  int kb = 0, left = 0;                            // k-16 steps left in the current scale block
-  auto fetch_next = [&]() {
-    if (kb + 1 < sc.n_kb) {
-      next0 = __ldg(sc.col0 + (long long)(kb + 1) * sc.step);
-      next1 = __ldg(sc.col1 + (long long)(kb + 1) * sc.step);
-    }
-  };
-  auto fold = [&]() {
-#pragma unroll
-    for (int i = 0; i < NT; ++i)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        tot[0][i][j] = fmaf(acc[0][i][j], s0, tot[0][i][j]);
-        tot[1][i][j] = fmaf(acc[1][i][j], s1, tot[1][i][j]);
-        acc[0][i][j] = acc[1][i][j] = 0.f;
-      }
-  };
-  if (FP8) {
-    kb = k0 / sc.bk;
-    left = (sc.bk - (k0 - kb * sc.bk)) / 16;
-    s0 = __ldg(sc.col0 + (long long)kb * sc.step);
-    s1 = __ldg(sc.col1 + (long long)kb * sc.step);
-    fetch_next();
-  }
+      for (int j = 0; j < 4; ++j) tot[t][i][j] = 0.f;
   const uint32_t w_off = FP8 ? 0u : uint32_t(warp >> 2) * Geo<FP8>::BOX;
   constexpr int TILE1 = (FP8 ? 1 : 2) * Geo<FP8>::BOX;
+  constexpr int STEPS = Geo<FP8>::KT / 32;         // two k-16 MMAs per step and tile
   for (int u = 0; u < n_units; ++u) {
     if (!mbar_wait(ring.full + ring.s * 8, ring.ph, give.flag)) give(STATUS_TIMEOUT_FULL);
-    const uint32_t w = ring.stages_addr + ring.s * ring.stage_bytes + w_off;
-    const uint32_t xa = ring.stages_addr + ring.s * ring.stage_bytes + W_STAGE;
-    constexpr int STEPS = Geo<FP8>::KT / 32;       // two k-16 MMAs per step and tile
+    const uint32_t stage = ring.stages_addr + ring.s * ring.stage_bytes, w = stage + w_off, xa = stage + W_STAGE;
+    float sc[2][8];
+    if (FP8) {
 #pragma unroll
-    for (int st = 0; st < STEPS; ++st) {
-      uint32_t raw[2][2][4], b[NT][4];
+      for (int t = 0; t < 2; ++t) {
+        const uint32_t at = stage + ring.stage_bytes - SCALE_STAGE + (t * 8 + warp) * 32;
+        lds128(at, sc[t][0], sc[t][1], sc[t][2], sc[t][3]);
+        lds128(at + 16, sc[t][4], sc[t][5], sc[t][6], sc[t][7]);
+      }
+    }
+    uint32_t raw[2][2][2][4];                      // [step parity][tile][k-16 step (bf16)]: one step ahead of the MMAs
+    auto fetch = [&](int st) {
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
         if (FP8) {
-          ldsm4t(raw[t][0], w + t * TILE1 + swz128(st * 32 + lane, warp));
+          ldsm4t(raw[st & 1][t][0], w + t * TILE1 + swz128(st * 32 + lane, warp));
         } else {
 #pragma unroll
           for (int h = 0; h < 2; ++h)
-            ldsm4t(raw[t][h], w + t * TILE1 + swz128(st * 32 + h * 16 + ((lane >> 4) << 3) + (lane & 7), (warp & 3) * 2 + ((lane >> 3) & 1)));
+            ldsm4t(raw[st & 1][t][h], w + t * TILE1 + swz128(st * 32 + h * 16 + ((lane >> 4) << 3) + (lane & 7), (warp & 3) * 2 + ((lane >> 3) & 1)));
         }
       }
+    };
+    fetch(0);
+#pragma unroll
+    for (int st = 0; st < STEPS; ++st) {
+      uint32_t b[NT][4];
 #pragma unroll
       for (int i = 0; i < NT; ++i) ldsm4(b[i], xa + (st >> 1) * rows_pad * 128 + i * 1024 + swz128(lane & 7, (st & 1) * 4 + (lane >> 3)));
+      if (st + 1 < STEPS) fetch(st + 1);
       uint32_t a[2][2][4];                         // [tile][k-16 step]
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
@@ -439,34 +475,32 @@ __device__ __forceinline__ void multiply(Ring& ring, int n_units, int k0, int ro
           // raw[j]: k = 8j + 2 (lane % 4) in the low half, k + 1 in the high half; columns 2 (lane / 4) and + 1 as the two bytes
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            const uint32_t v = __byte_perm(raw[t][0][j], 0, 0x3120);
-            a[t][j >> 1][(j & 1) * 2] = e4m3x2_to_bf16x2(uint16_t(v & 0xffffu));
-            a[t][j >> 1][(j & 1) * 2 + 1] = e4m3x2_to_bf16x2(uint16_t(v >> 16));
+            const uint32_t v = __byte_perm(raw[st & 1][t][0][j], 0, 0x3120);
+            a[t][j >> 1][(j & 1) * 2] = e4m3x2_to_f16x2(uint16_t(v & 0xffffu));
+            a[t][j >> 1][(j & 1) * 2 + 1] = e4m3x2_to_f16x2(uint16_t(v >> 16));
           }
         } else {
 #pragma unroll
           for (int h = 0; h < 2; ++h)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) a[t][h][j] = raw[t][h][j];
+            for (int j = 0; j < 4; ++j) a[t][h][j] = raw[st & 1][t][h][j];
         }
       }
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        if (FP8) {
-          if (left == 0) {                         // a new scale block begins here
-            fold();
-            s0 = next0;
-            s1 = next1;
-            ++kb;
-            left = sc.bk / 16;
-            fetch_next();
-          }
-          --left;
-        }
 #pragma unroll
         for (int i = 0; i < NT; ++i) {
-          mma16816(FP8 ? acc[0][i] : tot[0][i], a[0][h], b[i][2 * h], b[i][2 * h + 1]);
-          mma16816(FP8 ? acc[1][i] : tot[1][i], a[1][h], b[i][2 * h], b[i][2 * h + 1]);
+#pragma unroll
+          for (int t = 0; t < 2; ++t) {
+            if (FP8) {
+              float d[4];
+              mma16816_f16(d, a[t][h], b[i][2 * h], b[i][2 * h + 1]);
+#pragma unroll
+              for (int j = 0; j < 4; ++j) tot[t][i][j] = fmaf(d[j], sc[t][(st * 2 + h) & 7], tot[t][i][j]);
+            } else {
+              mma16816(tot[t][i], a[t][h], b[i][2 * h], b[i][2 * h + 1]);
+            }
+          }
         }
       }
     }
@@ -474,7 +508,6 @@ __device__ __forceinline__ void multiply(Ring& ring, int n_units, int k0, int ro
     if (lane == 0) mbar_arrive(ring.empty + ring.s * 8);
     ring.next();
   }
-  if (FP8) fold();
 }
 
 // ------------------------------------------------------------------------------------------------ the kernel
@@ -498,15 +531,6 @@ struct Block {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     return t * 128 + warp * 16 + (FP8 ? 2 * (lane >> 2) + second : (lane >> 2) + 8 * second);
   }
-  template <bool DOWN>
-  __device__ Scales scales(int e, int panel) const {
-    if (!FP8) return Scales{nullptr, nullptr, 0, 16, 0};
-    const int N = DOWN ? p.C : 2 * p.H, K = DOWN ? p.H : p.C, bn = DOWN ? p.dn_bn : p.up_bn, bk = DOWN ? p.dn_bk : p.up_bk;
-    const int first = panel * (DOWN ? PANEL : 128) + int(threadIdx.x >> 5) * 16, second = DOWN ? first + 128 : p.H + first;
-    const float* base = (DOWN ? p.down_scale : p.up_scale) + (long long)e * (K / bk) * (N / bn);
-    return Scales{base + min(first, N - 16) / bn, base + min(second, N - 16) / bn, N / bn, bk, K / bk};
-  }
-
   // A cut panel (units [q0, q0 + per)) is the first or the last of a team's run: slot 0 or 1 of the team's member.
   __device__ float* slot_of(const Runs& runs, int q0, int team, int size, int member) const {
     return p.slots + ((long long)(team * size + member) * 2 + (runs.begin(team) >= q0 ? 0 : 1)) * slot_rows(p.F) * PANEL;
@@ -528,7 +552,7 @@ struct Block {
     const int lane = threadIdx.x & 31;
     const int e = L.expert[a], base = L.base[a], cnt = L.base[a + 1] - base;
     float tot[2][NT][4];
-    multiply<FP8, NT>(ring, n, (u - q0) * KT, rows_pad, scales<false>(e, panel), give, tot);
+    multiply<FP8, NT>(ring, n, rows_pad, give, tot);
     if (n < up_units) {                            // cut: every thread leaves its registers in the slot and picks up the same ones
       const int first = runs.owner(q0), last = runs.owner(q0 + up_units - 1), member = c % up_team;
       float* slot = slot_of(runs, q0, c / up_team, up_team, member) + threadIdx.x;
@@ -558,12 +582,13 @@ struct Block {
           for (int j = 0; j < 2; ++j) {
             const int r = i * 8 + (lane & 3) * 2 + j;
             if (r < cnt) {
-              const float rstd = L.rstd[L.tok[base + r]];
-              float g = fmaf(rstd, tot[0][i][2 * s + j], bg), l = fmaf(rstd, tot[1][i][2 * s + j], bl);
+              const float gain = L.gain[L.tok[base + r]];
+              float g = fmaf(gain, tot[0][i][2 * s + j], bg), l = fmaf(gain, tot[1][i][2 * s + j], bl);
               // comparisons keep a NaN where fminf / fmaxf would drop it
               g = g > p.limit ? p.limit : g;
               l = l > p.limit ? p.limit : (l < -p.limit ? -p.limit : l);
-              p.act[(long long)(base + r) * p.H + h] = __float2bfloat16((l + 1.f) * g / (1.f + exp2f(-p.beta * L2E * g)));
+              const float act = (l + 1.f) * g / (1.f + exp2f(-p.beta * L2E * g));
+              p.act[(long long)(base + r) * p.H + h] = FP8 ? __half_as_ushort(__float2half_rn(act * p.act_scale)) : __bfloat16_as_ushort(__float2bfloat16(act));
             }
           }
         }
@@ -576,7 +601,7 @@ struct Block {
     const int lane = threadIdx.x & 31;
     const int e = L.expert[a], base = L.base[a], cnt = L.base[a + 1] - base;
     float tot[2][NT][4];
-    multiply<FP8, NT>(ring, n, k_unit * KT, rows_pad, scales<true>(e, panel), give, tot);
+    multiply<FP8, NT>(ring, n, rows_pad, give, tot);
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
 #pragma unroll
@@ -589,7 +614,7 @@ struct Block {
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
             const int r = i * 8 + (lane & 3) * 2 + j;
-            if (r < cnt) buf[L.tok[base + r] * PANEL + cc] += L.score[base + r] * (tot[t][i][2 * s + j] + bias);
+            if (r < cnt) buf[L.tok[base + r] * PANEL + cc] += L.score[base + r] * fmaf(tot[t][i][2 * s + j], FP8 ? p.act_gain : 1.f, bias);
           }
         }
       }
@@ -652,15 +677,26 @@ struct Block {
   __device__ void join() const {
     const int per = L.n_active * dn_units;
     const Runs runs = down_runs();
-    for (int i = c * THREADS + int(threadIdx.x); i < p.F * p.C; i += G * THREADS) {
-      const int t = i / p.C, g = i - t * p.C, q = g / PANEL, group = q / dn_team, q0 = group * per;
+    const int quads = p.C / 4;                     // C is a multiple of 8: four columns at a time stay inside a panel
+    for (int i = c * THREADS + int(threadIdx.x); i < p.F * quads; i += G * THREADS) {
+      const int t = i / quads, g = (i - t * quads) * 4, q = g / PANEL, group = q / dn_team, q0 = group * per;
       const int first = runs.owner(q0), last = runs.owner(q0 + per - 1);
       if (first == last) continue;
       const int at = t * PANEL + g % PANEL, member = q % dn_team;
-      float v = 0.f;
+      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 8
-      for (int k = first; k <= last; ++k) v += __ldcg(slot_of(runs, q0, k, dn_team, member) + at);
-      store_out(i, v);
+      for (int k = first; k <= last; ++k) {
+        const float4 part = __ldcg(reinterpret_cast<const float4*>(slot_of(runs, q0, k, dn_team, member) + at));
+        v.x += part.x;
+        v.y += part.y;
+        v.z += part.z;
+        v.w += part.w;
+      }
+      const long long o = (long long)t * p.C + g;
+      store_out(o, v.x);
+      store_out(o + 1, v.y);
+      store_out(o + 2, v.z);
+      store_out(o + 3, v.w);
     }
   }
 
@@ -709,12 +745,35 @@ struct Block {
   template <bool DOWN>
   __device__ void feed_rows(Ring& r, Cursor& w, int n) const {
     const int lane = threadIdx.x & 31;
+    // e4m3: this lane's column group (of 16; tile lane / 8 % 2, warp lane % 8) of the scale table and its first k-16 step
+    const int K = DOWN ? p.H : p.C, N = DOWN ? p.C : 2 * p.H, bk = DOWN ? p.dn_bk : p.up_bk, bn = DOWN ? p.dn_bn : p.up_bn;
+    const int n_kb = FP8 ? K / bk : 0, n_nb = FP8 ? N / bn : 0;
+    const float per_bk = 1.f / float(bk);
+    const float* scales = nullptr;
+    int scales_a = -1, scales_group = -1;
     for (int i = 0; i < n; ++i) {
       if (!mbar_wait(r.empty + r.s * 8, r.ph ^ 1, give.flag)) give(STATUS_TIMEOUT_EMPTY);
       __syncwarp();
       if (!*give.flag) {
         const uint32_t dst = r.stages_addr + r.s * r.stage_bytes + W_STAGE;
         const int base = L.base[w.a], cnt = L.base[w.a + 1] - base;
+        if (FP8) {
+          if (w.a != scales_a || w.group != scales_group) {
+            scales_a = w.a;
+            scales_group = w.group;
+            const int tile = (lane >> 3) & 1, wc = (lane & 7) * 16, panel = w.group * (DOWN ? dn_team : up_team) + c % (DOWN ? dn_team : up_team);
+            const int col = DOWN ? panel * PANEL + tile * 128 + wc : tile * p.H + panel * 128 + wc;
+            scales = (DOWN ? p.down_scale : p.up_scale) + (long long)L.expert[w.a] * n_kb * n_nb + min(col, N - 16) / bn;
+          }
+          const uint32_t table = r.stages_addr + (r.s + 1) * r.stage_bytes - SCALE_STAGE + (lane & 15) * 32;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int step = (lane >> 4) * 4 + j;
+            // block of the step's first input: exact for inputs below 2^21 (the half keeps the product off the integers)
+            const int kb = int((float(min(w.k * KT + step * 16, K - 16)) + 0.5f) * per_bk);
+            cp4(table + step * 4, scales + (long long)min(kb, n_kb - 1) * n_nb);
+          }
+        }
         if (DOWN)
           load_acts<FP8>(dst, lane, cnt, rows_pad, w.k * KT, p.H, [&](int j) { return p.act + (long long)(base + j) * p.H; });
         else
@@ -735,7 +794,7 @@ moe_block_kernel(const __grid_constant__ CUtensorMap up_map, const __grid_consta
   const int stage_bytes = W_STAGE + p.x_stage;
   uint8_t* after = smem + p.stages * stage_bytes;
   float* buf = reinterpret_cast<float*>(after);
-  Lists& L = *reinterpret_cast<Lists*>(after + p.F * PANEL * 4);
+  Lists& L = *reinterpret_cast<Lists*>(after + buf_bytes(p.F));
   __shared__ uint64_t full[MAX_STAGES], empty[MAX_STAGES];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int G = int(gridDim.x), c = int(blockIdx.x);
@@ -760,17 +819,20 @@ moe_block_kernel(const __grid_constant__ CUtensorMap up_map, const __grid_consta
     for (int e = threadIdx.x; e < p.E; e += CONSUMERS) L.bias[e] = p.router_bias ? __ldg(p.router_bias + e) : 0.f;
     const int n_counters = (p.E + p.shared) * blk.up_groups * blk.up_team;
     for (int i = c * CONSUMERS + threadIdx.x; i < n_counters; i += G * CONSUMERS) p.counters[i] = 0;
-    for (int i = c * CONSUMERS + threadIdx.x; i < p.F * p.C; i += G * CONSUMERS) p.xs[i] = __float2bfloat16(__bfloat162float(p.x[i]) * __ldg(p.norm + i % p.C));
+    if (FP8) {
+      for (int t = G - 1 - c; t < p.F; t += G) operand_row_f16(p, t, buf);     // the CTAs with the fewest router tasks
+    } else {
+      for (int i = c * CONSUMERS + threadIdx.x; i < p.F * p.C; i += G * CONSUMERS)
+        p.xs[i] = __bfloat16_as_ushort(__float2bfloat16(__bfloat162float(__ldg(p.x + i)) * __ldg(p.norm + i % p.C)));
+    }
     const int tasks = (p.E + RE - 1) / RE * ((p.F + RT - 1) / RT) * p.csplit;
-    for (int t = c; t < tasks; t += G) router_task(p, t, reinterpret_cast<float*>(smem));
+    for (int t = c; t < tasks; t += G) router_task(p, t, buf);
   } else if (lane == 0) {
     tma_prefetch_desc(&up_map);
     tma_prefetch_desc(&down_map);
   }
   grid.sync();
-  if (warp < CONSUMERS / 32) route(p, L, reinterpret_cast<float*>(smem));
-  // the router's reduction used the stages through the generic proxy; the TMA writes there next
-  fence_proxy_async_smem();
+  if (warp < CONSUMERS / 32) route(p, L, buf);
   __syncthreads();
 
   // ---- phases 2 and 3
@@ -840,7 +902,7 @@ int launch(const CUtensorMap& up, const CUtensorMap& down, const Params& p, int 
 
 struct Plan {
   int grid, csplit, stages, x_stage, smem, up_team, dn_team;
-  long long logits, sq, xs, act, slots, counters, total;      // byte offsets into the workspace
+  long long logits, sq, gain, xs, act, slots, counters, total;      // byte offsets into the workspace
 };
 
 // Grid, ring depth and workspace of a call: functions of the sizes alone.
@@ -866,8 +928,8 @@ inline Plan make_plan(int F, int C, int H, int E, int shared, int k, bool fp8) {
   if (q.csplit > MAX_CSPLIT) q.csplit = MAX_CSPLIT;
   if (q.csplit > C / 128) q.csplit = C / 128;
   if (q.csplit < 1) q.csplit = 1;
-  q.x_stage = (F + 7) / 8 * 8 * 128 * (KT / 64);
-  const int fixed = 1024 + F * PANEL * 4 + int(sizeof(Lists));
+  q.x_stage = (F + 7) / 8 * 8 * 128 * (KT / 64) + (fp8 ? SCALE_STAGE : 0);
+  const int fixed = 1024 + buf_bytes(F) + int(sizeof(Lists));
   q.stages = (232448 - 1024 - fixed) / (W_STAGE + q.x_stage);  // 227 KB per CTA; the barriers are static
   if (q.stages > MAX_STAGES) q.stages = MAX_STAGES;
   q.smem = fixed + q.stages * (W_STAGE + q.x_stage);
@@ -875,6 +937,7 @@ inline Plan make_plan(int F, int C, int H, int E, int shared, int k, bool fp8) {
   auto take = [&](long long bytes) { const long long here = at; at += (bytes + 255) / 256 * 256; return here; };
   q.logits = take(4LL * q.csplit * F * E);
   q.sq = take(4LL * q.csplit * F);
+  q.gain = take(4LL * F);
   q.xs = take(2LL * F * C);
   q.act = take(2LL * F * (k + shared) * H);
   q.slots = take(4LL * q.grid * 2 * slot_rows(F) * PANEL);
@@ -905,6 +968,7 @@ extern "C" int lyra_moe_block(const void* x, const float* norm, float eps, const
   using namespace lyra;
   using namespace lyra::moeblk;
   if (lyra_moe_block_workspace(F, C, H, E, shared, k, fp8) < 0) return -100;
+  if (fp8 && !(limit >= 0.f && limit <= 1e4f)) return -100;   // the fp16 operand's range is fitted to it
   if (fp8 && (!up_scale || !down_scale || up_bk % 16 || up_bn % 16 || dn_bk % 16 || dn_bn % 16 || up_bk < 16 || up_bn < 16 || dn_bk < 16 || dn_bn < 16 ||
               C % up_bk || (2 * H) % up_bn || H % dn_bk || C % dn_bn))
     return -100;
@@ -939,8 +1003,9 @@ extern "C" int lyra_moe_block(const void* x, const float* norm, float eps, const
   p.idx = idx;
   p.part_logits = reinterpret_cast<float*>(ws + q.logits);
   p.part_sq = reinterpret_cast<float*>(ws + q.sq);
-  p.xs = reinterpret_cast<__nv_bfloat16*>(ws + q.xs);
-  p.act = reinterpret_cast<__nv_bfloat16*>(ws + q.act);
+  p.gain = reinterpret_cast<float*>(ws + q.gain);
+  p.xs = reinterpret_cast<uint16_t*>(ws + q.xs);
+  p.act = reinterpret_cast<uint16_t*>(ws + q.act);
   p.slots = reinterpret_cast<float*>(ws + q.slots);
   p.counters = reinterpret_cast<int*>(ws + q.counters);
   p.status = status;
@@ -948,5 +1013,9 @@ extern "C" int lyra_moe_block(const void* x, const float* norm, float eps, const
   p.csplit = q.csplit; p.stages = q.stages; p.x_stage = q.x_stage; p.up_team = q.up_team; p.dn_team = q.dn_team;
   p.up_bk = up_bk; p.up_bn = up_bn; p.dn_bk = dn_bk; p.dn_bn = dn_bn;
   p.eps = eps; p.beta = beta; p.limit = limit; p.residual_scale = residual_scale;
+  int halvings = 0;                                            // that bring (limit + 1) * limit below fp16's 65504
+  while (fp8 && double(limit + 1.f) * limit > 60000.0 * exp2(halvings)) ++halvings;
+  p.act_scale = float(exp2(-halvings));
+  p.act_gain = float(exp2(halvings));
   return fp8 ? launch<true>(um, dm, p, q.grid, q.smem, stream) : launch<false>(um, dm, p, q.grid, q.smem, stream);
 }

@@ -319,6 +319,8 @@ def moe_block(x, norm_scale, eps, router, router_bias, w_up, up_bias, w_down, do
         raise ValueError(f"moe_block does not take {F_} tokens, C {C}, H {H}, {E} + {n_shared} experts, k {k}, weights "
                          f"{type(w_up).__name__} / {type(w_down).__name__} on a GPU (ops.decode.moe_block_supported)")
     quant = isinstance(w_up, QArray)
+    if quant and not 0.0 <= limit <= 1e4:
+        raise ValueError(f"moe_block with e4m3 weights takes a SwiGLU limit in 0..1e4, got {limit}")
     with native.on_device(x):
         if quant:
             wu, wd = w_up.qval.contiguous(), w_down.qval.contiguous()

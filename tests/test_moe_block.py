@@ -225,6 +225,42 @@ def test_weights_of_experts_nobody_chose_are_not_looked_at_gpu():
 
 
 @pytest.mark.gpu
+def test_every_e4m3_code_gpu():
+    """All 254 numbers of the format as weights of the up-projection (one column each) against their values. The NaN code is kept: it
+    makes its hidden unit NaN, and that every output (the down-projection is dense, 0 * NaN = NaN)."""
+    C, H = 16, 256
+    a = make(1, C, H, 1, 1, 0, False, False, "cuda")
+    codes = torch.arange(256, dtype=torch.uint8, device="cuda")
+    codes[codes % 128 == 127] = 0
+    up = torch.zeros(1, C, 2 * H, dtype=torch.uint8, device="cuda")
+    up[0, 3, H:] = codes                                                   # linear half: one non-zero input row
+    up[0, :, :H] = torch.full((), 0.5, device="cuda").to(E4M3).view(torch.uint8)
+    down = torch.zeros(1, H, C, device="cuda")
+
+    def run():
+        b = {**a, "up": QArray(up.view(E4M3), torch.ones(1, 1, 1, device="cuda"), (C, 2 * H)), "down": quantize(down, E4M3, (16, 16))}
+        with torch.no_grad():
+            return ops.moe_block(b["x"], b["norm"], EPS, b["router"], None, b["up"], None, b["down"], None, 1, 0, BETA, 1e4, 1.0)[0]
+
+    x = a["x"].double()
+    xn = x / torch.sqrt((x * x).mean() + EPS) * a["norm"].double()
+    w = up.view(E4M3).double()[0]
+    t, size = (xn @ w)[0], (xn.abs() @ w.abs())[0]
+    act = (t[H:] + 1) * t[:H] * torch.sigmoid(BETA * t[:H])
+    for start in range(0, H, C):
+        down.zero_()
+        for c in range(C):
+            down[0, start + c, c] = 1.0
+        magnitude = x[0].abs() + (size[H:] + 1)[start:start + C] * size[0] * 1.1
+        assert ((run()[0].double() - (x[0] + act[start:start + C])).abs() <= 4 * 2**-8 * magnitude).all()
+    for code in (127, 255):
+        up[0, 5, H + 17] = code
+        assert torch.isnan(run()).all()
+        up[0, 5, H + 17] = 0
+    assert torch.isfinite(run()).all()
+
+
+@pytest.mark.gpu
 def test_refusals_and_layouts_gpu():
     from lyra_b200.ops import decode
 
