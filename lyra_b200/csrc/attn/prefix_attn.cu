@@ -1,0 +1,995 @@
+// Attention of a batch whose sequences share a prefix: every sequence's queries see the prefix's keys (stored once) and its own.
+//
+//   out = (sum_j e^{s_j} v_j) / (sum_j e^{s_j} + e^{sink}),  j over the visible prefix positions and the visible own positions
+//
+// A softmax over two sets of keys is the merge of two partial softmaxes (maximum, sum, unnormalised output), so the work is split
+// where the reuse changes:
+//
+//   prefix_kernel  the rows of all sequences (and of the query heads that share a kv head) against the prefix. Per kv head this is a
+//                  dense product of M = B * T * rep rows with P keys: 128-row tiles on tcgen05 with accumulators in TMEM, keys read once
+//                  per row tile. Few row tiles: the key axis is split so that every SM has work.
+//   own_kernel     each sequence against its own cache: no reuse beyond the rep heads, bound by reading the cache, so warp MMAs with
+//                  many bytes in flight. Its last step merges the prefix partials, its own and the sink, and rounds once.
+//
+// Prefix kernel, per item (row tile, kv head, key split), one persistent CTA per SM:
+//   warp 0        TMA producer: K and V tiles of 128 keys (bf16: straight into the operand tiles; e4m3: into a raw ring)
+//   warp 1        tcgen05 issuer:  S_g = Q K_j^T  and  O_g += P_g V_j   (g = j mod 2)
+//   warps 2..9    two softmax groups of four warps, alternate key tiles, one row per thread; each has its own scores, maximum, sum and
+//                 accumulator, merged once per item. P replaces S in TMEM as packed bf16 and is the MMA's TMEM operand.
+//   warps 10, 11  gather the query rows (any strides) into the operand tile; e4m3: also turn raw K / V tiles into bf16 operand tiles.
+//                 That conversion is exact; a key's scale multiplies its score, a value's scale its probability, both in fp32.
+#include <cooperative_groups.h>
+#include <cuda_fp8.h>
+
+#include "../common/sm100.cuh"
+#include "../common/tmap.h"
+
+namespace lyra {
+namespace prefix {
+
+namespace cg = cooperative_groups;
+
+constexpr float L2E = 1.4426950408889634f;
+constexpr int THREADS = 384, LOADERS = 64;      // warps 0, 1 | 2..9 | 10, 11
+constexpr int BM = 128, BN = 128;               // rows and keys of a tile
+constexpr int MAX_SPLITS = 32;
+
+struct Params {
+  const __nv_bfloat16* q;                       // [B, Nq, T, D] by strides (in elements)
+  long long q_sb, q_sn, q_st;
+  const int* pos;                               // own positions before the new tokens, one per sequence (pos_n = B) or one for all
+  int pos_n, pos_host;                          // pos == null: pos_host
+  const float *pk_scale, *pv_scale;             // e4m3 prefix: [Nkv, P] with head strides
+  long long pks_sh, pvs_sh;
+  float* part_o;                                // [B * T * Nq, splits, D] unnormalised
+  float2* part_ml;                              // [B * T * Nq, splits] (maximum in log2 units, sum)
+  int B, T, P, Nq, Nkv, rep, window, splits, key0;   // key0: first prefix position any row can see
+  float scale_log2;
+  int* status;
+};
+
+__device__ __forceinline__ int position(const int* pos, int n, int host, int b) { return pos ? __ldg(pos + (n == 1 ? 0 : b)) : host; }
+
+struct Item {
+  int m0, h, split, key, tiles;                 // first row, kv head, first key and number of key tiles
+};
+
+template <int D, bool FP8>
+struct Smem {
+  static constexpr int TILE = 128 * D * 2, RAW_TILE = 128 * D;
+  static constexpr int RAW = D == 64 ? 4 : 3;   // raw e4m3 tiles in flight (what 227 KB leave room for)
+  static constexpr int BYTES = 5 * TILE + (FP8 ? RAW * RAW_TILE : 0) + 1024;
+};
+
+__device__ __forceinline__ uint32_t e4m3x2_to_bf16x2(uint16_t two) {      // exact
+  const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(two, __NV_E4M3);
+  const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h));
+  return pack_bf16(f.x, f.y);
+}
+
+template <int D, bool FP8>
+__global__ void __launch_bounds__(THREADS, 1)
+prefix_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv, const Params p) {
+  constexpr int TILE = Smem<D, FP8>::TILE, RAW_TILE = Smem<D, FP8>::RAW_TILE, RAW = Smem<D, FP8>::RAW;
+  constexpr int HALF = 128 * 128;               // bytes of one 64-column block of an operand tile
+  constexpr uint32_t TMEM_COLS = 512, S_COL = 0, O_COL = 256, GROUP_COLS = 128;
+  constexpr uint32_t IDESC_S = make_idesc(BM, BN, 1, 1, 0, 0), IDESC_O = make_idesc(BM, D, 1, 1, 0, 1);
+
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t *sQ = smem, *sK = sQ + TILE, *sV = sK + 2 * TILE, *sR = sV + 2 * TILE;
+  __shared__ uint64_t q_full, q_empty, k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], o_full, o_empty, l_full;
+  __shared__ uint64_t raw_full[RAW], raw_empty[RAW], sc_full[4];
+  __shared__ float xm[2][2][BM], xl[2][2][BM];  // [item parity][group][row]
+  __shared__ __align__(16) float ksc[FP8 ? 4 : 1][BN], vsc[FP8 ? 4 : 1][BN];   // scales of the key tiles in flight
+  __shared__ uint32_t tmem_holder;
+  __shared__ int abort_flag;
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int M = p.B * p.T * p.rep, n_mt = (M + BM - 1) / BM;
+  const int n_tiles = (p.P - p.key0 + BN - 1) / BN;
+  const int n_items = n_mt * p.Nkv * p.splits;
+
+  // Items of a CTA: row tiles fastest, so that the CTAs running at the same time read the same keys.
+  auto item_at = [&](int round, Item& it) -> bool {
+    const int idx = round * int(gridDim.x) + int(blockIdx.x);
+    if (idx >= n_items) return false;
+    const int mt = idx % n_mt, rest = idx / n_mt;
+    it.m0 = mt * BM;
+    it.h = rest % p.Nkv;
+    it.split = rest / p.Nkv;
+    const int t0 = int((long long)n_tiles * it.split / p.splits), t1 = int((long long)n_tiles * (it.split + 1) / p.splits);
+    it.key = p.key0 + t0 * BN;
+    it.tiles = t1 - t0;
+    return true;
+  };
+
+  if (threadIdx.x == 0) {
+    mbar_init(smem_u32(&q_full), LOADERS);
+    mbar_init(smem_u32(&q_empty), 1);
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(smem_u32(&k_full[s]), FP8 ? LOADERS : 1);
+      mbar_init(smem_u32(&k_empty[s]), 1);
+      mbar_init(smem_u32(&v_full[s]), FP8 ? LOADERS : 1);
+      mbar_init(smem_u32(&v_empty[s]), 1);
+      mbar_init(smem_u32(&s_full[s]), 1);
+      mbar_init(smem_u32(&p_full[s]), 128);
+    }
+    for (int s = 0; s < RAW; ++s) {
+      mbar_init(smem_u32(&raw_full[s]), 1);
+      mbar_init(smem_u32(&raw_empty[s]), LOADERS);
+    }
+    for (int s = 0; s < 4; ++s) mbar_init(smem_u32(&sc_full[s]), LOADERS);
+    mbar_init(smem_u32(&l_full), 256);
+    mbar_init(smem_u32(&o_full), 1);
+    mbar_init(smem_u32(&o_empty), 256);
+    abort_flag = 0;
+    fence_mbar_init();
+  }
+  if (warp == 1) {
+    tmem_alloc(smem_u32(&tmem_holder), TMEM_COLS);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tmem_holder;
+  volatile int* abortp = &abort_flag;
+  Item w;
+
+  // Counters that run across the items (every role advances its own copies the same way; every item has at least one key tile):
+  //   t   key tiles so far: stage t & 1 of the K and V operand tiles, slot t & 3 of the scales
+  //   n   items so far: parity of q_full / q_empty / o_full / o_empty / l_full
+  //   c_g tiles given to softmax group g so far: parity of s_full[g] / p_full[g]
+  if (warp == 0) {
+    if (lane == 0) {
+      tma_prefetch_desc(&tk);
+      tma_prefetch_desc(&tv);
+      uint32_t t = 0;
+      bool ok = true;
+      for (int round = 0; ok && item_at(round, w); ++round) {
+        for (int j = 0; ok && j < w.tiles; ++j, ++t) {
+          const int k0 = w.key + j * BN;
+          if (FP8) {
+            for (int which = 0; ok && which < 2; ++which) {
+              const uint32_t i = 2 * t + which, s = i % RAW;
+              if (!mbar_wait(smem_u32(&raw_empty[s]), ((i / RAW) & 1) ^ 1, abortp)) { ok = false; break; }
+              mbar_expect_tx(smem_u32(&raw_full[s]), RAW_TILE);
+              tma_load_3d(smem_u32(sR + s * RAW_TILE), which ? &tv : &tk, smem_u32(&raw_full[s]), 0, k0, w.h);
+            }
+          } else {
+            const uint32_t s = t & 1, ph = (t >> 1) & 1;
+            if (!mbar_wait(smem_u32(&k_empty[s]), ph ^ 1, abortp)) { ok = false; break; }
+            mbar_expect_tx(smem_u32(&k_full[s]), TILE);
+            for (int c = 0; c < D / 64; ++c) tma_load_3d(smem_u32(sK + s * TILE + c * HALF), &tk, smem_u32(&k_full[s]), c * 64, k0, w.h);
+            if (!mbar_wait(smem_u32(&v_empty[s]), ph ^ 1, abortp)) { ok = false; break; }
+            mbar_expect_tx(smem_u32(&v_full[s]), TILE);
+            for (int c = 0; c < D / 64; ++c) tma_load_3d(smem_u32(sV + s * TILE + c * HALF), &tv, smem_u32(&v_full[s]), c * 64, k0, w.h);
+          }
+        }
+      }
+      if (!ok) {
+        atomicCAS(p.status, 0, STATUS_TIMEOUT_EMPTY);
+        abort_flag = 1;
+      }
+    }
+  } else if (warp == 1) {
+    if (lane == 0) {
+      // MMAs of one thread retire in issue order: S_g(j + 2), issued after P_g(j) V_j, cannot overwrite P_g(j) before it was read, and
+      // s_full[g] of tile j + 2 tells the group that O_g is quiet until it releases the next P.
+      uint32_t t = 0, n = 0, c[2] = {0, 0};
+      bool ok = true;
+      const uint64_t dq0 = make_smem_desc(smem_u32(sQ), 16, 1024), dk0 = make_smem_desc(smem_u32(sK), 16, 1024);
+      const uint64_t dv0 = make_smem_desc(smem_u32(sV), HALF, 1024);
+      for (int round = 0; ok && item_at(round, w); ++round) {
+        const uint32_t t0 = t;
+        auto issue_s = [&](int j) -> bool {
+          const int g = j & 1, s = (t0 + j) & 1;
+          if (!mbar_wait(smem_u32(&k_full[s]), ((t0 + j) >> 1) & 1, abortp)) return false;
+          tc_fence_after();
+          const uint64_t dk = desc_advance(dk0, s * TILE);
+#pragma unroll
+          for (int k = 0; k < D / 16; ++k)
+            tc_mma_ss(tmem + S_COL + g * GROUP_COLS, desc_advance(dq0, (k / 4) * HALF + (k % 4) * 32), desc_advance(dk, (k / 4) * HALF + (k % 4) * 32), IDESC_S, k > 0);
+          tc_commit(smem_u32(&s_full[g]));
+          tc_commit(smem_u32(&k_empty[s]));
+          if (j == w.tiles - 1) tc_commit(smem_u32(&q_empty));
+          return true;
+        };
+        ok = mbar_wait(smem_u32(&q_full), n & 1, abortp);
+        if (ok) ok = issue_s(0);
+        if (ok && w.tiles > 1) ok = issue_s(1);
+        if (ok) ok = mbar_wait(smem_u32(&o_empty), (n & 1) ^ 1, abortp);     // the previous item's output has been read
+        for (int j = 0; j < w.tiles && ok; ++j) {
+          const int g = j & 1, s = (t0 + j) & 1;
+          if (!mbar_wait(smem_u32(&v_full[s]), ((t0 + j) >> 1) & 1, abortp)) { ok = false; break; }
+          if (!mbar_wait(smem_u32(&p_full[g]), c[g] & 1, abortp)) { ok = false; break; }
+          ++c[g];
+          tc_fence_after();
+          const uint64_t dv = desc_advance(dv0, s * TILE);
+#pragma unroll
+          for (int k = 0; k < BN / 16; ++k)
+            tc_mma_ts(tmem + O_COL + g * GROUP_COLS, tmem + S_COL + g * GROUP_COLS + k * 8, desc_advance(dv, k * 2048), IDESC_O, (j >= 2 || k > 0) ? 1u : 0u);
+          tc_commit(smem_u32(&v_empty[s]));
+          if (j + 2 < w.tiles) ok = issue_s(j + 2);
+        }
+        if (ok) tc_commit(smem_u32(&o_full));
+        t += w.tiles;
+        ++n;
+      }
+      if (!ok) {
+        atomicCAS(p.status, 0, STATUS_TIMEOUT_FULL);
+        abort_flag = 1;
+      }
+    }
+  } else if (warp >= 10) {
+    // ------------------------------------------------------------ query rows; e4m3 tiles to bf16
+    const int tid = threadIdx.x - 320;
+    constexpr int CPR = D / 8;                  // 16-byte chunks per query row
+    uint32_t t = 0, n = 0;
+    bool ok = true;
+    for (int round = 0; ok && item_at(round, w); ++round, ++n) {
+      if (!mbar_wait(smem_u32(&q_empty), (n & 1) ^ 1, abortp)) { ok = false; break; }
+#pragma unroll 4
+      for (int i = tid; i < BM * CPR; i += LOADERS) {
+        const int r = i / CPR, c = i % CPR, m = w.m0 + r;
+        uint4 v = make_uint4(0u, 0u, 0u, 0u);
+        if (m < M) {
+          const int bt = m / p.rep, b = bt / p.T;
+          v = __ldg(reinterpret_cast<const uint4*>(p.q + b * p.q_sb + (long long)(w.h * p.rep + m - bt * p.rep) * p.q_sn + (long long)(bt - b * p.T) * p.q_st) + c);
+        }
+        *reinterpret_cast<uint4*>(sQ + (c >> 3) * HALF + swz128(r, c & 7)) = v;
+      }
+      fence_proxy_async_smem();
+      mbar_arrive(smem_u32(&q_full));
+      if (FP8) {
+        for (int j = 0; ok && j < w.tiles; ++j, ++t) {
+          const uint32_t s = t & 1, ph = (t >> 1) & 1;
+          const int k0 = w.key + j * BN;
+          // slot t & 3 is free: tile t - 4 left softmax before the operand stage of tile t - 2 was released
+          for (int which = 0; which < 2; ++which) {
+            const uint32_t i = 2 * t + which, rs = i % RAW;
+            if (!mbar_wait(smem_u32(which ? &v_empty[s] : &k_empty[s]), ph ^ 1, abortp) || !mbar_wait(smem_u32(&raw_full[rs]), (i / RAW) & 1, abortp)) {
+              ok = false;
+              break;
+            }
+            const uint8_t* from = sR + rs * RAW_TILE;
+            uint8_t* to = (which ? sV : sK) + s * TILE;
+            constexpr int RC = D / 16;          // 16-byte chunks per raw row
+#pragma unroll 4
+            for (int x = tid; x < BN * RC; x += LOADERS) {
+              const int r = x / RC, c = x % RC;
+              const uint4 v = *reinterpret_cast<const uint4*>(from + x * 16);
+              const uint32_t in[4] = {v.x, v.y, v.z, v.w};
+              uint32_t o[8];
+#pragma unroll
+              for (int y = 0; y < 4; ++y) {
+                o[2 * y] = e4m3x2_to_bf16x2(uint16_t(in[y] & 0xffffu));
+                o[2 * y + 1] = e4m3x2_to_bf16x2(uint16_t(in[y] >> 16));
+              }
+              uint8_t* dst = to + (c >> 2) * HALF;
+              *reinterpret_cast<uint4*>(dst + swz128(r, (c & 3) * 2)) = make_uint4(o[0], o[1], o[2], o[3]);
+              *reinterpret_cast<uint4*>(dst + swz128(r, (c & 3) * 2 + 1)) = make_uint4(o[4], o[5], o[6], o[7]);
+            }
+            if (which == 0) {
+#pragma unroll
+              for (int y = 0; y < BN / LOADERS; ++y) {
+                const int key = k0 + tid + y * LOADERS;
+                const bool in = key < p.P;      // 1 past the end: those scores are masked, -inf * 0 would not be -inf
+                ksc[t & 3][tid + y * LOADERS] = in ? __ldg(p.pk_scale + w.h * p.pks_sh + key) * p.scale_log2 : 1.f;
+                vsc[t & 3][tid + y * LOADERS] = in ? __ldg(p.pv_scale + w.h * p.pvs_sh + key) : 1.f;
+              }
+              mbar_arrive(smem_u32(&sc_full[t & 3]));
+            }
+            fence_proxy_async_smem();
+            mbar_arrive(smem_u32(&raw_empty[rs]));
+            mbar_arrive(smem_u32(which ? &v_full[s] : &k_full[s]));
+          }
+        }
+      }
+    }
+    if (!ok) {
+      if (lane == 0) atomicCAS(p.status, 0, STATUS_TIMEOUT_EMPTY);
+      abort_flag = 1;
+    }
+  } else {
+    // ------------------------------------------------------------ softmax and epilogue
+    const int quarter = warp & 3;
+    const int row = quarter * 32 + lane;        // row of the tile == TMEM lane
+    const uint32_t lane_addr = uint32_t(quarter * 32) << 16;
+    const int g = (warp - 2) >> 2;              // group 0: key tiles 0, 2, ...; group 1: 1, 3, ...
+    const uint32_t s_addr = tmem + lane_addr + S_COL + g * GROUP_COLS, o_addr = tmem + lane_addr + O_COL + g * GROUP_COLS;
+    const float sc = p.scale_log2;
+    uint32_t t = 0, n = 0, cg_ = 0;
+    bool failed = false;
+
+    for (int round = 0; !failed && item_at(round, w); ++round) {
+      const int m_row = w.m0 + row;
+      const bool row_valid = m_row < M, warp_idle = w.m0 + quarter * 32 >= M;
+      const int bt = m_row / p.rep, b = bt / p.T;
+      const int lo = p.window > 0 && row_valid ? p.P + position(p.pos, p.pos_n, p.pos_host, b) + (bt - b * p.T) - p.window + 1 : 0;   // first visible key
+      float m = -INFINITY, l = 0.f;
+
+      for (int j = g; j < w.tiles; j += 2, ++cg_) {
+        const int k0 = w.key + j * BN;
+        const uint32_t slot = (t + j) & 3;
+        if (FP8 && !mbar_wait(smem_u32(&sc_full[slot]), ((t + j) >> 2) & 1, abortp)) { failed = true; break; }
+        if (!mbar_wait(smem_u32(&s_full[g]), cg_ & 1, abortp)) { failed = true; break; }
+        tc_fence_after();
+        if (!warp_idle) {                       // rows past the last one keep whatever their lanes hold: no other row sees it
+          const bool need_mask = k0 + BN > p.P || (p.window > 0);
+          auto load = [&](int c, uint32_t (&r)[32]) {
+            tmem_ld32(s_addr + c * 32, r);
+            tmem_ld_wait();
+            if (FP8) {
+#pragma unroll
+              for (int i = 0; i < 32; i += 4) {
+                const float4 f = *reinterpret_cast<const float4*>(&ksc[slot][c * 32 + i]);
+                r[i] = __float_as_uint(__uint_as_float(r[i]) * f.x);
+                r[i + 1] = __float_as_uint(__uint_as_float(r[i + 1]) * f.y);
+                r[i + 2] = __float_as_uint(__uint_as_float(r[i + 2]) * f.z);
+                r[i + 3] = __float_as_uint(__uint_as_float(r[i + 3]) * f.w);
+              }
+            }
+            if (need_mask) {
+#pragma unroll
+              for (int i = 0; i < 32; ++i) {
+                const int kk = k0 + c * 32 + i;
+                if (kk >= p.P || kk < lo) r[i] = 0xff800000u;
+              }
+            }
+          };
+          const float s2 = FP8 ? 1.f : sc;      // e4m3: the softmax scale came in with the key's
+          // A row without a reference yet (its first tile, or nothing visible so far) takes the tile's maximum first.
+          if (__any_sync(0xffffffffu, m == -INFINITY)) {
+            float mx = -INFINITY;
+#pragma unroll 1
+            for (int c = 0; c < 4; ++c) {
+              uint32_t r[32];
+              load(c, r);
+#pragma unroll
+              for (int i = 0; i < 32; ++i) mx = fmaxf(mx, __uint_as_float(r[i]));
+            }
+            if (m == -INFINITY) m = mx * s2;
+          }
+          // One pass in the common case: probabilities against the current reference while the tile's maximum is tracked; redone
+          // (the scores are still in TMEM) when a row has to move its reference by more than 2^8.
+          float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY}, sum4[4] = {0.f, 0.f, 0.f, 0.f};
+          uint32_t pk[2][32];
+          float ref = m == -INFINITY ? 0.f : m;
+          auto quarter_pass = [&](int c, bool track) {
+            uint32_t r[32];
+            load(c, r);
+#pragma unroll
+            for (int i = 0; i < 32; i += 2) {
+              const float a = __uint_as_float(r[i]), d = __uint_as_float(r[i + 1]);
+              if (track) mx4[c] = fmaxf(mx4[c], fmaxf(a, d));
+              float p0 = exp2f(fmaf(a, s2, -ref)), p1 = exp2f(fmaf(d, s2, -ref));
+              sum4[c] += p0 + p1;
+              if (FP8) {
+                const float2 f = *reinterpret_cast<const float2*>(&vsc[slot][c * 32 + i]);
+                p0 *= f.x;
+                p1 *= f.y;
+              }
+              pk[c >> 1][(c & 1) * 16 + (i >> 1)] = pack_bf16(p0, p1);
+            }
+          };
+#pragma unroll
+          for (int c = 0; c < 4; ++c) quarter_pass(c, true);
+          const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * s2;
+          if (__any_sync(0xffffffffu, mx > ref + 8.f)) {
+            float factor = 1.f;
+            if (mx > ref + 8.f) {
+              factor = exp2f(ref - mx);
+              m = ref = mx;
+            }
+            l *= factor;
+            if (j >= 2) {                       // O_g holds tiles j - 2, j - 4, ...: all retired (see the issuer)
+#pragma unroll 1
+              for (int c = 0; c < D / 32; ++c) {
+                uint32_t o[32];
+                tmem_ld32(o_addr + c * 32, o);
+                tmem_ld_wait();
+#pragma unroll
+                for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * factor);
+                tmem_st32(o_addr + c * 32, o);
+              }
+            }
+            sum4[0] = sum4[1] = sum4[2] = sum4[3] = 0.f;
+#pragma unroll
+            for (int c = 0; c < 4; ++c) quarter_pass(c, false);
+          }
+          tmem_st32(s_addr, pk[0]);
+          tmem_st32(s_addr + 32, pk[1]);
+          tmem_st_wait();
+          l += (sum4[0] + sum4[1]) + (sum4[2] + sum4[3]);
+        }
+        tc_fence_before();
+        mbar_arrive(smem_u32(&p_full[g]));
+      }
+      if (failed) break;
+      t += w.tiles;
+
+      // merge of the two groups -> the split's partial result
+      const int par = n & 1;
+      xm[par][g][row] = m;
+      xl[par][g][row] = l;
+      mbar_arrive(smem_u32(&l_full));
+      if (!mbar_wait(smem_u32(&o_full), par, abortp)) { failed = true; break; }
+      if (!mbar_wait(smem_u32(&l_full), par, abortp)) { failed = true; break; }
+      tc_fence_after();
+      const bool two = w.tiles > 1;
+      const float m0 = xm[par][0][row], m1 = two ? xm[par][1][row] : -INFINITY;
+      const float mt = fmaxf(m0, m1);
+      const float a0 = m0 == -INFINITY ? 0.f : exp2f(m0 - mt), a1 = m1 == -INFINITY ? 0.f : exp2f(m1 - mt);
+      const float lt = a0 * xl[par][0][row] + (two ? a1 * xl[par][1][row] : 0.f);
+      const long long out_row = ((long long)bt * p.Nq + w.h * p.rep + (m_row - bt * p.rep)) * p.splits + w.split;
+      if (!warp_idle) {
+#pragma unroll 1
+        for (int c = g; c < D / 32; c += 2) {   // each group writes half of the columns
+          uint32_t r0[32], r1[32];
+          tmem_ld32(tmem + lane_addr + O_COL + c * 32, r0);
+          if (two) tmem_ld32(tmem + lane_addr + O_COL + GROUP_COLS + c * 32, r1);
+          tmem_ld_wait();
+          if (row_valid) {
+            float* dst = p.part_o + out_row * D + c * 32;
+#pragma unroll
+            for (int i = 0; i < 32; i += 4) {
+              float4 v;
+              v.x = __uint_as_float(r0[i]) * a0;
+              v.y = __uint_as_float(r0[i + 1]) * a0;
+              v.z = __uint_as_float(r0[i + 2]) * a0;
+              v.w = __uint_as_float(r0[i + 3]) * a0;
+              if (two) {
+                v.x = fmaf(__uint_as_float(r1[i]), a1, v.x);
+                v.y = fmaf(__uint_as_float(r1[i + 1]), a1, v.y);
+                v.z = fmaf(__uint_as_float(r1[i + 2]), a1, v.z);
+                v.w = fmaf(__uint_as_float(r1[i + 3]), a1, v.w);
+              }
+              *reinterpret_cast<float4*>(dst + i) = v;
+            }
+          }
+        }
+        if (row_valid && g == 0) p.part_ml[out_row] = make_float2(mt, lt);
+      }
+      tc_fence_before();
+      mbar_arrive(smem_u32(&o_empty));
+      ++n;
+    }
+    if (failed) {
+      if (lane == 0) atomicCAS(p.status, 0, STATUS_TIMEOUT_TMEM);
+      abort_flag = 1;
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (abort_flag) {
+    for (int i = 0; i < 64; ++i) __nanosleep(1000);
+    __syncthreads();
+  }
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, TMEM_COLS);
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ own keys and merge
+constexpr int OWARPS = 4, OTHREADS = OWARPS * 32, OSTAGES = 2;
+
+struct OwnParams {
+  const __nv_bfloat16* q;
+  long long q_sb, q_sn, q_st;
+  const uint8_t *k, *v;                         // [B, Nkv, S, D] contiguous, bf16 or e4m3
+  const float *k_scale, *v_scale;               // e4m3: [B, Nkv, S]
+  const int* pos;
+  int pos_n, pos_host;
+  const float* sinks;                           // [Nq] or null
+  const float* part_o;                          // prefix partials (splits > 0)
+  const float2* part_ml;
+  __nv_bfloat16* out;                           // [B, T, Nq, D]
+  int B, T, S, Nq, Nkv, rep, window, splits, row_tiles, cluster;
+  float scale_log2;
+};
+
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src, int nbytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(nbytes) : "memory");
+}
+__device__ __forceinline__ void cp4(uint32_t dst, const void* src, int nbytes) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(nbytes) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
+}
+__device__ __forceinline__ void ldsm4t(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
+}
+__device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// ROWS: 64 query rows per CTA, 16 per warp, all warps walk the same key tiles (several tokens per sequence: the tiles are shared).
+// Otherwise at most 16 rows, and the warps (and the CTAs of a cluster) split the keys (one token: all bytes in flight at once).
+template <int D, bool FP8, bool ROWS>
+struct OwnGeo {
+  static constexpr int TK = 2048 / D;                            // keys per tile: 4 KB of bf16 keys
+  static constexpr int ROWB = D * 2 + 16;                        // padded operand row: ldmatrix rows fall in distinct banks
+  static constexpr int TILE_B = TK * ROWB;
+  static constexpr int RAW_B = FP8 ? TK * D : TILE_B;            // one K or V tile as it arrives
+  static constexpr int STAGE_B = 2 * RAW_B + 2 * TK * 4;         // + scales
+  static constexpr int RING_B = OSTAGES * STAGE_B + (FP8 ? 2 * TILE_B : 0);
+  static constexpr int ROWS_CTA = ROWS ? 64 : 16;
+  static constexpr int COMB_B = ROWS_CTA * D * 4, WARP_O_B = ROWS ? 0 : OWARPS * 16 * D * 4;
+  static constexpr int RINGS_B = (ROWS ? 1 : OWARPS) * RING_B;
+  static constexpr int SMEM_B = RINGS_B > COMB_B + WARP_O_B ? RINGS_B : COMB_B + WARP_O_B;
+};
+
+template <int D, bool FP8, bool ROWS>
+__global__ void __launch_bounds__(OTHREADS) own_kernel(const OwnParams p) {
+  using G_ = OwnGeo<D, FP8, ROWS>;
+  constexpr int TK = G_::TK, ROWB = G_::ROWB, TILE_B = G_::TILE_B, RAW_B = G_::RAW_B, STAGE_B = G_::STAGE_B, RC = G_::ROWS_CTA;
+  constexpr int ESZ = FP8 ? 1 : 2, LT = ROWS ? OTHREADS : 32;    // threads that fill one ring
+  constexpr int MAXW = 8 + MAX_SPLITS;
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ float red_m[OWARPS * 16], red_l[OWARPS * 16];       // per warp and row
+  __shared__ float comb_m[RC], comb_l[RC], weight[RC][MAXW + 1];
+  float* comb = reinterpret_cast<float*>(smem);                  // [RC][D], after the key loop
+  float* warp_o = comb + RC * D;                                 // [OWARPS][16][D]
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, lt = ROWS ? tid : lane;
+  const int rank = int(blockIdx.x) % p.cluster;
+  int rest = int(blockIdx.x) / p.cluster;
+  const int rt = rest % p.row_tiles;
+  rest /= p.row_tiles;
+  const int h = rest % p.Nkv, b = rest / p.Nkv;
+  const int R = p.T * p.rep, row0 = rt * RC, n_rows = min(RC, R - row0);
+  const int pos = position(p.pos, p.pos_n, p.pos_host, b);
+  auto out_row = [&](int r) {
+    const int rr = row0 + r, t = rr / p.rep;
+    return ((long long)b * p.T + t) * p.Nq + h * p.rep + (rr - t * p.rep);
+  };
+  const bool idle = pos < 0;                                     // an unused place of the batch: zeros
+  // keys any row of this CTA can see
+  const int t_lo = row0 / p.rep, t_hi = (row0 + n_rows - 1) / p.rep;
+  const int lo = p.window > 0 ? max(0, pos + t_lo - p.window + 1) : 0, hi = idle ? -1 : min(pos + t_hi, p.S - 1);
+  const int n_keys = max(hi - lo + 1, 0);
+  const int chunk = ((n_keys + p.cluster - 1) / p.cluster + TK - 1) / TK * TK;
+  const int kbeg = lo + rank * chunk, kend = min(kbeg + chunk, hi + 1);
+  const int n_tiles = kend > kbeg ? (kend - kbeg + TK - 1) / TK : 0;
+  const int first = ROWS ? 0 : warp, step = ROWS ? 1 : OWARPS;
+  const int nt = n_tiles > first ? (n_tiles - first + step - 1) / step : 0;
+
+  uint8_t* ring = smem + (ROWS ? 0 : warp * G_::RING_B);
+  const size_t head = (size_t(b) * p.Nkv + h) * p.S;
+  const uint8_t *kbase = p.k + head * D * ESZ, *vbase = p.v + head * D * ESZ;
+
+  auto issue = [&](int i) {                                      // i-th tile of this ring -> stage i % OSTAGES
+    const int key0 = kbeg + (first + i * step) * TK;
+    uint8_t* st = ring + (i % OSTAGES) * STAGE_B;
+    constexpr int CPR = D * ESZ / 16, DROW = FP8 ? D : ROWB;
+#pragma unroll
+    for (int j = 0; j < TK * CPR / LT; ++j) {
+      const int c = lt + LT * j, row = c / CPR, col = c % CPR, key = key0 + row;
+      const bool ok = key < kend;
+      const size_t off = size_t(ok ? key : kbeg) * D * ESZ + col * 16;
+      cp16(smem_u32(st + row * DROW + col * 16), kbase + off, ok ? 16 : 0);
+      cp16(smem_u32(st + RAW_B + row * DROW + col * 16), vbase + off, ok ? 16 : 0);
+    }
+    if (FP8 && lt < TK) {
+      const int key = key0 + lt;
+      const bool ok = key < kend;
+      const size_t off = head + (ok ? key : kbeg);
+      cp4(smem_u32(st + 2 * RAW_B + lt * 4), p.k_scale + off, ok ? 4 : 0);
+      cp4(smem_u32(st + 2 * RAW_B + TK * 4 + lt * 4), p.v_scale + off, ok ? 4 : 0);
+    }
+  };
+#pragma unroll
+  for (int s = 0; s < OSTAGES - 1; ++s) {
+    if (s < nt) issue(s);
+    cp_commit();
+  }
+
+  // ---- query fragments (rows past the last one are zero) and each row's visible keys
+  const int wr = (ROWS ? warp * 16 : 0) + (lane >> 2);           // this thread's first row; the second is 8 further on
+  uint32_t qa[D / 16][4];
+  int row_hi[2], row_lo[2];
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    const int r = wr + 8 * e, rr = row0 + r, t = rr / p.rep;
+    const bool ok = r < n_rows;
+    row_hi[e] = ok ? pos + t : -1;
+    row_lo[e] = p.window > 0 ? pos + t - p.window + 1 : 0;
+    const __nv_bfloat16* src = p.q + b * p.q_sb + (long long)(h * p.rep + (rr - t * p.rep)) * p.q_sn + t * p.q_st + (lane & 3) * 2;
+#pragma unroll
+    for (int ks = 0; ks < D / 16; ++ks) {
+      qa[ks][e] = ok ? __ldg(reinterpret_cast<const uint32_t*>(src + ks * 16)) : 0u;
+      qa[ks][e + 2] = ok ? __ldg(reinterpret_cast<const uint32_t*>(src + ks * 16 + 8)) : 0u;
+    }
+  }
+  float o[D / 8][4];
+#pragma unroll
+  for (int i = 0; i < D / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+
+  for (int i = 0; i < nt; ++i) {
+    if (i + OSTAGES - 1 < nt) issue(i + OSTAGES - 1);
+    cp_commit();
+    cp_wait<OSTAGES - 1>();
+    if (ROWS) __syncthreads(); else __syncwarp();
+    uint8_t* st = ring + (i % OSTAGES) * STAGE_B;
+    uint8_t *kt = st, *vt = st + RAW_B;
+    const float *ksc = reinterpret_cast<const float*>(st + 2 * RAW_B), *vsc = ksc + TK;
+    if (FP8) {                                                   // e4m3 rows -> bf16 operand rows, exactly; the scales come later
+      kt = ring + OSTAGES * STAGE_B;
+      vt = kt + TILE_B;
+      constexpr int CPR = D / 16;
+#pragma unroll
+      for (int j = 0; j < 2 * TK * CPR / LT; ++j) {
+        const int c = lt + LT * j, which = c / (TK * CPR), row = c % (TK * CPR) / CPR, col = c % CPR;
+        const uint4 raw = *reinterpret_cast<const uint4*>(st + which * RAW_B + row * D + col * 16);
+        const uint32_t in[4] = {raw.x, raw.y, raw.z, raw.w};
+        uint32_t ow[8];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          ow[2 * u] = e4m3x2_to_bf16x2(uint16_t(in[u] & 0xffffu));
+          ow[2 * u + 1] = e4m3x2_to_bf16x2(uint16_t(in[u] >> 16));
+        }
+        uint8_t* dst = (which ? vt : kt) + row * ROWB + col * 32;
+        *reinterpret_cast<uint4*>(dst) = make_uint4(ow[0], ow[1], ow[2], ow[3]);
+        *reinterpret_cast<uint4*>(dst + 16) = make_uint4(ow[4], ow[5], ow[6], ow[7]);
+      }
+      if (ROWS) __syncthreads(); else __syncwarp();
+    }
+    const int key0 = kbeg + (first + i * step) * TK;
+
+    float s[TK / 8][4];
+#pragma unroll
+    for (int j = 0; j < TK / 8; ++j) s[j][0] = s[j][1] = s[j][2] = s[j][3] = 0.f;
+    const uint32_t kaddr = smem_u32(kt) + ((lane >> 4) * 8 + (lane & 7)) * ROWB + ((lane >> 3) & 1) * 16;
+#pragma unroll
+    for (int ks = 0; ks < D / 16; ++ks) {
+#pragma unroll
+      for (int jp = 0; jp < TK / 16; ++jp) {
+        uint32_t r[4];
+        ldsm4(r, kaddr + jp * 16 * ROWB + ks * 32);
+        mma16816(s[jp * 2], qa[ks], r[0], r[1]);
+        mma16816(s[jp * 2 + 1], qa[ks], r[2], r[3]);
+      }
+    }
+    float mx[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+    for (int j = 0; j < TK / 8; ++j) {
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        const int e = x >> 1, at = j * 8 + (lane & 3) * 2 + (x & 1), key = key0 + at;
+        const float f = FP8 ? p.scale_log2 * ksc[at] : p.scale_log2;
+        s[j][x] = key < kend && key <= row_hi[e] && key >= row_lo[e] ? s[j][x] * f : -INFINITY;
+        mx[e] = fmaxf(mx[e], s[j][x]);
+      }
+    }
+    float alpha[2], ref[2], sum[2] = {0.f, 0.f};
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], 1));
+      mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], 2));
+      const float mn = fmaxf(m[e], mx[e]);
+      alpha[e] = mn == -INFINITY ? 1.f : exp2f(m[e] - mn);
+      ref[e] = mn == -INFINITY ? 0.f : mn;
+      m[e] = mn;
+    }
+#pragma unroll
+    for (int j = 0; j < TK / 8; ++j)
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        s[j][x] = exp2f(s[j][x] - ref[x >> 1]);
+        sum[x >> 1] += s[j][x];
+        if (FP8) s[j][x] *= vsc[j * 8 + (lane & 3) * 2 + (x & 1)];
+      }
+    l[0] = l[0] * alpha[0] + sum[0];
+    l[1] = l[1] * alpha[1] + sum[1];
+#pragma unroll
+    for (int d = 0; d < D / 8; ++d) {
+      o[d][0] *= alpha[0];
+      o[d][1] *= alpha[0];
+      o[d][2] *= alpha[1];
+      o[d][3] *= alpha[1];
+    }
+    const uint32_t vaddr = smem_u32(vt) + (((lane >> 3) & 1) * 8 + (lane & 7)) * ROWB + (lane >> 4) * 16;
+#pragma unroll
+    for (int kk = 0; kk < TK / 16; ++kk) {                       // P's accumulator layout is the A-operand layout of the next product
+      const uint32_t pa[4] = {pack_bf16(s[2 * kk][0], s[2 * kk][1]), pack_bf16(s[2 * kk][2], s[2 * kk][3]),
+                              pack_bf16(s[2 * kk + 1][0], s[2 * kk + 1][1]), pack_bf16(s[2 * kk + 1][2], s[2 * kk + 1][3])};
+#pragma unroll
+      for (int dp = 0; dp < D / 16; ++dp) {
+        uint32_t r[4];
+        ldsm4t(r, vaddr + kk * 16 * ROWB + dp * 32);
+        mma16816(o[dp * 2], pa, r[0], r[1]);
+        mma16816(o[dp * 2 + 1], pa, r[2], r[3]);
+      }
+    }
+    if (ROWS) __syncthreads(); else __syncwarp();
+  }
+  cp_wait<0>();
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    l[e] += __shfl_xor_sync(0xffffffffu, l[e], 1);
+    l[e] += __shfl_xor_sync(0xffffffffu, l[e], 2);
+  }
+  __syncthreads();                                               // every ring is drained: its space is reused
+
+  // ---- the CTA's partial result in comb / comb_m / comb_l
+  {
+    float* dst = ROWS ? comb + warp * 16 * D : warp_o + warp * 16 * D;
+    const int r0 = lane >> 2, c = (lane & 3) * 2;
+#pragma unroll
+    for (int d = 0; d < D / 8; ++d) {
+      *reinterpret_cast<float2*>(dst + r0 * D + d * 8 + c) = make_float2(o[d][0], o[d][1]);
+      *reinterpret_cast<float2*>(dst + (r0 + 8) * D + d * 8 + c) = make_float2(o[d][2], o[d][3]);
+    }
+    if ((lane & 3) == 0) {
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int at = warp * 16 + r0 + 8 * e;
+        if (ROWS) {
+          comb_m[at % RC] = m[e];
+          comb_l[at % RC] = l[e];
+        } else {
+          red_m[at] = m[e];
+          red_l[at] = l[e];
+        }
+      }
+    }
+  }
+  if (!ROWS) {
+    __syncthreads();
+    for (int i = tid; i < n_rows * D; i += OTHREADS) {
+      const int r = i / D, d = i % D;
+      float M = -INFINITY;
+#pragma unroll
+      for (int x = 0; x < OWARPS; ++x) M = fmaxf(M, red_m[x * 16 + r]);
+      float L = 0.f, O = 0.f;
+#pragma unroll
+      for (int x = 0; x < OWARPS; ++x) {
+        const float mw = red_m[x * 16 + r], f = mw == -INFINITY ? 0.f : exp2f(mw - M);
+        L += red_l[x * 16 + r] * f;
+        O += warp_o[(x * 16 + r) * D + d] * f;
+      }
+      comb[r * D + d] = O;
+      if (d == 0) {
+        comb_m[r] = M;
+        comb_l[r] = L;
+      }
+    }
+  }
+  __syncthreads();
+  cg::cluster_group cluster = cg::this_cluster();
+  if (!ROWS && p.cluster > 1) cluster.sync();
+
+  // ---- weights of all partial results of a row: the cluster's CTAs, then the prefix splits; the last place holds 1 / (their sum)
+  constexpr int TPR = OTHREADS / RC;                             // threads per row
+  {
+    const int r = tid / TPR, x = tid % TPR, n_own = ROWS ? 1 : p.cluster, n = n_own + p.splits;
+    const long long row = r < n_rows ? out_row(r) : 0;
+    float M = -INFINITY, L = 0.f;
+    auto ml = [&](int j) -> float2 {
+      if (j >= n_own) return __ldcg(p.part_ml + row * p.splits + (j - n_own));
+      if (ROWS || p.cluster == 1) return make_float2(comb_m[r], comb_l[r]);
+      return make_float2(*cluster.map_shared_rank(&comb_m[r], j), *cluster.map_shared_rank(&comb_l[r], j));
+    };
+    const float sink = p.sinks && r < n_rows ? __ldg(p.sinks + h * p.rep + (row0 + r) % p.rep) * L2E : -INFINITY;
+    if (r < n_rows)
+      for (int j = x; j < n; j += TPR) M = fmaxf(M, ml(j).x);
+#pragma unroll
+    for (int of = TPR / 2; of > 0; of >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, of));
+    M = fmaxf(M, sink);
+    if (r < n_rows)
+      for (int j = x; j < n; j += TPR) {
+        const float2 v = ml(j);
+        const float f = v.x == -INFINITY ? 0.f : exp2f(v.x - M);
+        weight[r][j] = f;
+        L += v.y * f;
+      }
+#pragma unroll
+    for (int of = TPR / 2; of > 0; of >>= 1) L += __shfl_xor_sync(0xffffffffu, L, of);
+    if (sink != -INFINITY) L += exp2f(sink - M);
+    if (r < n_rows && x == 0) weight[r][MAXW] = idle || L == 0.f ? 0.f : 1.f / L;      // nothing visible and no sink: zeros
+  }
+  __syncthreads();
+
+  // ---- output, four columns per thread; the CTAs of a cluster share the rows' columns
+  constexpr int Q = D / 4;
+  for (int i = rank * OTHREADS + tid; i < n_rows * Q; i += p.cluster * OTHREADS) {
+    const int r = i / Q, d = (i % Q) * 4;
+    const float inv = weight[r][MAXW];
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    auto add = [&](const float4& x, float f) {
+      v.x = fmaf(x.x, f, v.x);
+      v.y = fmaf(x.y, f, v.y);
+      v.z = fmaf(x.z, f, v.z);
+      v.w = fmaf(x.w, f, v.w);
+    };
+    const long long row = out_row(r);
+    if (!idle) {
+      const float* po = p.part_o + row * p.splits * D + d;
+#pragma unroll 4
+      for (int j = 0; j < p.splits; ++j) add(__ldcg(reinterpret_cast<const float4*>(po + j * D)), weight[r][(ROWS ? 1 : p.cluster) + j]);
+      if (ROWS || p.cluster == 1) {
+        add(*reinterpret_cast<const float4*>(comb + r * D + d), weight[r][0]);
+      } else {
+        for (int j = 0; j < p.cluster; ++j) add(*cluster.map_shared_rank(reinterpret_cast<const float4*>(comb + r * D + d), j), weight[r][j]);
+      }
+    }
+    uint2 packed = make_uint2(0u, 0u);
+    if (inv != 0.f) {
+      packed.x = pack_bf16(v.x * inv, v.y * inv);
+      packed.y = pack_bf16(v.z * inv, v.w * inv);
+    }
+    *reinterpret_cast<uint2*>(p.out + row * D + d) = packed;
+  }
+  if (!ROWS && p.cluster > 1) cluster.sync();                    // no CTA leaves while its shared memory is read
+}
+
+// ------------------------------------------------------------------------------------------------ host
+template <class K>
+int allow_smem(K kernel, int smem, int (&configured)[64]) {
+  static std::mutex lock;
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev >= 64) return -111;
+  std::lock_guard<std::mutex> guard(lock);
+  if (!configured[dev]) {
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return -112;
+    configured[dev] = 1;
+  }
+  return 0;
+}
+
+// Key splits of the prefix: the smallest estimated time of `waves of items on the SMs` x (key tiles of an item + two tiles' worth
+// of fixed cost per item).
+inline int prefix_splits(long long row_tiles, int Nkv, int n_tiles) {
+  const long long sms = sm_count();
+  long long best = 1LL << 60;
+  int best_s = 1;
+  for (int s = 1; s <= MAX_SPLITS && s <= n_tiles; ++s) {
+    const long long items = row_tiles * Nkv * s, cost = (items + sms - 1) / sms * ((n_tiles + s - 1) / s + 2);
+    if (cost < best) {
+      best = cost;
+      best_s = s;
+    }
+  }
+  return best_s;
+}
+
+struct Shape {
+  int key0, n_tiles, splits;
+};
+inline Shape prefix_shape(int B, int T, int P, int Nq, int Nkv, int window) {
+  Shape s;
+  s.key0 = window > 0 && P > window - 1 ? P - window + 1 : 0;      // the first new token of a sequence sees the most of the prefix
+  s.n_tiles = (P - s.key0 + BN - 1) / BN;
+  const long long rows = (long long)B * T * (Nq / Nkv);
+  s.splits = s.n_tiles > 0 ? prefix_splits((rows + BM - 1) / BM, Nkv, s.n_tiles) : 0;
+  return s;
+}
+
+template <int D, bool FP8>
+int launch_prefix(const CUtensorMap& tk, const CUtensorMap& tv, const Params& p, cudaStream_t stream) {
+  static int configured[64] = {};
+  constexpr int smem = Smem<D, FP8>::BYTES;
+  if (int rc = allow_smem(prefix_kernel<D, FP8>, smem, configured)) return rc;
+  const long long items = ((long long)p.B * p.T * p.rep + BM - 1) / BM * p.Nkv * p.splits;
+  const int sms = sm_count();
+  prefix_kernel<D, FP8><<<unsigned(items < sms ? items : sms), THREADS, smem, stream>>>(tk, tv, p);
+  LYRA_CHECK_LAUNCH();
+  return 0;
+}
+
+template <int D, bool FP8, bool ROWS>
+int launch_own(const OwnParams& p, cudaStream_t stream) {
+  static int configured[64] = {};
+  constexpr int smem = OwnGeo<D, FP8, ROWS>::SMEM_B;
+  if (int rc = allow_smem(own_kernel<D, FP8, ROWS>, smem, configured)) return rc;
+  const long long ctas = (long long)p.B * p.Nkv * p.row_tiles * p.cluster;
+  if (ctas > 0x7fffffffLL) return -113;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(unsigned(ctas));
+  cfg.blockDim = dim3(OTHREADS);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = p.cluster;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if (cudaLaunchKernelEx(&cfg, own_kernel<D, FP8, ROWS>, p) != cudaSuccess) {
+    LYRA_CHECK_LAUNCH();
+    return -114;
+  }
+  return 0;
+}
+
+template <int D>
+int launch_own_d(const OwnParams& p, bool fp8, bool rows, cudaStream_t s) {
+  if (fp8) return rows ? launch_own<D, true, true>(p, s) : launch_own<D, true, false>(p, s);
+  return rows ? launch_own<D, false, true>(p, s) : launch_own<D, false, false>(p, s);
+}
+
+}  // namespace prefix
+}  // namespace lyra
+
+// Bytes of workspace of a call (no initialisation needed).
+extern "C" long long lyra_prefix_attention_workspace(int B, int T, int P, int Nq, int Nkv, int D, int window) {
+  using namespace lyra::prefix;
+  if (B < 1 || T < 1 || P < 0 || Nkv < 1 || Nq < 1 || Nq % Nkv || (D != 64 && D != 128)) return -110;
+  const long long rows = (long long)B * T * Nq;
+  if (rows > (1LL << 30)) return -110;
+  const Shape s = prefix_shape(B, T, P, Nq, Nkv, window);
+  return rows * s.splits * (D * 4 + 8);
+}
+
+// q [B, Nq, T, D] bf16 by element strides (unit inner stride, 16-byte aligned rows); prefix K / V [Nkv, P, D] by (head, position) element
+// strides, bf16 or e4m3 with fp32 scales [Nkv, P] by head stride; own caches [B, Nkv, S, D] contiguous, bf16 or e4m3 with scales
+// [B, Nkv, S]; pos int32 on the device, pos_n (1 or B) values, or null and pos_host; out [B, T, Nq, D] bf16.
+extern "C" int lyra_prefix_attention(const void* q, long long q_sb, long long q_sn, long long q_st, const void* pk, long long pk_sh, long long pk_sp,
+                                     const void* pv, long long pv_sh, long long pv_sp, const float* pk_scale, long long pks_sh, const float* pv_scale,
+                                     long long pvs_sh, int prefix_fp8, const void* k, const void* v, const float* k_scale, const float* v_scale, int own_fp8,
+                                     const float* sinks, const int* pos, int pos_n, int pos_host, void* out, void* workspace, int B, int T, int P, int S,
+                                     int Nq, int Nkv, int D, float scale, int window, int* status, cudaStream_t stream) {
+  using namespace lyra;
+  using namespace lyra::prefix;
+  if (lyra_prefix_attention_workspace(B, T, P, Nq, Nkv, D, window) < 0 || S < 0 || window < 0 || !(scale > 0.f)) return -110;
+  if (pos && pos_n != 1 && pos_n != B) return -110;
+  if ((prefix_fp8 && P > 0 && (!pk_scale || !pv_scale)) || (own_fp8 && S > 0 && (!k_scale || !v_scale))) return -110;
+  const Shape shape = prefix_shape(B, T, P, Nq, Nkv, window);
+  const long long rows = (long long)B * T * Nq;
+  float* part_o = static_cast<float*>(workspace);
+  float2* part_ml = reinterpret_cast<float2*>(part_o + rows * shape.splits * D);
+  const int rep = Nq / Nkv;
+  if (shape.splits > 0) {
+    CUtensorMap tk, tv;
+    const uint64_t esz = prefix_fp8 ? 1 : 2;
+    const CUtensorMapDataType dt = prefix_fp8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+    const CUtensorMapSwizzle swz = prefix_fp8 ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B;
+    const uint64_t dims[3] = {uint64_t(D), uint64_t(P), uint64_t(Nkv)};
+    const uint32_t box[3] = {uint32_t(prefix_fp8 ? D : 64), uint32_t(BN), 1};
+    const uint64_t ks[2] = {uint64_t(pk_sp) * esz, uint64_t(pk_sh) * esz}, vs[2] = {uint64_t(pv_sp) * esz, uint64_t(pv_sh) * esz};
+    if (make_tmap_cached(&tk, pk, dt, 3, dims, ks, box, swz) || make_tmap_cached(&tv, pv, dt, 3, dims, vs, box, swz)) return -115;
+    Params p;
+    p.q = static_cast<const __nv_bfloat16*>(q);
+    p.q_sb = q_sb; p.q_sn = q_sn; p.q_st = q_st;
+    p.pos = pos; p.pos_n = pos_n; p.pos_host = pos_host;
+    p.pk_scale = pk_scale; p.pv_scale = pv_scale; p.pks_sh = pks_sh; p.pvs_sh = pvs_sh;
+    p.part_o = part_o; p.part_ml = part_ml;
+    p.B = B; p.T = T; p.P = P; p.Nq = Nq; p.Nkv = Nkv; p.rep = rep; p.window = window; p.splits = shape.splits; p.key0 = shape.key0;
+    p.scale_log2 = scale * L2E;
+    p.status = status;
+    int rc;
+    if (D == 64) rc = prefix_fp8 ? launch_prefix<64, true>(tk, tv, p, stream) : launch_prefix<64, false>(tk, tv, p, stream);
+    else rc = prefix_fp8 ? launch_prefix<128, true>(tk, tv, p, stream) : launch_prefix<128, false>(tk, tv, p, stream);
+    if (rc) return rc;
+  }
+  OwnParams o;
+  o.q = static_cast<const __nv_bfloat16*>(q);
+  o.q_sb = q_sb; o.q_sn = q_sn; o.q_st = q_st;
+  o.k = static_cast<const uint8_t*>(k); o.v = static_cast<const uint8_t*>(v);
+  o.k_scale = k_scale; o.v_scale = v_scale;
+  o.pos = pos; o.pos_n = pos_n; o.pos_host = pos_host;
+  o.sinks = sinks; o.part_o = part_o; o.part_ml = part_ml;
+  o.out = static_cast<__nv_bfloat16*>(out);
+  o.B = B; o.T = T; o.S = S; o.Nq = Nq; o.Nkv = Nkv; o.rep = rep; o.window = window; o.splits = shape.splits;
+  o.scale_log2 = scale * L2E;
+  const bool by_rows = T * rep > 16;
+  o.row_tiles = by_rows ? (T * rep + 63) / 64 : 1;
+  // One token per sequence, few sequences, long caches: up to eight CTAs share a cache (128 keys each at least) until there are three
+  // for every SM.
+  o.cluster = 1;
+  const int seen = window > 0 && window + T < S ? window + T : S;
+  while (!by_rows && o.cluster < 8 && (long long)B * Nkv * o.cluster * 2 <= 3LL * sm_count() && seen >= o.cluster * 256) o.cluster *= 2;
+  return D == 64 ? launch_own_d<64>(o, own_fp8, by_rows, stream) : launch_own_d<128>(o, own_fp8, by_rows, stream);
+}

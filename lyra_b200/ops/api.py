@@ -113,6 +113,30 @@ def decode_attention(q, k_cache, v_cache, sinks, scale: float, window: int, pos,
     return ref.attention(q, k, v, sinks, scale, window, pos)[0]
 
 
+def prefix_attention(q, prefix_k, prefix_v, k_cache, v_cache, sinks, scale: float, window: int, pos, implementation: str = "auto"):
+    """Attention of a batch whose sequences share a prefix, without a gradient: ``T`` new tokens per sequence over the prefix's keys
+    (stored once, ``prefix_k, prefix_v [Nkv, P, D]``) and the sequence's own cache (``[B, Nkv, S, D]``, the new tokens' keys already
+    written). ``q [B, Nq, T, D]`` -> ``[B, Nq, T, D]``. Prefix and caches are bf16 tensors or e4m3 ``QArray``s with one scale per (head,
+    position), each its own choice.
+
+    ``pos`` is the number of own positions before the new tokens: an int, or an int32 tensor on the device with one value or one per
+    sequence (then the call can be captured and replayed). Query ``t`` stands at absolute position ``P + pos + t``; it sees every key at
+    or before it, with ``window > 0`` the last ``window`` of them. ``sinks [Nq]`` (or None) adds ``exp(sink)`` to the denominator. A sequence
+    with ``pos < 0`` is an unused place of the batch: zeros, as for a query that sees nothing without a sink.
+
+    On a GPU: head dim 64 or 128; the prefix is read once per 128 query rows of a kv head instead of once per sequence."""
+    from lyra_b200.nn.quant import QArray, dequantize
+    from lyra_b200.ops import attention as attn_k
+
+    attn_k.check_prefix_attention(q, prefix_k, prefix_v, k_cache, v_cache, sinks, scale, window, pos)
+    if use_kernels(q, implementation):
+        return attn_k.prefix_attention(q, prefix_k, prefix_v, k_cache, v_cache, sinks, scale, window, pos)
+    full = torch.float64 if q.dtype == torch.float64 else torch.float32
+    plain = lambda t: dequantize(t, full) if isinstance(t, QArray) else t
+    at = pos.reshape(-1).expand(q.shape[0]) if isinstance(pos, torch.Tensor) else torch.full((q.shape[0],), int(pos), device=q.device)
+    return ref.prefix_attention(q, plain(prefix_k), plain(prefix_v), plain(k_cache), plain(v_cache), sinks, scale, window, at)
+
+
 def gate_xsa(t, h, w_gate, v, xsa_alpha, implementation: str = "auto"):
     """SDPA output gate ``t *= 2*sigmoid(h @ W_gate)`` (per token and query head, fp32 logits) followed by
     tanh-XSA ``t -= tanh(alpha_head) * (t . v_hat) * v_hat`` with ``v_hat`` the token's own unit value vector

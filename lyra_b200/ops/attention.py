@@ -5,6 +5,7 @@ from __future__ import annotations
 
 import torch
 
+from lyra_b200.nn.quant import QArray
 from lyra_b200.ops import native
 from lyra_b200.ops.native import c_float, c_int, c_ll, ptr
 
@@ -89,3 +90,97 @@ class FlashAttention(torch.autograd.Function):
 
 def flash_attention(q, k, v, sinks, scale: float, window: int, q_start: int = 0):
     return FlashAttention.apply(q, k, v, sinks, scale, window, q_start)
+
+
+# --------------------------------------------------------------------------- shared prefix (csrc/attn/prefix_attn.cu)
+def check_prefix_attention(q, prefix_k, prefix_v, k_cache, v_cache, sinks, scale: float, window: int, pos) -> None:
+    """Refuses arguments that do not describe a batch with a shared prefix."""
+    if q.ndim != 4 or not q.is_floating_point():
+        raise ValueError(f"q must be a floating-point [B, Nq, T, D], got {tuple(q.shape)} {q.dtype}")
+    B, Nq, T, D = q.shape
+    tensors = [q]
+    for name, kv, lead in (("prefix", (prefix_k, prefix_v), ()), ("own cache", (k_cache, v_cache), (B,))):
+        if isinstance(kv[0], QArray) != isinstance(kv[1], QArray):
+            raise ValueError(f"{name}: keys and values must both be quantised or both not")
+        shape = tuple(kv[0].shape)
+        if tuple(kv[1].shape) != shape or len(shape) != len(lead) + 3 or shape[:-3] != lead or shape[-1] != D or shape[-3] < 1 or Nq % shape[-3]:
+            raise ValueError(f"{name}: keys {shape} and values {tuple(kv[1].shape)} must be {[*lead, 'Nkv', 'positions', D]} with Nkv a divisor of {Nq}")
+        for t in kv:
+            if isinstance(t, QArray):
+                if tuple(t.block) != (1, D) or tuple(t.scale.shape) != (*shape[:-1], 1):
+                    raise ValueError(f"{name}: a quantised cache has blocks (1, {D}), got {t.block} with scales {tuple(t.scale.shape)}")
+                tensors += [t.qval, t.scale]
+            else:
+                tensors.append(t)
+    if prefix_k.shape[0] != k_cache.shape[1]:
+        raise ValueError(f"{prefix_k.shape[0]} kv heads in the prefix, {k_cache.shape[1]} in the caches")
+    if sinks is not None:
+        if tuple(sinks.shape) != (Nq,):
+            raise ValueError(f"sinks {tuple(sinks.shape)} must be [{Nq}]")
+        tensors.append(sinks)
+    if not scale > 0 or window < 0:
+        raise ValueError(f"scale {scale} must be positive and window {window} not negative")
+    if isinstance(pos, torch.Tensor):
+        if pos.dtype not in (torch.int32, torch.int64) or pos.numel() not in (1, B):
+            raise ValueError(f"pos must hold 1 or {B} integers, got {tuple(pos.shape)} {pos.dtype}")
+        tensors.append(pos)
+    elif pos + T > k_cache.shape[2]:
+        raise ValueError(f"{T} tokens from position {pos} on do not fit a cache of {k_cache.shape[2]}")
+    if any(t.device != q.device for t in tensors):
+        raise ValueError(f"all arguments must be on {q.device}")
+    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
+        raise ValueError("prefix_attention has no backward pass: call it under torch.no_grad()")
+
+
+def _rows16(t: torch.Tensor) -> torch.Tensor:
+    """``t`` with unit inner stride and 16-byte steps on every other axis (copied if it is not so already)."""
+    size = t.element_size()
+    if t.numel() and (t.stride(-1) != 1 or t.data_ptr() % 16 or any((s * size) % 16 or s <= 0 for s, n in zip(t.stride()[:-1], t.shape[:-1]) if n > 1)):
+        return t.contiguous() if not t.is_contiguous() else t.clone()
+    return t
+
+
+def prefix_attention(q, prefix_k, prefix_v, k_cache, v_cache, sinks, scale: float, window: int, pos):
+    """CUDA path; the arguments have passed :func:`check_prefix_attention`. The workspace is allocated per call."""
+    B, Nq, T, D = q.shape
+    quant, own_quant = isinstance(prefix_k, QArray), isinstance(k_cache, QArray)
+    pk, pv = (prefix_k.qval, prefix_v.qval) if quant else (prefix_k, prefix_v)
+    kc, vc = (k_cache.qval, v_cache.qval) if own_quant else (k_cache, v_cache)
+    if D not in (64, 128):
+        raise ValueError(f"prefix_attention takes head dim 64 or 128 on a GPU, got {D}")
+    for t, q8 in ((pk, quant), (pv, quant), (kc, own_quant), (vc, own_quant)):
+        if t.dtype != (torch.float8_e4m3fn if q8 else torch.bfloat16):
+            raise ValueError(f"prefix and caches must be bf16, or e4m3 with scales, on a GPU; got {t.dtype}")
+    Nkv, P = pk.shape[0], pk.shape[1]
+    S = kc.shape[2]
+    out = torch.empty(B, T, Nq, D, dtype=torch.bfloat16, device=q.device)
+    if out.numel() == 0:
+        return out.transpose(1, 2).to(q.dtype)
+    lib = native.kernels()
+    with native.on_device(q):
+        qb, pk, pv = _rows16(q.to(torch.bfloat16)), _rows16(pk), _rows16(pv)
+        kc, vc = _rows16(kc.contiguous()), _rows16(vc.contiguous())
+        scales = lambda t, contiguous: (lambda s: s.contiguous() if contiguous or s.stride(1) != 1 else s)(t.scale.float()[..., 0])
+        pks, pvs = (scales(prefix_k, False), scales(prefix_v, False)) if quant and P else (None, None)
+        ks, vs = (scales(k_cache, True), scales(v_cache, True)) if own_quant else (None, None)
+        sk = sinks.float().contiguous() if sinks is not None else None
+        at = pos.reshape(-1).to(torch.int32).contiguous() if isinstance(pos, torch.Tensor) else None
+        lib.lyra_prefix_attention_workspace.restype = c_ll
+        need = lib.lyra_prefix_attention_workspace(B, T, P, Nq, Nkv, D, int(window))
+        if need < 0:
+            raise ValueError(f"prefix_attention does not take B {B}, T {T}, {Nq} / {Nkv} heads on a GPU")
+        ws = torch.empty(max(need, 16), dtype=torch.uint8, device=q.device)
+        rc = lib.lyra_prefix_attention(
+            ptr(qb), c_ll(qb.stride(0)), c_ll(qb.stride(1)), c_ll(qb.stride(2)), ptr(pk), c_ll(_step(pk, 0)), c_ll(_step(pk, 1)), ptr(pv), c_ll(_step(pv, 0)),
+            c_ll(_step(pv, 1)), ptr(pks), c_ll(pks.stride(0) if pks is not None else 0), ptr(pvs), c_ll(pvs.stride(0) if pvs is not None else 0),
+            c_int(int(quant)), ptr(kc), ptr(vc), ptr(ks), ptr(vs), c_int(int(own_quant)), ptr(sk), ptr(at), c_int(at.numel() if at is not None else 0),
+            c_int(int(pos) if at is None else 0), ptr(out), ptr(ws), c_int(B), c_int(T), c_int(P), c_int(S), c_int(Nq), c_int(Nkv), c_int(D),
+            c_float(scale), c_int(int(window)), ptr(native.status_word()), native.stream_ptr())
+    native.check(rc, "lyra_prefix_attention")
+    native.count_launch(2 if P else 1)
+    return out.transpose(1, 2).to(q.dtype)
+
+
+def _step(t: torch.Tensor, axis: int) -> int:
+    """Stride of an axis; an axis of length one has none that matters, but a TMA map wants one it can use."""
+    return t.stride(axis) if t.shape[axis] > 1 else max(t.shape[-1], 16)

@@ -64,6 +64,40 @@ def attention(q, k, v, sinks, scale: float, window: int = 0, q_start=0):
     return out.view(B, Nq, T, D).to(q.dtype), lse.view(B, Nq, T)
 
 
+def prefix_attention(q, prefix_k, prefix_v, k, v, sinks, scale: float, window: int, pos):
+    """Attention over a shared prefix and each sequence's own cache; see ``ops.api.prefix_attention``. ``prefix_k, prefix_v [Nkv, P, D]``,
+    ``k, v [B, Nkv, S, D]``, ``pos`` an integer tensor ``[B]``."""
+    dt = torch.float64 if q.dtype == torch.float64 else torch.float32
+    B, Nq, T, D = q.shape
+    Nkv, P, S = prefix_k.shape[0], prefix_k.shape[1], k.shape[2]
+    rep = Nq // Nkv
+    qf = q.to(dt).reshape(B, Nkv, rep, T, D)
+    own_at = pos.long()[:, None] + torch.arange(T, device=q.device)                                       # [B, T]
+    keys_at = torch.cat([torch.arange(P, device=q.device), P + torch.arange(S, device=q.device)])          # absolute positions
+    visible = keys_at <= (P + own_at)[..., None]
+    if window > 0:
+        visible = visible & (keys_at > (P + own_at)[..., None] - window)
+    visible = (visible & (pos >= 0)[:, None, None])[:, None, None]                                         # [B, 1, 1, T, P + S]
+    s = torch.cat([torch.einsum("bkrtd,kpd->bkrtp", qf, prefix_k.to(dt)), torch.einsum("bkrtd,bksd->bkrts", qf, k.to(dt))], dim=-1) * scale
+    s = s.masked_fill(~visible, float("-inf"))
+    m = s.amax(-1, keepdim=True) if P + S else s.new_full((*s.shape[:-1], 1), float("-inf"))
+    if sinks is not None:
+        sink = sinks.to(dt).view(1, Nkv, rep, 1, 1)
+        m = torch.maximum(m, sink)
+    m = m.masked_fill(m == float("-inf"), 0.0)
+    e = torch.exp(s - m)
+    total = e.sum(-1, keepdim=True)
+    if sinks is not None:
+        total = total + torch.exp(sink - m)
+    # a masked value must not reach a row through 0 * inf; a visible NaN must
+    clean = lambda x, seen: torch.where(seen[..., None], x.to(dt), torch.zeros((), dtype=dt, device=q.device))
+    o = torch.einsum("bkrtp,kpd->bkrtd", e[..., :P], clean(prefix_v, visible[..., :P].any(0).any(-2)[0].expand(Nkv, P)))
+    o = o + torch.einsum("bkrts,bksd->bkrtd", e[..., P:], clean(v, visible[..., P:].any(-2)[:, 0].expand(B, Nkv, S)))
+    out = torch.where(total > 0, o / total, torch.where(total == 0, torch.zeros_like(o), o / total))
+    out = out.masked_fill((pos < 0).view(B, 1, 1, 1, 1), 0.0)
+    return out.reshape(B, Nq, T, D).to(q.dtype)
+
+
 def linear_cross_entropy(x: torch.Tensor, w: torch.Tensor, y: torch.Tensor, vocab_size: int, reduction: str = "sum",
                          chunk: int = 4096):
     """Cross entropy of ``x [T, C] @ w[V, C]^T`` against ``y [T]`` without keeping ``[T, V]`` logits alive:
