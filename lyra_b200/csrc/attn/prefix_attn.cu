@@ -33,6 +33,7 @@ constexpr float L2E = 1.4426950408889634f;
 constexpr int THREADS = 384, LOADERS = 64;      // warps 0, 1 | 2..9 | 10, 11
 constexpr int BM = 128, BN = 128;               // rows and keys of a tile
 constexpr int MAX_SPLITS = 32;
+constexpr int SLOTS = 8;                        // scales of so many key tiles
 
 struct Params {
   const __nv_bfloat16* q;                       // [B, Nq, T, D] by strides (in elements)
@@ -41,8 +42,8 @@ struct Params {
   int pos_n, pos_host;                          // pos == null: pos_host
   const float *pk_scale, *pv_scale;             // e4m3 prefix: [Nkv, P] with head strides
   long long pks_sh, pvs_sh;
-  float* part_o;                                // [B * T * Nq, splits, D] unnormalised
-  float2* part_ml;                              // [B * T * Nq, splits] (maximum in log2 units, sum)
+  float* part_o;                                // [Nkv, row tiles, splits, D, 128] unnormalised: a column's rows side by side
+  float2* part_ml;                              // [Nkv, row tiles, splits, 128] (maximum in log2 units, sum)
   int B, T, P, Nq, Nkv, rep, window, splits, key0;   // key0: first prefix position any row can see
   float scale_log2;
   int* status;
@@ -54,11 +55,29 @@ struct Item {
   int m0, h, split, key, tiles;                 // first row, kv head, first key and number of key tiles
 };
 
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src, int nbytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(nbytes) : "memory");
+}
+// Barrier of the two loader warps that also tells both whether both are well: they leave together or not at all.
+__device__ __forceinline__ bool loaders_agree(bool ok) {
+  uint32_t all;
+  asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbar.red.and.pred q, 2, 64, p;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(all) : "r"(uint32_t(ok)) : "memory");
+  return all != 0;
+}
+__device__ __forceinline__ bool elect_one() {
+  uint32_t one;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(one));
+  return one != 0;
+}
+
 template <int D, bool FP8>
 struct Smem {
   static constexpr int TILE = 128 * D * 2, RAW_TILE = 128 * D;
   static constexpr int RAW = D == 64 ? 4 : 3;   // raw e4m3 tiles in flight (what 227 KB leave room for)
-  static constexpr int BYTES = 5 * TILE + (FP8 ? RAW * RAW_TILE : 0) + 1024;
+  // Score buffers in TMEM and stages of the K and V rings. Head dim 64: two accumulators leave room for a third score buffer, so the
+  // scores of a group's next tile are ready when it finishes one; with two it waits for P V and Q K^T in between.
+  static constexpr int NS = D == 64 ? 3 : 2;
+  static constexpr int BYTES = (1 + 2 * NS) * TILE + (FP8 ? RAW * RAW_TILE : 0) + 1024;
 };
 
 __device__ __forceinline__ uint32_t e4m3x2_to_bf16x2(uint16_t two) {      // exact
@@ -70,18 +89,19 @@ __device__ __forceinline__ uint32_t e4m3x2_to_bf16x2(uint16_t two) {      // exa
 template <int D, bool FP8>
 __global__ void __launch_bounds__(THREADS, 1)
 prefix_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv, const Params p) {
-  constexpr int TILE = Smem<D, FP8>::TILE, RAW_TILE = Smem<D, FP8>::RAW_TILE, RAW = Smem<D, FP8>::RAW;
+  constexpr int TILE = Smem<D, FP8>::TILE, RAW_TILE = Smem<D, FP8>::RAW_TILE, RAW = Smem<D, FP8>::RAW, NS = Smem<D, FP8>::NS;
   constexpr int HALF = 128 * 128;               // bytes of one 64-column block of an operand tile
-  constexpr uint32_t TMEM_COLS = 512, S_COL = 0, O_COL = 256, GROUP_COLS = 128;
+  constexpr uint32_t TMEM_COLS = 512, S_COL = 0, O_COL = NS * 128, O_COLS = NS == 3 ? 64 : 128;
   constexpr uint32_t IDESC_S = make_idesc(BM, BN, 1, 1, 0, 0), IDESC_O = make_idesc(BM, D, 1, 1, 0, 1);
 
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint8_t *sQ = smem, *sK = sQ + TILE, *sV = sK + 2 * TILE, *sR = sV + 2 * TILE;
-  __shared__ uint64_t q_full, q_empty, k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], o_full, o_empty, l_full;
-  __shared__ uint64_t raw_full[RAW], raw_empty[RAW], sc_full[4];
+  uint8_t *sQ = smem, *sK = sQ + TILE, *sV = sK + NS * TILE, *sR = sV + NS * TILE;
+  __shared__ uint64_t q_full, q_empty, k_full[NS], k_empty[NS], v_full[NS], v_empty[NS], s_full[NS], p_full[NS], pv_done[2], o_full, o_empty, l_full;
+  __shared__ uint64_t raw_full[RAW], raw_empty[RAW], sc_full[SLOTS];
   __shared__ float xm[2][2][BM], xl[2][2][BM];  // [item parity][group][row]
-  __shared__ __align__(16) float ksc[FP8 ? 4 : 1][BN], vsc[FP8 ? 4 : 1][BN];   // scales of the key tiles in flight
+  __shared__ __align__(16) float ksc[FP8 ? SLOTS : 1][BN], vsc[FP8 ? SLOTS : 1][BN];   // scales of the key tiles in flight
+  __shared__ long long q_row[BM];
   __shared__ uint32_t tmem_holder;
   __shared__ int abort_flag;
 
@@ -107,7 +127,7 @@ prefix_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CU
   if (threadIdx.x == 0) {
     mbar_init(smem_u32(&q_full), LOADERS);
     mbar_init(smem_u32(&q_empty), 1);
-    for (int s = 0; s < 2; ++s) {
+    for (int s = 0; s < NS; ++s) {
       mbar_init(smem_u32(&k_full[s]), FP8 ? LOADERS : 1);
       mbar_init(smem_u32(&k_empty[s]), 1);
       mbar_init(smem_u32(&v_full[s]), FP8 ? LOADERS : 1);
@@ -119,7 +139,8 @@ prefix_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CU
       mbar_init(smem_u32(&raw_full[s]), 1);
       mbar_init(smem_u32(&raw_empty[s]), LOADERS);
     }
-    for (int s = 0; s < 4; ++s) mbar_init(smem_u32(&sc_full[s]), LOADERS);
+    for (int s = 0; s < SLOTS; ++s) mbar_init(smem_u32(&sc_full[s]), LOADERS);
+    for (int g = 0; g < 2; ++g) mbar_init(smem_u32(&pv_done[g]), 1);
     mbar_init(smem_u32(&l_full), 256);
     mbar_init(smem_u32(&o_full), 1);
     mbar_init(smem_u32(&o_empty), 256);
@@ -133,14 +154,14 @@ prefix_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CU
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = tmem_holder;
+  const uint32_t tmem = __shfl_sync(0xffffffffu, tmem_holder, 0);
   volatile int* abortp = &abort_flag;
   Item w;
 
   // Counters that run across the items (every role advances its own copies the same way; every item has at least one key tile):
-  //   t   key tiles so far: stage t & 1 of the K and V operand tiles, slot t & 3 of the scales
+  //   t   key tiles so far: stage t % NS of the K and V operand tiles, score buffer t % NS (s_full, p_full), slot t % 8 of the scales
   //   n   items so far: parity of q_full / q_empty / o_full / o_empty / l_full
-  //   c_g tiles given to softmax group g so far: parity of s_full[g] / p_full[g]
+  //   c_g tiles given to softmax group g so far: parity of pv_done[g]
   if (warp == 0) {
     if (lane == 0) {
       tma_prefetch_desc(&tk);
@@ -158,7 +179,7 @@ prefix_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CU
               tma_load_3d(smem_u32(sR + s * RAW_TILE), which ? &tv : &tk, smem_u32(&raw_full[s]), 0, k0, w.h);
             }
           } else {
-            const uint32_t s = t & 1, ph = (t >> 1) & 1;
+            const uint32_t s = t % NS, ph = (t / NS) & 1;
             if (!mbar_wait(smem_u32(&k_empty[s]), ph ^ 1, abortp)) { ok = false; break; }
             mbar_expect_tx(smem_u32(&k_full[s]), TILE);
             for (int c = 0; c < D / 64; ++c) tma_load_3d(smem_u32(sK + s * TILE + c * HALF), &tk, smem_u32(&k_full[s]), c * 64, k0, w.h);
@@ -174,53 +195,58 @@ prefix_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CU
       }
     }
   } else if (warp == 1) {
-    if (lane == 0) {
-      // MMAs of one thread retire in issue order: S_g(j + 2), issued after P_g(j) V_j, cannot overwrite P_g(j) before it was read, and
-      // s_full[g] of tile j + 2 tells the group that O_g is quiet until it releases the next P.
-      uint32_t t = 0, n = 0, c[2] = {0, 0};
-      bool ok = true;
-      const uint64_t dq0 = make_smem_desc(smem_u32(sQ), 16, 1024), dk0 = make_smem_desc(smem_u32(sK), 16, 1024);
-      const uint64_t dv0 = make_smem_desc(smem_u32(sV), HALF, 1024);
-      for (int round = 0; ok && item_at(round, w); ++round) {
-        const uint32_t t0 = t;
-        auto issue_s = [&](int j) -> bool {
-          const int g = j & 1, s = (t0 + j) & 1;
-          if (!mbar_wait(smem_u32(&k_full[s]), ((t0 + j) >> 1) & 1, abortp)) return false;
-          tc_fence_after();
-          const uint64_t dk = desc_advance(dk0, s * TILE);
+    // The whole warp walks the tiles and one elected lane issues: the loop's values are then the same in all lanes for the compiler
+    // too and live in uniform registers, from which the MMA takes its descriptors. (With the loop itself inside `lane == 0`, moving
+    // them there took most of 2000 clk per tile; the tensor core needs about 600 for it.)
+    // MMAs of one thread retire in issue order: the scores of tile j + NS, issued after P(j) V_j, cannot overwrite P(j) before it
+    // was read.
+    uint32_t n = 0, ks = 0, kph = 0, vs = 0, vph = 0;       // stage and parity of the next K tile (scores) and of the next V tile
+    bool ok = true;
+    const uint64_t dq0 = make_smem_desc(smem_u32(sQ), 16, 1024), dk0 = make_smem_desc(smem_u32(sK), 16, 1024);
+    const uint64_t dv0 = make_smem_desc(smem_u32(sV), HALF, 1024);
+    for (int round = 0; ok && item_at(round, w); ++round) {
+      auto issue_s = [&](bool last) -> bool {
+        if (!mbar_wait(smem_u32(&k_full[ks]), kph, abortp)) return false;
+        tc_fence_after();
+        if (elect_one()) {
+          const uint64_t dk = desc_advance(dk0, ks * TILE);
 #pragma unroll
           for (int k = 0; k < D / 16; ++k)
-            tc_mma_ss(tmem + S_COL + g * GROUP_COLS, desc_advance(dq0, (k / 4) * HALF + (k % 4) * 32), desc_advance(dk, (k / 4) * HALF + (k % 4) * 32), IDESC_S, k > 0);
-          tc_commit(smem_u32(&s_full[g]));
-          tc_commit(smem_u32(&k_empty[s]));
-          if (j == w.tiles - 1) tc_commit(smem_u32(&q_empty));
-          return true;
-        };
-        ok = mbar_wait(smem_u32(&q_full), n & 1, abortp);
-        if (ok) ok = issue_s(0);
-        if (ok && w.tiles > 1) ok = issue_s(1);
-        if (ok) ok = mbar_wait(smem_u32(&o_empty), (n & 1) ^ 1, abortp);     // the previous item's output has been read
-        for (int j = 0; j < w.tiles && ok; ++j) {
-          const int g = j & 1, s = (t0 + j) & 1;
-          if (!mbar_wait(smem_u32(&v_full[s]), ((t0 + j) >> 1) & 1, abortp)) { ok = false; break; }
-          if (!mbar_wait(smem_u32(&p_full[g]), c[g] & 1, abortp)) { ok = false; break; }
-          ++c[g];
-          tc_fence_after();
-          const uint64_t dv = desc_advance(dv0, s * TILE);
+            tc_mma_ss(tmem + S_COL + ks * 128, desc_advance(dq0, (k / 4) * HALF + (k % 4) * 32), desc_advance(dk, (k / 4) * HALF + (k % 4) * 32), IDESC_S, k > 0);
+          tc_commit(smem_u32(&s_full[ks]));
+          tc_commit(smem_u32(&k_empty[ks]));
+          if (last) tc_commit(smem_u32(&q_empty));
+        }
+        __syncwarp();
+        if (++ks == NS) { ks = 0; kph ^= 1; }
+        return true;
+      };
+      ok = mbar_wait(smem_u32(&q_full), n & 1, abortp);
+      for (int j = 0; ok && j < NS && j < w.tiles; ++j) ok = issue_s(j == w.tiles - 1);
+      if (ok) ok = mbar_wait(smem_u32(&o_empty), (n & 1) ^ 1, abortp);       // the previous item's output has been read
+      for (int j = 0; j < w.tiles && ok; ++j) {
+        const int g = j & 1;
+        if (!mbar_wait(smem_u32(&v_full[vs]), vph, abortp)) { ok = false; break; }
+        if (!mbar_wait(smem_u32(&p_full[vs]), vph, abortp)) { ok = false; break; }
+        tc_fence_after();
+        if (elect_one()) {
+          const uint64_t dv = desc_advance(dv0, vs * TILE);
 #pragma unroll
           for (int k = 0; k < BN / 16; ++k)
-            tc_mma_ts(tmem + O_COL + g * GROUP_COLS, tmem + S_COL + g * GROUP_COLS + k * 8, desc_advance(dv, k * 2048), IDESC_O, (j >= 2 || k > 0) ? 1u : 0u);
-          tc_commit(smem_u32(&v_empty[s]));
-          if (j + 2 < w.tiles) ok = issue_s(j + 2);
+            tc_mma_ts(tmem + O_COL + g * O_COLS, tmem + S_COL + vs * 128 + k * 8, desc_advance(dv, k * 2048), IDESC_O, (j >= 2 || k > 0) ? 1u : 0u);
+          tc_commit(smem_u32(&v_empty[vs]));
+          tc_commit(smem_u32(&pv_done[g]));
+          if (j == w.tiles - 1) tc_commit(smem_u32(&o_full));
         }
-        if (ok) tc_commit(smem_u32(&o_full));
-        t += w.tiles;
-        ++n;
+        __syncwarp();
+        if (++vs == NS) { vs = 0; vph ^= 1; }
+        if (j + NS < w.tiles) ok = issue_s(j + NS == w.tiles - 1);
       }
-      if (!ok) {
-        atomicCAS(p.status, 0, STATUS_TIMEOUT_FULL);
-        abort_flag = 1;
-      }
+      ++n;
+    }
+    if (!ok) {
+      if (lane == 0) atomicCAS(p.status, 0, STATUS_TIMEOUT_FULL);
+      abort_flag = 1;
     }
   } else if (warp >= 10) {
     // ------------------------------------------------------------ query rows; e4m3 tiles to bf16
@@ -228,25 +254,32 @@ prefix_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CU
     constexpr int CPR = D / 8;                  // 16-byte chunks per query row
     uint32_t t = 0, n = 0;
     bool ok = true;
-    for (int round = 0; ok && item_at(round, w); ++round, ++n) {
-      if (!mbar_wait(smem_u32(&q_empty), (n & 1) ^ 1, abortp)) { ok = false; break; }
-#pragma unroll 4
-      for (int i = tid; i < BM * CPR; i += LOADERS) {
-        const int r = i / CPR, c = i % CPR, m = w.m0 + r;
-        uint4 v = make_uint4(0u, 0u, 0u, 0u);
-        if (m < M) {
-          const int bt = m / p.rep, b = bt / p.T;
-          v = __ldg(reinterpret_cast<const uint4*>(p.q + b * p.q_sb + (long long)(w.h * p.rep + m - bt * p.rep) * p.q_sn + (long long)(bt - b * p.T) * p.q_st) + c);
-        }
-        *reinterpret_cast<uint4*>(sQ + (c >> 3) * HALF + swz128(r, c & 7)) = v;
+    for (int round = 0; item_at(round, w); ++round, ++n) {
+#pragma unroll
+      for (int r = tid; r < BM; r += LOADERS) {              // where each row of the item starts, in elements; -1: past the last row
+        const int m = w.m0 + r, bt = m / p.rep, b = bt / p.T;
+        q_row[r] = m < M ? b * p.q_sb + (long long)(w.h * p.rep + m - bt * p.rep) * p.q_sn + (long long)(bt - b * p.T) * p.q_st : -1;
       }
+      if (!(ok = loaders_agree(ok))) break;
+      if (!mbar_wait(smem_u32(&q_empty), (n & 1) ^ 1, abortp)) ok = false;
+      if (ok) {
+#pragma unroll 8
+        for (int i = tid; i < BM * CPR; i += LOADERS) {
+          const int r = i / CPR, c = i % CPR;
+          const long long at = q_row[r];
+          cp16(smem_u32(sQ + (c >> 3) * HALF + swz128(r, c & 7)), p.q + (at < 0 ? 0 : at + c * 8), at < 0 ? 0 : 16);
+        }
+        asm volatile("cp.async.wait_all;" ::: "memory");
+      }
+      if (!(ok = loaders_agree(ok))) break;                  // the table is rewritten for the next item after this
       fence_proxy_async_smem();
       mbar_arrive(smem_u32(&q_full));
       if (FP8) {
         for (int j = 0; ok && j < w.tiles; ++j, ++t) {
-          const uint32_t s = t & 1, ph = (t >> 1) & 1;
+          const uint32_t s = t % NS, ph = (t / NS) & 1;
           const int k0 = w.key + j * BN;
-          // slot t & 3 is free: tile t - 4 left softmax before the operand stage of tile t - 2 was released
+          // slot t % 8 is free: the stage of tile t is, so the scores of tile t - NS are done; they were asked for after the
+          // probabilities of tile t - 2 NS, and those came after the group was through with tile t - 8
           for (int which = 0; which < 2; ++which) {
             const uint32_t i = 2 * t + which, rs = i % RAW;
             if (!mbar_wait(smem_u32(which ? &v_empty[s] : &k_empty[s]), ph ^ 1, abortp) || !mbar_wait(smem_u32(&raw_full[rs]), (i / RAW) & 1, abortp)) {
@@ -276,10 +309,10 @@ prefix_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CU
               for (int y = 0; y < BN / LOADERS; ++y) {
                 const int key = k0 + tid + y * LOADERS;
                 const bool in = key < p.P;      // 1 past the end: those scores are masked, -inf * 0 would not be -inf
-                ksc[t & 3][tid + y * LOADERS] = in ? __ldg(p.pk_scale + w.h * p.pks_sh + key) * p.scale_log2 : 1.f;
-                vsc[t & 3][tid + y * LOADERS] = in ? __ldg(p.pv_scale + w.h * p.pvs_sh + key) : 1.f;
+                ksc[t % SLOTS][tid + y * LOADERS] = in ? __ldg(p.pk_scale + w.h * p.pks_sh + key) * p.scale_log2 : 1.f;
+                vsc[t % SLOTS][tid + y * LOADERS] = in ? __ldg(p.pv_scale + w.h * p.pvs_sh + key) : 1.f;
               }
-              mbar_arrive(smem_u32(&sc_full[t & 3]));
+              mbar_arrive(smem_u32(&sc_full[t % SLOTS]));
             }
             fence_proxy_async_smem();
             mbar_arrive(smem_u32(&raw_empty[rs]));
@@ -298,9 +331,9 @@ prefix_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CU
     const int row = quarter * 32 + lane;        // row of the tile == TMEM lane
     const uint32_t lane_addr = uint32_t(quarter * 32) << 16;
     const int g = (warp - 2) >> 2;              // group 0: key tiles 0, 2, ...; group 1: 1, 3, ...
-    const uint32_t s_addr = tmem + lane_addr + S_COL + g * GROUP_COLS, o_addr = tmem + lane_addr + O_COL + g * GROUP_COLS;
+    const uint32_t o_addr = tmem + lane_addr + O_COL + g * O_COLS;
     const float sc = p.scale_log2;
-    uint32_t t = 0, n = 0, cg_ = 0;
+    uint32_t t = 0, n = 0, done = 0;            // done: tiles of this group so far
     bool failed = false;
 
     for (int round = 0; !failed && item_at(round, w); ++round) {
@@ -310,17 +343,17 @@ prefix_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CU
       const int lo = p.window > 0 && row_valid ? p.P + position(p.pos, p.pos_n, p.pos_host, b) + (bt - b * p.T) - p.window + 1 : 0;   // first visible key
       float m = -INFINITY, l = 0.f;
 
-      for (int j = g; j < w.tiles; j += 2, ++cg_) {
+      for (int j = g; j < w.tiles; j += 2, ++done) {
         const int k0 = w.key + j * BN;
-        const uint32_t slot = (t + j) & 3;
-        if (FP8 && !mbar_wait(smem_u32(&sc_full[slot]), ((t + j) >> 2) & 1, abortp)) { failed = true; break; }
-        if (!mbar_wait(smem_u32(&s_full[g]), cg_ & 1, abortp)) { failed = true; break; }
+        const uint32_t slot = (t + j) % SLOTS, sb = (t + j) % NS;
+        const uint32_t s_addr = tmem + lane_addr + S_COL + sb * 128;
+        if (FP8 && !mbar_wait(smem_u32(&sc_full[slot]), ((t + j) / SLOTS) & 1, abortp)) { failed = true; break; }
+        if (!mbar_wait(smem_u32(&s_full[sb]), ((t + j) / NS) & 1, abortp)) { failed = true; break; }
         tc_fence_after();
         if (!warp_idle) {                       // rows past the last one keep whatever their lanes hold: no other row sees it
           const bool need_mask = k0 + BN > p.P || (p.window > 0);
-          auto load = [&](int c, uint32_t (&r)[32]) {
-            tmem_ld32(s_addr + c * 32, r);
-            tmem_ld_wait();
+          // scores as they enter the softmax: times the key's scale (e4m3), -inf where the row must not look
+          auto prepare = [&](int c, uint32_t (&r)[32]) {
             if (FP8) {
 #pragma unroll
               for (int i = 0; i < 32; i += 4) {
@@ -346,36 +379,46 @@ prefix_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CU
 #pragma unroll 1
             for (int c = 0; c < 4; ++c) {
               uint32_t r[32];
-              load(c, r);
+              tmem_ld32(s_addr + c * 32, r);
+              tmem_ld_wait();
+              prepare(c, r);
 #pragma unroll
               for (int i = 0; i < 32; ++i) mx = fmaxf(mx, __uint_as_float(r[i]));
             }
             if (m == -INFINITY) m = mx * s2;
           }
           // One pass in the common case: probabilities against the current reference while the tile's maximum is tracked; redone
-          // (the scores are still in TMEM) when a row has to move its reference by more than 2^8.
-          float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY}, sum4[4] = {0.f, 0.f, 0.f, 0.f};
+          // (the scores are still in TMEM) when a row has to move its reference by more than 2^8. The next quarter of the scores is
+          // on its way while one is exponentiated.
+          float mx4[4], sum4[4];
           uint32_t pk[2][32];
           float ref = m == -INFINITY ? 0.f : m;
-          auto quarter_pass = [&](int c, bool track) {
-            uint32_t r[32];
-            load(c, r);
+          auto pass = [&]() {
+            uint32_t r[2][32];
+            tmem_ld32(s_addr, r[0]);
 #pragma unroll
-            for (int i = 0; i < 32; i += 2) {
-              const float a = __uint_as_float(r[i]), d = __uint_as_float(r[i + 1]);
-              if (track) mx4[c] = fmaxf(mx4[c], fmaxf(a, d));
-              float p0 = exp2f(fmaf(a, s2, -ref)), p1 = exp2f(fmaf(d, s2, -ref));
-              sum4[c] += p0 + p1;
-              if (FP8) {
-                const float2 f = *reinterpret_cast<const float2*>(&vsc[slot][c * 32 + i]);
-                p0 *= f.x;
-                p1 *= f.y;
+            for (int c = 0; c < 4; ++c) {
+              tmem_ld_wait();
+              if (c < 3) tmem_ld32(s_addr + (c + 1) * 32, r[(c + 1) & 1]);
+              prepare(c, r[c & 1]);
+              mx4[c] = -INFINITY;
+              sum4[c] = 0.f;
+#pragma unroll
+              for (int i = 0; i < 32; i += 2) {
+                const float a = __uint_as_float(r[c & 1][i]), d = __uint_as_float(r[c & 1][i + 1]);
+                mx4[c] = fmaxf(mx4[c], fmaxf(a, d));
+                float p0 = exp2f(fmaf(a, s2, -ref)), p1 = exp2f(fmaf(d, s2, -ref));
+                sum4[c] += p0 + p1;
+                if (FP8) {
+                  const float2 f = *reinterpret_cast<const float2*>(&vsc[slot][c * 32 + i]);
+                  p0 *= f.x;
+                  p1 *= f.y;
+                }
+                pk[c >> 1][(c & 1) * 16 + (i >> 1)] = pack_bf16(p0, p1);
               }
-              pk[c >> 1][(c & 1) * 16 + (i >> 1)] = pack_bf16(p0, p1);
             }
           };
-#pragma unroll
-          for (int c = 0; c < 4; ++c) quarter_pass(c, true);
+          pass();
           const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * s2;
           if (__any_sync(0xffffffffu, mx > ref + 8.f)) {
             float factor = 1.f;
@@ -384,7 +427,9 @@ prefix_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CU
               m = ref = mx;
             }
             l *= factor;
-            if (j >= 2) {                       // O_g holds tiles j - 2, j - 4, ...: all retired (see the issuer)
+            if (j >= 2) {                       // O_g holds tiles j - 2, j - 4, ...: wait until the last of them has been added
+              if (!mbar_wait(smem_u32(&pv_done[g]), (done - 1) & 1, abortp)) abort_flag = 1;
+              tc_fence_after();
 #pragma unroll 1
               for (int c = 0; c < D / 32; ++c) {
                 uint32_t o[32];
@@ -395,9 +440,7 @@ prefix_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CU
                 tmem_st32(o_addr + c * 32, o);
               }
             }
-            sum4[0] = sum4[1] = sum4[2] = sum4[3] = 0.f;
-#pragma unroll
-            for (int c = 0; c < 4; ++c) quarter_pass(c, false);
+            pass();
           }
           tmem_st32(s_addr, pk[0]);
           tmem_st32(s_addr + 32, pk[1]);
@@ -405,7 +448,7 @@ prefix_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CU
           l += (sum4[0] + sum4[1]) + (sum4[2] + sum4[3]);
         }
         tc_fence_before();
-        mbar_arrive(smem_u32(&p_full[g]));
+        mbar_arrive(smem_u32(&p_full[sb]));
       }
       if (failed) break;
       t += w.tiles;
@@ -423,34 +466,23 @@ prefix_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CU
       const float mt = fmaxf(m0, m1);
       const float a0 = m0 == -INFINITY ? 0.f : exp2f(m0 - mt), a1 = m1 == -INFINITY ? 0.f : exp2f(m1 - mt);
       const float lt = a0 * xl[par][0][row] + (two ? a1 * xl[par][1][row] : 0.f);
-      const long long out_row = ((long long)bt * p.Nq + w.h * p.rep + (m_row - bt * p.rep)) * p.splits + w.split;
+      const long long part = ((long long)w.h * n_mt + w.m0 / BM) * p.splits + w.split;
       if (!warp_idle) {
+        float* dst = p.part_o + part * D * BM + row;         // the warp's 32 rows of one column make one 128-byte store
 #pragma unroll 1
-        for (int c = g; c < D / 32; c += 2) {   // each group writes half of the columns
+        for (int c = g; c < D / 32; c += 2) {                // each group writes half of the columns
           uint32_t r0[32], r1[32];
           tmem_ld32(tmem + lane_addr + O_COL + c * 32, r0);
-          if (two) tmem_ld32(tmem + lane_addr + O_COL + GROUP_COLS + c * 32, r1);
+          if (two) tmem_ld32(tmem + lane_addr + O_COL + O_COLS + c * 32, r1);
           tmem_ld_wait();
-          if (row_valid) {
-            float* dst = p.part_o + out_row * D + c * 32;
 #pragma unroll
-            for (int i = 0; i < 32; i += 4) {
-              float4 v;
-              v.x = __uint_as_float(r0[i]) * a0;
-              v.y = __uint_as_float(r0[i + 1]) * a0;
-              v.z = __uint_as_float(r0[i + 2]) * a0;
-              v.w = __uint_as_float(r0[i + 3]) * a0;
-              if (two) {
-                v.x = fmaf(__uint_as_float(r1[i]), a1, v.x);
-                v.y = fmaf(__uint_as_float(r1[i + 1]), a1, v.y);
-                v.z = fmaf(__uint_as_float(r1[i + 2]), a1, v.z);
-                v.w = fmaf(__uint_as_float(r1[i + 3]), a1, v.w);
-              }
-              *reinterpret_cast<float4*>(dst + i) = v;
-            }
+          for (int i = 0; i < 32; ++i) {
+            float v = __uint_as_float(r0[i]) * a0;
+            if (two) v = fmaf(__uint_as_float(r1[i]), a1, v);
+            dst[(c * 32 + i) * BM] = v;
           }
         }
-        if (row_valid && g == 0) p.part_ml[out_row] = make_float2(mt, lt);
+        if (g == 0) p.part_ml[part * BM + row] = make_float2(mt, lt);
       }
       tc_fence_before();
       mbar_arrive(smem_u32(&o_empty));
@@ -488,13 +520,10 @@ struct OwnParams {
   const float* part_o;                          // prefix partials (splits > 0)
   const float2* part_ml;
   __nv_bfloat16* out;                           // [B, T, Nq, D]
-  int B, T, S, Nq, Nkv, rep, window, splits, row_tiles, cluster;
+  int B, T, S, Nq, Nkv, rep, window, splits, row_tiles, cluster, prefix_tiles;
   float scale_log2;
 };
 
-__device__ __forceinline__ void cp16(uint32_t dst, const void* src, int nbytes) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(nbytes) : "memory");
-}
 __device__ __forceinline__ void cp4(uint32_t dst, const void* src, int nbytes) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(nbytes) : "memory");
 }
@@ -524,7 +553,8 @@ struct OwnGeo {
   static constexpr int STAGE_B = 2 * RAW_B + 2 * TK * 4;         // + scales
   static constexpr int RING_B = OSTAGES * STAGE_B + (FP8 ? 2 * TILE_B : 0);
   static constexpr int ROWS_CTA = ROWS ? 64 : 16;
-  static constexpr int COMB_B = ROWS_CTA * D * 4, WARP_O_B = ROWS ? 0 : OWARPS * 16 * D * 4;
+  static constexpr int PITCH = D + 4;                            // floats per row of the partial results: rows start in different banks
+  static constexpr int COMB_B = ROWS_CTA * PITCH * 4, WARP_O_B = ROWS ? 0 : OWARPS * 16 * PITCH * 4;
   static constexpr int RINGS_B = (ROWS ? 1 : OWARPS) * RING_B;
   static constexpr int SMEM_B = RINGS_B > COMB_B + WARP_O_B ? RINGS_B : COMB_B + WARP_O_B;
 };
@@ -532,14 +562,14 @@ struct OwnGeo {
 template <int D, bool FP8, bool ROWS>
 __global__ void __launch_bounds__(OTHREADS) own_kernel(const OwnParams p) {
   using G_ = OwnGeo<D, FP8, ROWS>;
-  constexpr int TK = G_::TK, ROWB = G_::ROWB, TILE_B = G_::TILE_B, RAW_B = G_::RAW_B, STAGE_B = G_::STAGE_B, RC = G_::ROWS_CTA;
+  constexpr int TK = G_::TK, ROWB = G_::ROWB, TILE_B = G_::TILE_B, RAW_B = G_::RAW_B, STAGE_B = G_::STAGE_B, RC = G_::ROWS_CTA, PITCH = G_::PITCH;
   constexpr int ESZ = FP8 ? 1 : 2, LT = ROWS ? OTHREADS : 32;    // threads that fill one ring
   constexpr int MAXW = 8 + MAX_SPLITS;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ float red_m[OWARPS * 16], red_l[OWARPS * 16];       // per warp and row
   __shared__ float comb_m[RC], comb_l[RC], weight[RC][MAXW + 1];
-  float* comb = reinterpret_cast<float*>(smem);                  // [RC][D], after the key loop
-  float* warp_o = comb + RC * D;                                 // [OWARPS][16][D]
+  float* comb = reinterpret_cast<float*>(smem);                  // [RC][PITCH], after the key loop
+  float* warp_o = comb + RC * PITCH;                             // [OWARPS][16][PITCH]
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, lt = ROWS ? tid : lane;
   const int rank = int(blockIdx.x) % p.cluster;
@@ -724,12 +754,12 @@ __global__ void __launch_bounds__(OTHREADS) own_kernel(const OwnParams p) {
 
   // ---- the CTA's partial result in comb / comb_m / comb_l
   {
-    float* dst = ROWS ? comb + warp * 16 * D : warp_o + warp * 16 * D;
+    float* dst = (ROWS ? comb : warp_o) + warp * 16 * PITCH;
     const int r0 = lane >> 2, c = (lane & 3) * 2;
 #pragma unroll
     for (int d = 0; d < D / 8; ++d) {
-      *reinterpret_cast<float2*>(dst + r0 * D + d * 8 + c) = make_float2(o[d][0], o[d][1]);
-      *reinterpret_cast<float2*>(dst + (r0 + 8) * D + d * 8 + c) = make_float2(o[d][2], o[d][3]);
+      *reinterpret_cast<float2*>(dst + r0 * PITCH + d * 8 + c) = make_float2(o[d][0], o[d][1]);
+      *reinterpret_cast<float2*>(dst + (r0 + 8) * PITCH + d * 8 + c) = make_float2(o[d][2], o[d][3]);
     }
     if ((lane & 3) == 0) {
 #pragma unroll
@@ -757,9 +787,9 @@ __global__ void __launch_bounds__(OTHREADS) own_kernel(const OwnParams p) {
       for (int x = 0; x < OWARPS; ++x) {
         const float mw = red_m[x * 16 + r], f = mw == -INFINITY ? 0.f : exp2f(mw - M);
         L += red_l[x * 16 + r] * f;
-        O += warp_o[(x * 16 + r) * D + d] * f;
+        O += warp_o[(x * 16 + r) * PITCH + d] * f;
       }
-      comb[r * D + d] = O;
+      comb[r * PITCH + d] = O;
       if (d == 0) {
         comb_m[r] = M;
         comb_l[r] = L;
@@ -774,10 +804,11 @@ __global__ void __launch_bounds__(OTHREADS) own_kernel(const OwnParams p) {
   constexpr int TPR = OTHREADS / RC;                             // threads per row
   {
     const int r = tid / TPR, x = tid % TPR, n_own = ROWS ? 1 : p.cluster, n = n_own + p.splits;
-    const long long row = r < n_rows ? out_row(r) : 0;
+    const int mrow = b * R + row0 + (r < n_rows ? r : 0);      // row of the prefix product
+    const float2* prefix_ml = p.part_ml + ((long long)h * p.prefix_tiles + mrow / BM) * p.splits * BM + mrow % BM;
     float M = -INFINITY, L = 0.f;
     auto ml = [&](int j) -> float2 {
-      if (j >= n_own) return __ldcg(p.part_ml + row * p.splits + (j - n_own));
+      if (j >= n_own) return __ldcg(prefix_ml + (j - n_own) * BM);
       if (ROWS || p.cluster == 1) return make_float2(comb_m[r], comb_l[r]);
       return make_float2(*cluster.map_shared_rank(&comb_m[r], j), *cluster.map_shared_rank(&comb_l[r], j));
     };
@@ -801,35 +832,38 @@ __global__ void __launch_bounds__(OTHREADS) own_kernel(const OwnParams p) {
   }
   __syncthreads();
 
-  // ---- output, four columns per thread; the CTAs of a cluster share the rows' columns
-  constexpr int Q = D / 4;
-  for (int i = rank * OTHREADS + tid; i < n_rows * Q; i += p.cluster * OTHREADS) {
-    const int r = i / Q, d = (i % Q) * 4;
+  auto finish = [&](int r, int d, float v) -> float {             // + the prefix's splits, times 1 / L
     const float inv = weight[r][MAXW];
-    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-    auto add = [&](const float4& x, float f) {
-      v.x = fmaf(x.x, f, v.x);
-      v.y = fmaf(x.y, f, v.y);
-      v.z = fmaf(x.z, f, v.z);
-      v.w = fmaf(x.w, f, v.w);
-    };
-    const long long row = out_row(r);
-    if (!idle) {
-      const float* po = p.part_o + row * p.splits * D + d;
-#pragma unroll 4
-      for (int j = 0; j < p.splits; ++j) add(__ldcg(reinterpret_cast<const float4*>(po + j * D)), weight[r][(ROWS ? 1 : p.cluster) + j]);
-      if (ROWS || p.cluster == 1) {
-        add(*reinterpret_cast<const float4*>(comb + r * D + d), weight[r][0]);
-      } else {
-        for (int j = 0; j < p.cluster; ++j) add(*cluster.map_shared_rank(reinterpret_cast<const float4*>(comb + r * D + d), j), weight[r][j]);
-      }
+    if (inv == 0.f) return 0.f;                                  // nothing visible, or an unused place: whatever the sums hold
+    const int mrow = b * R + row0 + r;
+    const float* po = p.part_o + (((long long)h * p.prefix_tiles + mrow / BM) * p.splits * D + d) * BM + mrow % BM;
+    const float* wp = &weight[r][ROWS ? 1 : p.cluster];
+#pragma unroll 8
+    for (int j = 0; j < p.splits; ++j) v = fmaf(__ldcg(po + (long long)j * D * BM), wp[j], v);
+    return v * inv;
+  };
+  // ---- sums, a row's columns dealt to the CTAs of a cluster. Neighbouring threads take neighbouring rows, which lie side by side in
+  // the prefix partials; the results go through shared memory (over this CTA's own partial) and leave row by row.
+  const int dn = D / p.cluster, d0 = rank * dn;                  // this CTA's columns
+  if (ROWS || p.cluster == 1) {
+    for (int i = tid; i < n_rows * D; i += OTHREADS) {
+      const int d = i / n_rows, r = i - d * n_rows;
+      comb[r * PITCH + d] = finish(r, d, comb[r * PITCH + d] * weight[r][0]);
     }
-    uint2 packed = make_uint2(0u, 0u);
-    if (inv != 0.f) {
-      packed.x = pack_bf16(v.x * inv, v.y * inv);
-      packed.y = pack_bf16(v.z * inv, v.w * inv);
+  } else {
+    for (int i = tid; i < n_rows * dn; i += OTHREADS) {
+      const int d = d0 + i / n_rows, r = i % n_rows;
+      float v = 0.f;
+      for (int j = 0; j < p.cluster; ++j) v += *cluster.map_shared_rank(comb + r * PITCH + d, j) * weight[r][j];
+      warp_o[r * PITCH + d] = finish(r, d, v);
     }
-    *reinterpret_cast<uint2*>(p.out + row * D + d) = packed;
+  }
+  __syncthreads();
+  const float* done = ROWS || p.cluster == 1 ? comb : warp_o;
+  for (int i = tid; i < n_rows * (dn / 8); i += OTHREADS) {
+    const int r = i / (dn / 8), d = d0 + i % (dn / 8) * 8;
+    const float4 x = *reinterpret_cast<const float4*>(done + r * PITCH + d), y = *reinterpret_cast<const float4*>(done + r * PITCH + d + 4);
+    *reinterpret_cast<uint4*>(p.out + out_row(r) * D + d) = make_uint4(pack_bf16(x.x, x.y), pack_bf16(x.z, x.w), pack_bf16(y.x, y.y), pack_bf16(y.z, y.w));
   }
   if (!ROWS && p.cluster > 1) cluster.sync();                    // no CTA leaves while its shared memory is read
 }
@@ -930,7 +964,8 @@ extern "C" long long lyra_prefix_attention_workspace(int B, int T, int P, int Nq
   const long long rows = (long long)B * T * Nq;
   if (rows > (1LL << 30)) return -110;
   const Shape s = prefix_shape(B, T, P, Nq, Nkv, window);
-  return rows * s.splits * (D * 4 + 8);
+  const long long tiles = (rows / Nkv + BM - 1) / BM * Nkv;
+  return tiles * BM * s.splits * (D * 4 + 8);
 }
 
 // q [B, Nq, T, D] bf16 by element strides (unit inner stride, 16-byte aligned rows); prefix K / V [Nkv, P, D] by (head, position) element
@@ -947,10 +982,9 @@ extern "C" int lyra_prefix_attention(const void* q, long long q_sb, long long q_
   if (pos && pos_n != 1 && pos_n != B) return -110;
   if ((prefix_fp8 && P > 0 && (!pk_scale || !pv_scale)) || (own_fp8 && S > 0 && (!k_scale || !v_scale))) return -110;
   const Shape shape = prefix_shape(B, T, P, Nq, Nkv, window);
-  const long long rows = (long long)B * T * Nq;
+  const int rep = Nq / Nkv, prefix_tiles = int(((long long)B * T * rep + BM - 1) / BM);
   float* part_o = static_cast<float*>(workspace);
-  float2* part_ml = reinterpret_cast<float2*>(part_o + rows * shape.splits * D);
-  const int rep = Nq / Nkv;
+  float2* part_ml = reinterpret_cast<float2*>(part_o + (long long)prefix_tiles * Nkv * BM * shape.splits * D);
   if (shape.splits > 0) {
     CUtensorMap tk, tv;
     const uint64_t esz = prefix_fp8 ? 1 : 2;
@@ -982,7 +1016,7 @@ extern "C" int lyra_prefix_attention(const void* q, long long q_sb, long long q_
   o.pos = pos; o.pos_n = pos_n; o.pos_host = pos_host;
   o.sinks = sinks; o.part_o = part_o; o.part_ml = part_ml;
   o.out = static_cast<__nv_bfloat16*>(out);
-  o.B = B; o.T = T; o.S = S; o.Nq = Nq; o.Nkv = Nkv; o.rep = rep; o.window = window; o.splits = shape.splits;
+  o.B = B; o.T = T; o.S = S; o.Nq = Nq; o.Nkv = Nkv; o.rep = rep; o.window = window; o.splits = shape.splits; o.prefix_tiles = prefix_tiles;
   o.scale_log2 = scale * L2E;
   const bool by_rows = T * rep > 16;
   o.row_tiles = by_rows ? (T * rep + 63) / 64 : 1;
