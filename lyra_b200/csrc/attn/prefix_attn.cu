@@ -33,6 +33,7 @@ constexpr float L2E = 1.4426950408889634f;
 constexpr int THREADS = 384, LOADERS = 64;      // warps 0, 1 | 2..9 | 10, 11
 constexpr int BM = 128, BN = 128;               // rows and keys of a tile
 constexpr int MAX_SPLITS = 32;
+constexpr int POLY_AT = 6;                      // place in a run of eight scores of the pair that is exponentiated by polynomial
 constexpr int SLOTS = 8;                        // scales of so many key tiles
 
 struct Params {
@@ -63,6 +64,41 @@ __device__ __forceinline__ bool loaders_agree(bool ok) {
   uint32_t all;
   asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbar.red.and.pred q, 2, 64, p;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(all) : "r"(uint32_t(ok)) : "memory");
   return all != 0;
+}
+// Two fp32 operations per instruction.
+__device__ __forceinline__ uint64_t pair(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void unpair(uint64_t v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+// 2^x of both halves without the special-function unit (16 results per clock and SM, 1024 clk for a 128 x 128 tile): x = n + f with n the
+// nearest integer (adding 1.5 * 2^23 leaves it in the low bits), 2^f by the polynomial of degree 4 with the smallest largest relative
+// error on [-1/2, 1/2] (2.7e-6, fitted by reweighted least squares), n added to the exponent. Inputs below -126 give 2^-126.
+__device__ __forceinline__ uint64_t exp2_poly(uint64_t x) {
+  float a, b;
+  unpair(x, a, b);
+  x = pair(fmaxf(a, -126.f), fmaxf(b, -126.f));
+  const uint64_t magic = pair(12582912.f, 12582912.f), minus = pair(-12582912.f, -12582912.f), one = pair(-1.f, -1.f);
+  const uint64_t t = add2(x, magic), f = fma2(add2(t, minus), one, x);
+  uint64_t y = fma2(f, pair(0.009570079855620861f, 0.009570079855620861f), pair(0.05591783672571182f, 0.05591783672571182f));
+  y = fma2(y, f, pair(0.240247443318367f, 0.240247443318367f));
+  y = fma2(y, f, pair(0.6931217908859253f, 0.6931217908859253f));
+  y = fma2(y, f, pair(0.9999992847442627f, 0.9999992847442627f));
+  float ta, tb, ya, yb;
+  unpair(t, ta, tb);
+  unpair(y, ya, yb);
+  return pair(__uint_as_float(__float_as_uint(ya) + (__float_as_uint(ta) << 23)), __uint_as_float(__float_as_uint(yb) + (__float_as_uint(tb) << 23)));
 }
 __device__ __forceinline__ bool elect_one() {
   uint32_t one;
@@ -97,7 +133,7 @@ prefix_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CU
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t *sQ = smem, *sK = sQ + TILE, *sV = sK + NS * TILE, *sR = sV + NS * TILE;
-  __shared__ uint64_t q_full, q_empty, k_full[NS], k_empty[NS], v_full[NS], v_empty[NS], s_full[NS], p_full[NS], pv_done[2], o_full, o_empty, l_full;
+  __shared__ uint64_t q_full, q_empty, k_full[NS], v_full[NS], v_empty[NS], s_full[NS], p_full[NS], o_full, o_empty, l_full;
   __shared__ uint64_t raw_full[RAW], raw_empty[RAW], sc_full[SLOTS];
   __shared__ float xm[2][2][BM], xl[2][2][BM];  // [item parity][group][row]
   __shared__ __align__(16) float ksc[FP8 ? SLOTS : 1][BN], vsc[FP8 ? SLOTS : 1][BN];   // scales of the key tiles in flight
@@ -129,7 +165,6 @@ prefix_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CU
     mbar_init(smem_u32(&q_empty), 1);
     for (int s = 0; s < NS; ++s) {
       mbar_init(smem_u32(&k_full[s]), FP8 ? LOADERS : 1);
-      mbar_init(smem_u32(&k_empty[s]), 1);
       mbar_init(smem_u32(&v_full[s]), FP8 ? LOADERS : 1);
       mbar_init(smem_u32(&v_empty[s]), 1);
       mbar_init(smem_u32(&s_full[s]), 1);
@@ -140,7 +175,6 @@ prefix_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CU
       mbar_init(smem_u32(&raw_empty[s]), LOADERS);
     }
     for (int s = 0; s < SLOTS; ++s) mbar_init(smem_u32(&sc_full[s]), LOADERS);
-    for (int g = 0; g < 2; ++g) mbar_init(smem_u32(&pv_done[g]), 1);
     mbar_init(smem_u32(&l_full), 256);
     mbar_init(smem_u32(&o_full), 1);
     mbar_init(smem_u32(&o_empty), 256);
@@ -161,7 +195,7 @@ prefix_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CU
   // Counters that run across the items (every role advances its own copies the same way; every item has at least one key tile):
   //   t   key tiles so far: stage t % NS of the K and V operand tiles, score buffer t % NS (s_full, p_full), slot t % 8 of the scales
   //   n   items so far: parity of q_full / q_empty / o_full / o_empty / l_full
-  //   c_g tiles given to softmax group g so far: parity of pv_done[g]
+  // s_full of a tile (its scores are done) also means that its K stage is free, v_empty (its P V is done) that O holds it.
   if (warp == 0) {
     if (lane == 0) {
       tma_prefetch_desc(&tk);
@@ -180,7 +214,7 @@ prefix_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CU
             }
           } else {
             const uint32_t s = t % NS, ph = (t / NS) & 1;
-            if (!mbar_wait(smem_u32(&k_empty[s]), ph ^ 1, abortp)) { ok = false; break; }
+            if (!mbar_wait(smem_u32(&s_full[s]), ph ^ 1, abortp)) { ok = false; break; }      // scores done = K stage free
             mbar_expect_tx(smem_u32(&k_full[s]), TILE);
             for (int c = 0; c < D / 64; ++c) tma_load_3d(smem_u32(sK + s * TILE + c * HALF), &tk, smem_u32(&k_full[s]), c * 64, k0, w.h);
             if (!mbar_wait(smem_u32(&v_empty[s]), ph ^ 1, abortp)) { ok = false; break; }
@@ -214,7 +248,6 @@ prefix_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CU
           for (int k = 0; k < D / 16; ++k)
             tc_mma_ss(tmem + S_COL + ks * 128, desc_advance(dq0, (k / 4) * HALF + (k % 4) * 32), desc_advance(dk, (k / 4) * HALF + (k % 4) * 32), IDESC_S, k > 0);
           tc_commit(smem_u32(&s_full[ks]));
-          tc_commit(smem_u32(&k_empty[ks]));
           if (last) tc_commit(smem_u32(&q_empty));
         }
         __syncwarp();
@@ -235,7 +268,6 @@ prefix_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CU
           for (int k = 0; k < BN / 16; ++k)
             tc_mma_ts(tmem + O_COL + g * O_COLS, tmem + S_COL + vs * 128 + k * 8, desc_advance(dv, k * 2048), IDESC_O, (j >= 2 || k > 0) ? 1u : 0u);
           tc_commit(smem_u32(&v_empty[vs]));
-          tc_commit(smem_u32(&pv_done[g]));
           if (j == w.tiles - 1) tc_commit(smem_u32(&o_full));
         }
         __syncwarp();
@@ -282,7 +314,7 @@ prefix_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CU
           // probabilities of tile t - 2 NS, and those came after the group was through with tile t - 8
           for (int which = 0; which < 2; ++which) {
             const uint32_t i = 2 * t + which, rs = i % RAW;
-            if (!mbar_wait(smem_u32(which ? &v_empty[s] : &k_empty[s]), ph ^ 1, abortp) || !mbar_wait(smem_u32(&raw_full[rs]), (i / RAW) & 1, abortp)) {
+            if (!mbar_wait(smem_u32(which ? &v_empty[s] : &s_full[s]), ph ^ 1, abortp) || !mbar_wait(smem_u32(&raw_full[rs]), (i / RAW) & 1, abortp)) {
               ok = false;
               break;
             }
@@ -333,7 +365,7 @@ prefix_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CU
     const int g = (warp - 2) >> 2;              // group 0: key tiles 0, 2, ...; group 1: 1, 3, ...
     const uint32_t o_addr = tmem + lane_addr + O_COL + g * O_COLS;
     const float sc = p.scale_log2;
-    uint32_t t = 0, n = 0, done = 0;            // done: tiles of this group so far
+    uint32_t t = 0, n = 0;
     bool failed = false;
 
     for (int round = 0; !failed && item_at(round, w); ++round) {
@@ -343,7 +375,7 @@ prefix_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CU
       const int lo = p.window > 0 && row_valid ? p.P + position(p.pos, p.pos_n, p.pos_host, b) + (bt - b * p.T) - p.window + 1 : 0;   // first visible key
       float m = -INFINITY, l = 0.f;
 
-      for (int j = g; j < w.tiles; j += 2, ++done) {
+      for (int j = g; j < w.tiles; j += 2) {
         const int k0 = w.key + j * BN;
         const uint32_t slot = (t + j) % SLOTS, sb = (t + j) % NS;
         const uint32_t s_addr = tmem + lane_addr + S_COL + sb * 128;
@@ -390,11 +422,14 @@ prefix_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CU
           // One pass in the common case: probabilities against the current reference while the tile's maximum is tracked; redone
           // (the scores are still in TMEM) when a row has to move its reference by more than 2^8. The next quarter of the scores is
           // on its way while one is exponentiated.
-          float mx4[4], sum4[4];
+          float mx4[4];
+          uint64_t sum2[2];
           uint32_t pk[2][32];
           float ref = m == -INFINITY ? 0.f : m;
           auto pass = [&]() {
             uint32_t r[2][32];
+            const uint64_t scale2 = pair(s2, s2), ref2 = pair(-ref, -ref);
+            sum2[0] = sum2[1] = pair(0.f, 0.f);
             tmem_ld32(s_addr, r[0]);
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
@@ -402,13 +437,22 @@ prefix_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CU
               if (c < 3) tmem_ld32(s_addr + (c + 1) * 32, r[(c + 1) & 1]);
               prepare(c, r[c & 1]);
               mx4[c] = -INFINITY;
-              sum4[c] = 0.f;
 #pragma unroll
               for (int i = 0; i < 32; i += 2) {
                 const float a = __uint_as_float(r[c & 1][i]), d = __uint_as_float(r[c & 1][i + 1]);
                 mx4[c] = fmaxf(mx4[c], fmaxf(a, d));
-                float p0 = exp2f(fmaf(a, s2, -ref)), p1 = exp2f(fmaf(d, s2, -ref));
-                sum4[c] += p0 + p1;
+                uint64_t x = fma2(pair(a, d), scale2, ref2);
+                float p0, p1;
+                if (i % 8 == POLY_AT) {         // a quarter of the exponentials: the special-function unit is what they queue for
+                  x = exp2_poly(x);
+                  unpair(x, p0, p1);
+                } else {
+                  unpair(x, p0, p1);
+                  p0 = exp2f(p0);
+                  p1 = exp2f(p1);
+                  x = pair(p0, p1);
+                }
+                sum2[(i >> 1) & 1] = add2(sum2[(i >> 1) & 1], x);
                 if (FP8) {
                   const float2 f = *reinterpret_cast<const float2*>(&vsc[slot][c * 32 + i]);
                   p0 *= f.x;
@@ -428,7 +472,7 @@ prefix_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CU
             }
             l *= factor;
             if (j >= 2) {                       // O_g holds tiles j - 2, j - 4, ...: wait until the last of them has been added
-              if (!mbar_wait(smem_u32(&pv_done[g]), (done - 1) & 1, abortp)) abort_flag = 1;
+              if (!mbar_wait(smem_u32(&v_empty[(t + j - 2) % NS]), ((t + j - 2) / NS) & 1, abortp)) abort_flag = 1;
               tc_fence_after();
 #pragma unroll 1
               for (int c = 0; c < D / 32; ++c) {
@@ -445,7 +489,9 @@ prefix_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CU
           tmem_st32(s_addr, pk[0]);
           tmem_st32(s_addr + 32, pk[1]);
           tmem_st_wait();
-          l += (sum4[0] + sum4[1]) + (sum4[2] + sum4[3]);
+          float sum_a, sum_b;
+          unpair(add2(sum2[0], sum2[1]), sum_a, sum_b);
+          l += sum_a + sum_b;
         }
         tc_fence_before();
         mbar_arrive(smem_u32(&p_full[sb]));
