@@ -128,6 +128,7 @@ prefix_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CU
   constexpr int TILE = Smem<D, FP8>::TILE, RAW_TILE = Smem<D, FP8>::RAW_TILE, RAW = Smem<D, FP8>::RAW, NS = Smem<D, FP8>::NS;
   constexpr int HALF = 128 * 128;               // bytes of one 64-column block of an operand tile
   constexpr uint32_t TMEM_COLS = 512, S_COL = 0, O_COL = NS * 128, O_COLS = NS == 3 ? 64 : 128;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");         // own_kernel may start wherever there is room
   constexpr uint32_t IDESC_S = make_idesc(BM, BN, 1, 1, 0, 0), IDESC_O = make_idesc(BM, D, 1, 1, 0, 1);
 
   extern __shared__ uint8_t smem_raw[];
@@ -592,7 +593,7 @@ __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], 
 // Otherwise at most 16 rows, and the warps (and the CTAs of a cluster) split the keys (one token: all bytes in flight at once).
 template <int D, bool FP8, bool ROWS>
 struct OwnGeo {
-  static constexpr int TK = 2048 / D;                            // keys per tile: 4 KB of bf16 keys
+  static constexpr int TK = ROWS ? 2048 / D : 16;                // keys per tile; split keys: small rings, so that 12 to 16 warps fit an SM
   static constexpr int ROWB = D * 2 + 16;                        // padded operand row: ldmatrix rows fall in distinct banks
   static constexpr int TILE_B = TK * ROWB;
   static constexpr int RAW_B = FP8 ? TK * D : TILE_B;            // one K or V tile as it arrives
@@ -606,11 +607,12 @@ struct OwnGeo {
 };
 
 template <int D, bool FP8, bool ROWS>
-__global__ void __launch_bounds__(OTHREADS) own_kernel(const OwnParams p) {
+__global__ void __launch_bounds__(OTHREADS, D == 64 ? 4 : 3) own_kernel(const OwnParams p) {
   using G_ = OwnGeo<D, FP8, ROWS>;
   constexpr int TK = G_::TK, ROWB = G_::ROWB, TILE_B = G_::TILE_B, RAW_B = G_::RAW_B, STAGE_B = G_::STAGE_B, RC = G_::ROWS_CTA, PITCH = G_::PITCH;
   constexpr int ESZ = FP8 ? 1 : 2, LT = ROWS ? OTHREADS : 32;    // threads that fill one ring
   constexpr int MAXW = 8 + MAX_SPLITS;
+  static_assert(TK * D * ESZ / 16 % LT == 0 && 2 * TK * (D / 16) % LT == 0 && TK <= LT && TK % 16 == 0, "every thread of a ring copies and converts whole pieces");
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ float red_m[OWARPS * 16], red_l[OWARPS * 16];       // per warp and row
   __shared__ float comb_m[RC], comb_l[RC], weight[RC][MAXW + 1];
@@ -846,6 +848,7 @@ __global__ void __launch_bounds__(OTHREADS) own_kernel(const OwnParams p) {
   cg::cluster_group cluster = cg::this_cluster();
   if (!ROWS && p.cluster > 1) cluster.sync();
 
+  if (p.splits > 0) asm volatile("griddepcontrol.wait;" ::: "memory");     // the prefix kernel is through
   // ---- weights of all partial results of a row: the cluster's CTAs, then the prefix splits; the last place holds 1 / (their sum)
   constexpr int TPR = OTHREADS / RC;                             // threads per row
   {
@@ -980,13 +983,17 @@ int launch_own(const OwnParams& p, cudaStream_t stream) {
   cfg.blockDim = dim3(OTHREADS);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
+  // After the prefix kernel: launched beside it, waits for it just before the merge. All it reads until then (queries, caches,
+  // positions) was there before the prefix kernel started.
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = p.cluster;
   attr[0].val.clusterDim.y = 1;
   attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = p.splits > 0 ? 2 : 1;
   if (cudaLaunchKernelEx(&cfg, own_kernel<D, FP8, ROWS>, p) != cudaSuccess) {
     LYRA_CHECK_LAUNCH();
     return -114;

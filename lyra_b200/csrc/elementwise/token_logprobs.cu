@@ -41,7 +41,7 @@ struct Fwd {
   const long long* target;           // [N], negative: the row has no target (logprob 0)
   float* logprob;                    // [N]
   float* entropy;                    // [N]
-  float* norm;                       // [2, N]: m and log s, for the gradient
+  float* norm;                       // [2, N]: m and log s, for the gradient; or null
   float* top_lp;                     // [N, k]
   long long* top_id;                 // [N, k]
   long long stride;                  // elements between rows
@@ -383,8 +383,10 @@ __global__ void __launch_bounds__(THREADS, 2) token_logprobs_kernel(const Fwd p)
     else if (tg < p.V && !bad) lp = logp(Vec<T>::load(rowp + tg));
     p.logprob[row_id] = lp;
     p.entropy[row_id] = bad ? nan : float(log_s - double(t.u) / double(t.s));
-    p.norm[row_id] = bad ? nan : t.m;
-    p.norm[p.N + row_id] = bad ? nan : float(log_s);
+    if (p.norm) {
+      p.norm[row_id] = bad ? nan : t.m;
+      p.norm[p.N + row_id] = bad ? nan : float(log_s);
+    }
   }
   for (int i = tid; i < p.k; i += THREADS) {
     const unsigned long long b = sh.best[i];

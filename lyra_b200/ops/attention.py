@@ -118,7 +118,7 @@ def check_prefix_attention(q, prefix_k, prefix_v, k_cache, v_cache, sinks, scale
         if tuple(sinks.shape) != (Nq,):
             raise ValueError(f"sinks {tuple(sinks.shape)} must be [{Nq}]")
         tensors.append(sinks)
-    if not scale > 0 or window < 0:
+    if not scale > 0 or window < 0 or window != int(window):
         raise ValueError(f"scale {scale} must be positive and window {window} not negative")
     if isinstance(pos, torch.Tensor):
         if pos.dtype not in (torch.int32, torch.int64) or pos.numel() not in (1, B):
@@ -134,10 +134,22 @@ def check_prefix_attention(q, prefix_k, prefix_v, k_cache, v_cache, sinks, scale
 
 def _rows16(t: torch.Tensor) -> torch.Tensor:
     """``t`` with unit inner stride and 16-byte steps on every other axis (copied if it is not so already)."""
-    size = t.element_size()
-    if t.numel() and (t.stride(-1) != 1 or t.data_ptr() % 16 or any((s * size) % 16 or s <= 0 for s, n in zip(t.stride()[:-1], t.shape[:-1]) if n > 1)):
-        return t.contiguous() if not t.is_contiguous() else t.clone()
-    return t
+    if t.data_ptr() % 16 == 0:
+        if t.is_contiguous() and t.shape[-1] * t.element_size() % 16 == 0:
+            return t
+        unit, strides = 16 // t.element_size(), t.stride()
+        if strides[-1] == 1 and all(s > 0 and s % unit == 0 for s, n in zip(strides[:-1], t.shape) if n > 1):
+            return t
+    return t.contiguous() if not t.is_contiguous() else t.clone()
+
+
+def _scales(t: QArray, contiguous: bool) -> torch.Tensor:
+    """fp32 ``[..., positions]`` of a cache's scales."""
+    s = t.scale if t.scale.dtype == torch.float32 else t.scale.float()
+    if contiguous:
+        return s if s.is_contiguous() else s.contiguous()
+    s = s[..., 0]
+    return s if s.stride(-1) == 1 or s.shape[-1] <= 1 else s.contiguous()
 
 
 def prefix_attention(q, prefix_k, prefix_v, k_cache, v_cache, sinks, scale: float, window: int, pos):
@@ -153,34 +165,45 @@ def prefix_attention(q, prefix_k, prefix_v, k_cache, v_cache, sinks, scale: floa
             raise ValueError(f"prefix and caches must be bf16, or e4m3 with scales, on a GPU; got {t.dtype}")
     Nkv, P = pk.shape[0], pk.shape[1]
     S = kc.shape[2]
-    out = torch.empty(B, T, Nq, D, dtype=torch.bfloat16, device=q.device)
+    dev = q.device
+    out = torch.empty(B, T, Nq, D, dtype=torch.bfloat16, device=dev)
     if out.numel() == 0:
         return out.transpose(1, 2).to(q.dtype)
-    lib = native.kernels()
     with native.on_device(q):
-        qb, pk, pv = _rows16(q.to(torch.bfloat16)), _rows16(pk), _rows16(pv)
-        kc, vc = _rows16(kc.contiguous()), _rows16(vc.contiguous())
-        scales = lambda t, contiguous: (lambda s: s.contiguous() if contiguous or s.stride(1) != 1 else s)(t.scale.float()[..., 0])
-        pks, pvs = (scales(prefix_k, False), scales(prefix_v, False)) if quant and P else (None, None)
-        ks, vs = (scales(k_cache, True), scales(v_cache, True)) if own_quant else (None, None)
-        sk = sinks.float().contiguous() if sinks is not None else None
-        at = pos.reshape(-1).to(torch.int32).contiguous() if isinstance(pos, torch.Tensor) else None
-        lib.lyra_prefix_attention_workspace.restype = c_ll
-        need = lib.lyra_prefix_attention_workspace(B, T, P, Nq, Nkv, D, int(window))
+        need = native.function("lyra_prefix_attention_workspace", "iiiiiii", c_ll)(B, T, P, Nq, Nkv, D, window)
         if need < 0:
             raise ValueError(f"prefix_attention does not take B {B}, T {T}, {Nq} / {Nkv} heads on a GPU")
-        ws = torch.empty(max(need, 16), dtype=torch.uint8, device=q.device)
-        rc = lib.lyra_prefix_attention(
-            ptr(qb), c_ll(qb.stride(0)), c_ll(qb.stride(1)), c_ll(qb.stride(2)), ptr(pk), c_ll(_step(pk, 0)), c_ll(_step(pk, 1)), ptr(pv), c_ll(_step(pv, 0)),
-            c_ll(_step(pv, 1)), ptr(pks), c_ll(pks.stride(0) if pks is not None else 0), ptr(pvs), c_ll(pvs.stride(0) if pvs is not None else 0),
-            c_int(int(quant)), ptr(kc), ptr(vc), ptr(ks), ptr(vs), c_int(int(own_quant)), ptr(sk), ptr(at), c_int(at.numel() if at is not None else 0),
-            c_int(int(pos) if at is None else 0), ptr(out), ptr(ws), c_int(B), c_int(T), c_int(P), c_int(S), c_int(Nq), c_int(Nkv), c_int(D),
-            c_float(scale), c_int(int(window)), ptr(native.status_word()), native.stream_ptr())
+        ws = torch.empty(need, dtype=torch.uint8, device=dev)
+        qb, pk, pv = _rows16(q if q.dtype == torch.bfloat16 else q.to(torch.bfloat16)), _rows16(pk), _rows16(pv)
+        kc, vc = _rows16(kc.contiguous()), _rows16(vc.contiguous())
+        pks = pvs = ks = vs = sk = at = None
+        pks_step = pvs_step = 0
+        if quant and P:
+            pks, pvs = _scales(prefix_k, False), _scales(prefix_v, False)
+            pks_step, pvs_step = pks.stride(0), pvs.stride(0)
+        if own_quant:
+            ks, vs = _scales(k_cache, True), _scales(v_cache, True)
+        if sinks is not None:
+            sk = sinks if sinks.dtype == torch.float32 and sinks.is_contiguous() else sinks.float().contiguous()
+        if isinstance(pos, torch.Tensor):
+            at = pos if pos.dtype == torch.int32 and pos.is_contiguous() else pos.to(torch.int32).contiguous()
+        address = lambda t: t.data_ptr() if t is not None else None
+        fn = native.function("lyra_prefix_attention", _PREFIX_ARGS)
+        qs, ps, vs_ = qb.stride(), _steps(pk), _steps(pv)
+        rc = fn(qb.data_ptr(), qs[0], qs[1], qs[2], pk.data_ptr(), ps[0], ps[1], pv.data_ptr(), vs_[0], vs_[1], address(pks), pks_step, address(pvs), pvs_step,
+                quant, kc.data_ptr(), vc.data_ptr(), address(ks), address(vs), own_quant, address(sk), address(at), at.numel() if at is not None else 0,
+                int(pos) if at is None else 0, out.data_ptr(), ws.data_ptr(), B, T, P, S, Nq, Nkv, D, scale, window, native.status_word().data_ptr(),
+                native.stream_address())
     native.check(rc, "lyra_prefix_attention")
     native.count_launch(2 if P else 1)
-    return out.transpose(1, 2).to(q.dtype)
+    out = out.transpose(1, 2)
+    return out if q.dtype == torch.bfloat16 else out.to(q.dtype)
 
 
-def _step(t: torch.Tensor, axis: int) -> int:
-    """Stride of an axis; an axis of length one has none that matters, but a TMA map wants one it can use."""
-    return t.stride(axis) if t.shape[axis] > 1 else max(t.shape[-1], 16)
+_PREFIX_ARGS = "plllpllpllplpl" + "ippppippii" + "ppiiiiiiifipp"
+
+
+def _steps(t: torch.Tensor) -> tuple[int, int]:
+    """(head, position) strides of a prefix; an axis of length one has none that matters, but a TMA map wants one it can use."""
+    row = t.shape[2] if t.shape[1] <= 1 else t.stride(1)
+    return (row * max(t.shape[1], 1) if t.shape[0] <= 1 else t.stride(0)), row

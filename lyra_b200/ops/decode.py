@@ -295,9 +295,11 @@ def moe_block_supported(F_: int, C: int, H: int, E: int, n_shared: int, k: int, 
         return False
     if quant and any(w.qval.dtype != torch.float8_e4m3fn or w.block[0] % 16 or w.block[1] % 16 for w in (w_up, w_down)):
         return False
-    lib = native.kernels()
-    lib.lyra_moe_block_workspace.restype = c_ll
-    return F_ >= 1 and lib.lyra_moe_block_workspace(F_, C, H, E, n_shared, k, int(quant)) >= 0
+    return F_ >= 1 and _moe_block_workspace(F_, C, H, E, n_shared, k, quant) >= 0
+
+
+def _moe_block_workspace(F_, C, H, E, n_shared, k, quant) -> int:
+    return native.function("lyra_moe_block_workspace", "iiiiiii", c_ll)(F_, C, H, E, n_shared, k, quant)
 
 
 def moe_block(x, norm_scale, eps, router, router_bias, w_up, up_bias, w_down, down_bias, k, n_shared, beta, limit, residual_scale):
@@ -323,26 +325,32 @@ def moe_block(x, norm_scale, eps, router, router_bias, w_up, up_bias, w_down, do
         raise ValueError(f"moe_block with e4m3 weights takes a SwiGLU limit in 0..1e4, got {limit}")
     with native.on_device(x):
         if quant:
-            wu, wd = w_up.qval.contiguous(), w_down.qval.contiguous()
-            us, ds = w_up.scale.float().contiguous(), w_down.scale.float().contiguous()
+            wu, wd = _aligned(w_up.qval), _aligned(w_down.qval)
+            us, ds = (w.scale if w.scale.dtype == torch.float32 and w.scale.is_contiguous() else w.scale.float().contiguous() for w in (w_up, w_down))
             blocks = (*w_up.block, *w_down.block)
         else:
-            wu, wd = cuda_ops.bf16_weight(w_up).contiguous(), cuda_ops.bf16_weight(w_down).contiguous()
+            wu, wd = _aligned(cuda_ops.bf16_weight(w_up)), _aligned(cuda_ops.bf16_weight(w_down))
             us = ds = None
             blocks = (16, 16, 16, 16)
-        f32 = lambda p: None if p is None else cuda_ops.fp32_param(p).contiguous()
-        xc, ns, rw, rb, ub, db = _aligned(x), f32(norm_scale), f32(router), f32(router_bias), f32(up_bias), f32(down_bias)
-        wu, wd = _aligned(wu), _aligned(wd)
+        xc, ns, rw, rb, ub, db = _aligned(x), _fp32(norm_scale), _fp32(router), _fp32(router_bias), _fp32(up_bias), _fp32(down_bias)
         out = torch.empty(F_, C, dtype=BF16, device=dev)
-        lib = native.kernels()
-        ws = torch.empty(lib.lyra_moe_block_workspace(F_, C, H, E, n_shared, k, int(quant)), dtype=torch.uint8, device=dev)
-        rc = lib.lyra_moe_block(ptr(xc), ptr(ns), c_float(eps), ptr(rw), ptr(rb), ptr(wu), ptr(us), c_int(blocks[0]), c_int(blocks[1]), ptr(ub), ptr(wd),
-                                ptr(ds), c_int(blocks[2]), c_int(blocks[3]), ptr(db), ptr(out), ptr(scores), ptr(idx), ptr(ws), c_int(F_), c_int(C), c_int(H),
-                                c_int(E), c_int(n_shared), c_int(k), c_int(int(quant)), c_float(beta), c_float(limit), c_float(residual_scale),
-                                ptr(native.status_word()), native.stream_ptr())
+        ws = torch.empty(_moe_block_workspace(F_, C, H, E, n_shared, k, quant), dtype=torch.uint8, device=dev)
+        address = lambda t: t.data_ptr() if t is not None else None
+        fn = native.function("lyra_moe_block", "ppfppppiipppiippppp" + "iiiiiiifffpp")
+        rc = fn(xc.data_ptr(), ns.data_ptr(), eps, rw.data_ptr(), address(rb), wu.data_ptr(), address(us), blocks[0], blocks[1], address(ub), wd.data_ptr(),
+                address(ds), blocks[2], blocks[3], address(db), out.data_ptr(), scores.data_ptr(), idx.data_ptr(), ws.data_ptr(), F_, C, H, E, n_shared, k,
+                quant, beta, limit, residual_scale, native.status_word().data_ptr(), native.stream_address())
     native.check(rc, "lyra_moe_block")
     native.count_launch()
     return out, scores, idx
+
+
+def _fp32(p: torch.Tensor | None) -> torch.Tensor | None:
+    if p is None or (p.dtype == torch.float32 and p.is_contiguous()):
+        return p
+    from lyra_b200.ops import cuda_ops
+
+    return cuda_ops.fp32_param(p).contiguous()
 
 
 def _aligned(t: torch.Tensor) -> torch.Tensor:

@@ -8,7 +8,6 @@ from typing import NamedTuple
 import torch
 
 from lyra_b200.ops import native
-from lyra_b200.ops.native import c_int, c_ll, ptr
 
 MAX_TOP_K = 32
 
@@ -38,20 +37,24 @@ def check_arguments(logits: torch.Tensor, targets: torch.Tensor, top_k: int, voc
     return vocab
 
 
+def _forward(logits, targets, k: int, vocab: int, norm: torch.Tensor | None):
+    N, dev = logits.shape[0], logits.device
+    logprob, entropy = torch.empty(N, dtype=torch.float32, device=dev), torch.empty(N, dtype=torch.float32, device=dev)
+    top_lp, top_id = torch.empty(N, k, dtype=torch.float32, device=dev), torch.empty(N, k, dtype=torch.int64, device=dev)
+    if N:
+        fn = native.function("lyra_token_logprobs", "pippppppiiilp")
+        native.check(fn(logits.data_ptr(), logits.dtype == torch.bfloat16, targets.data_ptr(), logprob.data_ptr(), entropy.data_ptr(),
+                        norm.data_ptr() if norm is not None else None, top_lp.data_ptr(), top_id.data_ptr(), N, vocab, k, logits.stride(0),
+                        native.stream_address()), "lyra_token_logprobs")
+        native.count_launch()
+    return logprob, entropy, top_lp, top_id
+
+
 class _TokenLogprobs(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, targets, k, vocab):
-        N, W = logits.shape
-        dev = logits.device
-        logprob, entropy = torch.empty(2, N, dtype=torch.float32, device=dev).unbind(0)
-        norm = torch.empty(2, N, dtype=torch.float32, device=dev)          # row maxima and log sums, for the gradient
-        top_lp = torch.empty(N, k, dtype=torch.float32, device=dev)
-        top_id = torch.empty(N, k, dtype=torch.int64, device=dev)
-        if N:
-            native.check(native.kernels().lyra_token_logprobs(ptr(logits), c_int(int(logits.dtype == torch.bfloat16)), ptr(targets), ptr(logprob),
-                                                              ptr(entropy), ptr(norm), ptr(top_lp), ptr(top_id), c_int(N), c_int(vocab), c_int(k),
-                                                              c_ll(logits.stride(0)), native.stream_ptr()), "lyra_token_logprobs")
-            native.count_launch()
+        norm = torch.empty(2, logits.shape[0], dtype=torch.float32, device=logits.device)      # row maxima and log sums, for the gradient
+        logprob, entropy, top_lp, top_id = _forward(logits, targets, k, vocab, norm)
         ctx.save_for_backward(logits, targets, norm, entropy)
         ctx.vocab = vocab
         ctx.mark_non_differentiable(top_lp, top_id)
@@ -69,10 +72,11 @@ class _TokenLogprobs(torch.autograd.Function):
         if N:
             gl = g_logprob.float().contiguous() if g_logprob is not None else None
             gh = g_entropy.float().contiguous() if g_entropy is not None else None
+            address = lambda t: t.data_ptr() if t is not None else None
             with native.on_device(logits):
-                native.check(native.kernels().lyra_token_logprobs_bwd(ptr(logits), c_int(int(logits.dtype == torch.bfloat16)), ptr(grad), ptr(targets),
-                                                                      ptr(norm), ptr(entropy), ptr(gl), ptr(gh), c_int(N), c_int(ctx.vocab), c_int(W),
-                                                                      c_ll(logits.stride(0)), native.stream_ptr()), "lyra_token_logprobs_bwd")
+                fn = native.function("lyra_token_logprobs_bwd", "pippppppiiilp")
+                native.check(fn(logits.data_ptr(), logits.dtype == torch.bfloat16, grad.data_ptr(), targets.data_ptr(), norm.data_ptr(), entropy.data_ptr(),
+                                address(gl), address(gh), N, ctx.vocab, W, logits.stride(0), native.stream_address()), "lyra_token_logprobs_bwd")
             native.count_launch()
         return grad, None, None, None
 
@@ -82,9 +86,16 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, top_k: int, voca
     if logits.dtype not in (torch.float32, torch.bfloat16):
         raise ValueError(f"logits must be fp32 or bf16 on a GPU, got {logits.dtype}")
     lead = logits.shape[:-1]
-    rows = logits.reshape(-1, logits.shape[-1])
+    rows, flat = logits, targets
+    if logits.ndim != 2:
+        rows, flat = logits.reshape(-1, logits.shape[-1]), targets.reshape(-1)
     if rows.shape[0] and (rows.stride(1) != 1 or rows.stride(0) < rows.shape[1]):
         rows = rows.contiguous()                              # transposed logits, or one row expanded to many
+    if flat.dtype != torch.int64 or not flat.is_contiguous():
+        flat = flat.long().contiguous()
     with native.on_device(logits):
-        out = _TokenLogprobs.apply(rows, targets.reshape(-1).long().contiguous(), top_k, vocab)
-    return TokenLogprobs(*(t.reshape(*lead, *t.shape[1:]) for t in out))
+        if torch.is_grad_enabled() and rows.requires_grad:
+            out = _TokenLogprobs.apply(rows, flat, top_k, vocab)
+        else:
+            out = _forward(rows, flat, top_k, vocab, None)
+    return TokenLogprobs(*out) if logits.ndim == 2 else TokenLogprobs(*(t.reshape(*lead, *t.shape[1:]) for t in out))

@@ -64,8 +64,22 @@ def kernels_available() -> bool:
     return True
 
 
+@functools.cache
+def function(name: str, arguments: str, restype=c_int):
+    """An entry point of the kernel library with its argument types declared: ``p`` pointer, ``i`` int, ``l`` 64-bit int, ``f`` float.
+    Plain Python numbers (and None for a null pointer) can then be passed, which costs a third of wrapping each of them."""
+    fn = getattr(kernels(), name)
+    fn.argtypes = [{"p": c_void_p, "i": c_int, "l": c_ll, "f": c_float}[a] for a in arguments]
+    fn.restype = restype
+    return fn
+
+
 def ptr(t: torch.Tensor | None) -> c_void_p:
     return c_void_p(0 if t is None else t.data_ptr())
+
+
+def stream_address() -> int:
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
 
 
 def stream_ptr() -> c_void_p:
