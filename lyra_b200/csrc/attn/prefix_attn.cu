@@ -1027,11 +1027,12 @@ extern "C" long long lyra_prefix_attention_workspace(int B, int T, int P, int Nq
 extern "C" int lyra_prefix_attention(const void* q, long long q_sb, long long q_sn, long long q_st, const void* pk, long long pk_sh, long long pk_sp,
                                      const void* pv, long long pv_sh, long long pv_sp, const float* pk_scale, long long pks_sh, const float* pv_scale,
                                      long long pvs_sh, int prefix_fp8, const void* k, const void* v, const float* k_scale, const float* v_scale, int own_fp8,
-                                     const float* sinks, const int* pos, int pos_n, int pos_host, void* out, void* workspace, int B, int T, int P, int S,
-                                     int Nq, int Nkv, int D, float scale, int window, int* status, cudaStream_t stream) {
+                                     const float* sinks, const int* pos, int pos_n, int pos_host, void* out, void* workspace, long long workspace_bytes,
+                                     int B, int T, int P, int S,                                     int Nq, int Nkv, int D, float scale, int window, int* status, cudaStream_t stream) {
   using namespace lyra;
   using namespace lyra::prefix;
-  if (lyra_prefix_attention_workspace(B, T, P, Nq, Nkv, D, window) < 0 || S < 0 || window < 0 || !(scale > 0.f)) return -110;
+  const long long need = lyra_prefix_attention_workspace(B, T, P, Nq, Nkv, D, window);
+  if (need < 0 || workspace_bytes < need || S < 0 || window < 0 || !(scale > 0.f)) return -110;
   if (pos && pos_n != 1 && pos_n != B) return -110;
   if ((prefix_fp8 && P > 0 && (!pk_scale || !pv_scale)) || (own_fp8 && S > 0 && (!k_scale || !v_scale))) return -110;
   const Shape shape = prefix_shape(B, T, P, Nq, Nkv, window);

@@ -963,11 +963,12 @@ extern "C" long long lyra_moe_block_workspace(int F, int C, int H, int E, int sh
 // x, out [F, C] bf16; up [n, C, 2H], down [n, H, C] bf16 or e4m3 with fp32 scales per (bk x bn) block; n = E + shared.
 extern "C" int lyra_moe_block(const void* x, const float* norm, float eps, const float* router, const float* router_bias, const void* up, const float* up_scale,
                               int up_bk, int up_bn, const float* up_bias, const void* down, const float* down_scale, int dn_bk, int dn_bn,
-                              const float* down_bias, void* out, float* scores, long long* idx, void* workspace, int F, int C, int H, int E, int shared,
-                              int k, int fp8, float beta, float limit, float residual_scale, int* status, cudaStream_t stream) {
+                              const float* down_bias, void* out, float* scores, long long* idx, void* workspace, long long workspace_bytes, int F, int C, int H, int E,
+                              int shared,                              int k, int fp8, float beta, float limit, float residual_scale, int* status, cudaStream_t stream) {
   using namespace lyra;
   using namespace lyra::moeblk;
-  if (lyra_moe_block_workspace(F, C, H, E, shared, k, fp8) < 0) return -100;
+  const long long need = lyra_moe_block_workspace(F, C, H, E, shared, k, fp8);
+  if (need < 0 || workspace_bytes < need) return -100;
   if (fp8 && !(limit >= 0.f && limit <= 1e4f)) return -100;   // the fp16 operand's range is fitted to it
   if (fp8 && (!up_scale || !down_scale || up_bk % 16 || up_bn % 16 || dn_bk % 16 || dn_bn % 16 || up_bk < 16 || up_bn < 16 || dn_bk < 16 || dn_bn < 16 ||
               C % up_bk || (2 * H) % up_bn || H % dn_bk || C % dn_bn))

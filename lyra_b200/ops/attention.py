@@ -192,7 +192,7 @@ def prefix_attention(q, prefix_k, prefix_v, k_cache, v_cache, sinks, scale: floa
         qs, ps, vs_ = qb.stride(), _steps(pk), _steps(pv)
         rc = fn(qb.data_ptr(), qs[0], qs[1], qs[2], pk.data_ptr(), ps[0], ps[1], pv.data_ptr(), vs_[0], vs_[1], address(pks), pks_step, address(pvs), pvs_step,
                 quant, kc.data_ptr(), vc.data_ptr(), address(ks), address(vs), own_quant, address(sk), address(at), at.numel() if at is not None else 0,
-                int(pos) if at is None else 0, out.data_ptr(), ws.data_ptr(), B, T, P, S, Nq, Nkv, D, scale, window, native.status_word().data_ptr(),
+                int(pos) if at is None else 0, out.data_ptr(), ws.data_ptr(), need, B, T, P, S, Nq, Nkv, D, scale, window, native.status_word().data_ptr(),
                 native.stream_address())
     native.check(rc, "lyra_prefix_attention")
     native.count_launch(2 if P else 1)
@@ -200,7 +200,7 @@ def prefix_attention(q, prefix_k, prefix_v, k_cache, v_cache, sinks, scale: floa
     return out if q.dtype == torch.bfloat16 else out.to(q.dtype)
 
 
-_PREFIX_ARGS = "plllpllpllplpl" + "ippppippii" + "ppiiiiiiifipp"
+_PREFIX_ARGS = "plllpllpllplpl" + "ippppippii" + "ppliiiiiiifipp"
 
 
 def _steps(t: torch.Tensor) -> tuple[int, int]:

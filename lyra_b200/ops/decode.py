@@ -334,11 +334,12 @@ def moe_block(x, norm_scale, eps, router, router_bias, w_up, up_bias, w_down, do
             blocks = (16, 16, 16, 16)
         xc, ns, rw, rb, ub, db = _aligned(x), _fp32(norm_scale), _fp32(router), _fp32(router_bias), _fp32(up_bias), _fp32(down_bias)
         out = torch.empty(F_, C, dtype=BF16, device=dev)
-        ws = torch.empty(_moe_block_workspace(F_, C, H, E, n_shared, k, quant), dtype=torch.uint8, device=dev)
+        need = _moe_block_workspace(F_, C, H, E, n_shared, k, quant)
+        ws = torch.empty(need, dtype=torch.uint8, device=dev)
         address = lambda t: t.data_ptr() if t is not None else None
-        fn = native.function("lyra_moe_block", "ppfppppiipppiippppp" + "iiiiiiifffpp")
+        fn = native.function("lyra_moe_block", "ppfppppiipppiippppp" + "liiiiiiifffpp")
         rc = fn(xc.data_ptr(), ns.data_ptr(), eps, rw.data_ptr(), address(rb), wu.data_ptr(), address(us), blocks[0], blocks[1], address(ub), wd.data_ptr(),
-                address(ds), blocks[2], blocks[3], address(db), out.data_ptr(), scores.data_ptr(), idx.data_ptr(), ws.data_ptr(), F_, C, H, E, n_shared, k,
+                address(ds), blocks[2], blocks[3], address(db), out.data_ptr(), scores.data_ptr(), idx.data_ptr(), ws.data_ptr(), need, F_, C, H, E, n_shared, k,
                 quant, beta, limit, residual_scale, native.status_word().data_ptr(), native.stream_address())
     native.check(rc, "lyra_moe_block")
     native.count_launch()
