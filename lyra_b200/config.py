@@ -158,6 +158,9 @@ class ModelConfig:
     mode: Mode = Mode.NOCACHE
     use_presorted_emb_gather: bool = True
     implementation: Implementation = "auto"
+    fused_moe_decode: bool = False
+    """Decode steps of few tokens run each MoE layer (norm, router, experts, residual) as one kernel; the router then sees the
+    normalised input before it is rounded, so near-equal experts may change places against the step-by-step path."""
 
     # Misc
     sample_topk: int = 4

@@ -30,16 +30,20 @@ class InferenceConfig:
     fp8: bool = False
     temperature: float | None = None
     top_k: int | None = None
+    fused_moe: bool = False
 
 
 def apply_inference_overrides(mcfg: ModelConfig, icfg: InferenceConfig) -> ModelConfig:
-    """``--fp8`` quantises the MLP weights and the KV cache, not the attention projections (lyra/generate.py:31-38)."""
+    """``--fp8`` quantises the MLP weights and the KV cache, not the attention projections (lyra/generate.py:31-38); ``--fused-moe`` runs
+    each MoE layer of a decode step as one kernel."""
     if icfg.temperature is not None:
         mcfg = replace(mcfg, sample_temperature=icfg.temperature)
     if icfg.top_k is not None:
         mcfg = replace(mcfg, sample_topk=icfg.top_k)
     if icfg.fp8:
         mcfg = replace(mcfg, gemm_dtype=torch.float8_e4m3fn, quantize_mlp=True, quantize_cache=True)
+    if icfg.fused_moe:
+        mcfg = replace(mcfg, fused_moe_decode=True)
     return mcfg
 
 
@@ -116,7 +120,9 @@ class BatchedGenerator:
     """Batched prefill + greedy/sampled decode. ``prompts [B, P]`` are equal-length token rows on this rank; with an
     expert-parallel runtime every rank serves its own rows and the experts are shared across ranks.
 
-    ``prefill`` returns the first generated token per row and its duration; ``decode`` runs ``n`` further tokens.
+    ``prefill`` returns the first generated token per row; ``decode`` runs ``n`` further tokens. With ``prefix`` all prompts continue
+    one shared token sequence (a system prompt, in-context examples): it is prefilled once, kept once, and every later attention
+    reads it once for the whole batch; ``capacity`` then counts the positions after it.
     With ``use_cuda_graph`` the per-token launch sequence is captured once and replayed."""
 
     def __init__(self, model: ModelWeights, mcfg: ModelConfig, *, batch: int, capacity: int, device, rt=None, use_cuda_graph: bool = False):
@@ -136,8 +142,21 @@ class BatchedGenerator:
         self._static_out = None
 
     @torch.no_grad()
-    def prefill(self, prompts: torch.Tensor) -> torch.Tensor:
+    def prefill(self, prompts: torch.Tensor, prefix: torch.Tensor | None = None) -> torch.Tensor:
+        """First token after each of ``prompts [B, P]``, which continue ``prefix [N]`` when it is given."""
         B, P = prompts.shape
+        kv_local = getattr(self.rt, "n_kv_local", None)
+        if prefix is not None:
+            longest = int(self.prefill_cfg.seq_len * self.prefill_cfg.rope_scale)
+            if prefix.ndim != 1 or prefix.numel() < 1 or prefix.numel() + P > longest:
+                raise ValueError(f"a prefix is a row of at least one token that leaves room for the prompts within {longest} positions, got {tuple(prefix.shape)}")
+            shared = init_cache(self.prefill_cfg, prefix.numel(), self.device, 1, kv_local)
+            _, _, shared = model_apply(prefix[None].long(), self.model, shared, self.prefill_cfg, return_hidden_states=True, rt=self.rt)
+            self.cache = ModelCache.share(shared, self.prefill_cfg, self.batch, self.capacity, self.device, kv_local)
+            self._graph = None                                # it was recorded with another cache
+        elif self.cache.prefix_len:
+            self.cache = init_cache(self.prefill_cfg, self.capacity, self.device, self.batch, kv_local)
+            self._graph = None
         self.cache.pos = 0
         hidden, _, self.cache = model_apply(prompts.long(), self.model, self.cache, self.prefill_cfg, return_hidden_states=True, rt=self.rt)
         return self._next_from_hidden(hidden[:, -1])

@@ -88,6 +88,8 @@ def rope_tables(config: ModelConfig, device) -> tuple[torch.Tensor, torch.Tensor
 class LayerCache:
     k: Any  # [B, Nkv, S, D] tensor or QArray
     v: Any
+    prefix_k: Any = None  # [Nkv, P, D] tensor or QArray: keys and values of a prefix that all sequences share
+    prefix_v: Any = None
 
 
 def _kv_append_kernel(cache: LayerCache, k: torch.Tensor, v: torch.Tensor, pos_dev: torch.Tensor) -> bool:
@@ -136,7 +138,7 @@ def cache_update(cache: LayerCache, k: torch.Tensor, v: torch.Tensor, start_pos:
         return cache
     if isinstance(cache.k, QArray):
         start = (0, 0, int(start_pos), 0)
-        return LayerCache(k=qupdate(cache.k, k, start), v=qupdate(cache.v, v, start))
+        return replace(cache, k=qupdate(cache.k, k, start), v=qupdate(cache.v, v, start))
     T = k.shape[2]
     cache.k[:, :, start_pos:start_pos + T] = k.to(cache.k.dtype)
     cache.v[:, :, start_pos:start_pos + T] = v.to(cache.v.dtype)
@@ -148,6 +150,7 @@ class ModelCache:
     layers: tuple[LayerCache, ...]
     pos: int
     pos_dev: Any = None  # optional int32 device scalar mirroring ``pos``: single-token decode then reads the position on the device
+    prefix_len: int = 0  # positions of the shared prefix in front of every sequence; ``pos`` counts the sequences' own positions
 
     @staticmethod
     def create(config: ModelConfig, batch: int, capacity: int, device, n_kv_local: int | None = None) -> "ModelCache":
@@ -156,6 +159,18 @@ class ModelCache:
         mk = lambda: torch.zeros(shape, dtype=config.compute_dtype, device=device)
         cache = ModelCache(layers=tuple(LayerCache(k=mk(), v=mk()) for _ in range(config.n_layers)), pos=0)
         return ModelCache.quantize(cache, config)
+
+    @staticmethod
+    def share(prefix: "ModelCache", config: ModelConfig, batch: int, capacity: int, device, n_kv_local: int | None = None) -> "ModelCache":
+        """An empty cache for ``batch`` sequences that all continue the one sequence ``prefix`` holds (its ``pos`` positions, not copied):
+        ``capacity`` own positions each, attention over the prefix computed once for all of them (``ops.api.prefix_attention``)."""
+        P = prefix.pos
+        if prefix.prefix_len:
+            raise ValueError("a cache that continues a shared prefix cannot itself be one")
+        cut = lambda a: QArray(a.qval[0, :, :P], a.scale[0, :, :P], a.block) if isinstance(a, QArray) else a[0, :, :P]
+        own = ModelCache.create(config, batch, capacity, device, n_kv_local)
+        layers = tuple(replace(o, prefix_k=cut(l.k), prefix_v=cut(l.v)) for o, l in zip(own.layers, prefix.layers))
+        return ModelCache(layers=layers, pos=0, prefix_len=P)
 
     @staticmethod
     def quantize(cache: "ModelCache", config: ModelConfig) -> "ModelCache":
@@ -268,7 +283,10 @@ def attention_apply(x, w: AttentionWeights, idx: int, pos: int, freq_cis, cache:
             else:
                 assert cache is not None
                 updated_cache = cache_update(cache, k, v, pos, pos_dev)
-                if c.mode == Mode.DECODE:
+                if cache.prefix_k is not None:
+                    t = ops.prefix_attention(q, cache.prefix_k, cache.prefix_v, updated_cache.k, updated_cache.v, sinks, c.head_dim**-0.5, window,
+                                             pos if pos_dev is None else pos_dev, impl)
+                elif c.mode == Mode.DECODE:
                     t = ops.decode_attention(q, updated_cache.k, updated_cache.v, sinks, c.head_dim**-0.5, window, pos, impl, pos_dev=pos_dev)
                 else:
                     t = ops.attention(q, k, v, sinks, c.head_dim**-0.5, window, pos, impl) if pos == 0 else \
@@ -434,6 +452,21 @@ def bpermute(expert_ids: torch.Tensor, n_experts: int):
     return permutation, destinations
 
 
+def _takes_moe_block(x, w: MoEWeights, config: ModelConfig, probe: Probe, rt) -> bool:
+    """Whether a decode step's MoE layer runs as one kernel: asked for (``ModelConfig.fused_moe_decode``), no gradient, nothing to
+    record, experts whole on this rank, and a size the kernel takes."""
+    c = config
+    if (not c.fused_moe_decode or c.mode != Mode.DECODE or torch.is_grad_enabled() or probe.enabled or ROUTING_TAPE is not None
+            or (rt is not None and (rt.tp_size > 1 or rt.ep_size > 1))):
+        return False
+    if not ops.use_kernels(x, c.implementation):
+        return True
+    from lyra_b200.ops import decode
+
+    return x.dtype == torch.bfloat16 and decode.moe_block_supported(x.shape[0] * x.shape[1], c.n_embd, c.expert_hidden, c.n_routed_experts,
+                                                                    c.n_shared_experts, c.n_active_routed_experts, w.mlp_up, w.mlp_down)
+
+
 def moe_apply(x, w: MoEWeights, config: ModelConfig, *, probe: Probe = NO_PROBE, rt=None):
     """Pre-norm mixture-of-experts block with residual; returns ``(x + branch, aux_loss)`` (lyra/model.py:498-567).
 
@@ -444,6 +477,15 @@ def moe_apply(x, w: MoEWeights, config: ModelConfig, *, probe: Probe = NO_PROBE,
     impl = c.implementation
     B, T, C = x.shape
     W = (lambda p: rt.materialize(p) if rt is not None else p)
+    if _takes_moe_block(x, w, c, probe, rt):
+        with scope("moe"):
+            out, _, indices = ops.moe_block(x.reshape(B * T, C), W(w.norm_scale), c.norm_eps, W(w.router), W(w.router_bias), w.mlp_up, w.mlp_up_bias,
+                                            w.mlp_down, w.mlp_down_bias, c.n_active_routed_experts, c.n_shared_experts, c.swiglu_beta, c.swiglu_limit,
+                                            c.residual_scale, impl)
+            meter = getattr(rt, "load_meter", None)
+            if meter is not None and meter.always:
+                meter.add(rt._layer, indices)
+            return out.reshape(B, T, C), x.new_zeros((), dtype=torch.float32)    # no gradient, no auxiliary loss
     with scope("moe"):
         xn = ops.rms_norm(x, W(w.norm_scale), c.norm_eps, impl)
         probe.tensor("norm_out", xn)
@@ -636,11 +678,13 @@ def model_apply(tokens, model: ModelWeights, cache: ModelCache | None, config: M
         start_pos = cache.pos if cache is not None else 0
         cos, sin = rope_tables(c, h.device)
         pos_dev = cache.pos_dev if (cache is not None and c.mode == Mode.DECODE and T == 1) else None
+        behind = cache.prefix_len if cache is not None else 0          # positions of the shared prefix in front of the sequences
         if pos_dev is not None:
-            at = pos_dev.reshape(1).long()
+            at = pos_dev.reshape(1).long() + behind
             freq_cis = (cos.index_select(0, at)[None, :, None, :], sin.index_select(0, at)[None, :, None, :])
         else:
-            freq_cis = (cos[start_pos:start_pos + T][None, :, None, :], sin[start_pos:start_pos + T][None, :, None, :])
+            first = behind + start_pos
+            freq_cis = (cos[first:first + T][None, :, None, :], sin[first:first + T][None, :, None, :])
 
         aux_loss = torch.zeros((), dtype=torch.float32, device=h.device)
         caches = []
@@ -656,7 +700,7 @@ def model_apply(tokens, model: ModelWeights, cache: ModelCache | None, config: M
             caches.append(lc)
         if c.n_moe_layers:
             aux_loss = aux_loss / c.n_moe_layers
-        updated = None if cache is None else ModelCache(layers=tuple(caches), pos=start_pos + T, pos_dev=cache.pos_dev)
+        updated = None if cache is None else ModelCache(layers=tuple(caches), pos=start_pos + T, pos_dev=cache.pos_dev, prefix_len=behind)
 
         head = probe.scope("head")
         head.tensor("pre_norm", h)

@@ -37,7 +37,7 @@ DEFAULT_SAMPLE_PROMPTS = (
 )
 RUN_ARTIFACTS = ("metrics.jsonl", "samples.jsonl", "numerics.jsonl")
 MODEL_FIELDS_IGNORED_ON_RESUME = ("w_init", "b_init", "norm_init", "mode", "sample_topk", "sample_temperature", "quantize_cache",
-                                  "implementation", "sharding")
+                                  "implementation", "sharding", "fused_moe_decode")
 SCHEDULE_FIELDS = ("steps", "batch_size", "accumulation_steps", "decay_type", "warmup_fraction", "stable_fraction")
 
 

@@ -33,6 +33,8 @@ class Args:
     """auto takes a GPU when there is one."""
     batch_size: int = 8
     """Continuations scored per forward pass."""
+    share_prefix: bool = False
+    """Run the tokens that a batch of requests has in common (in-context examples, a question's text) once for the batch."""
     limit: int | None = None
     """Score only the first N documents of each task."""
     fewshot: dict[str, int] = field(default_factory=dict)
@@ -59,7 +61,7 @@ def main(argv: list[str] | None = None) -> int:
     config = model_variant(args.variant)
     where = join_tensor_parallel(place(args.device), config)
     scorer = Scorer(open_model(args, where, config), config, batch_size=args.batch_size, harmony=args.format == "gpt-oss",
-                    device=where.device, rt=where.runtime)
+                    device=where.device, rt=where.runtime, share_prefix=args.share_prefix)
     summary = []
     for name in args.tasks:
         shots = args.fewshot.get(name, 0)

@@ -40,6 +40,8 @@ class Args:
     """Sample among the k most likely tokens; the variant's own setting when omitted."""
     fp8: bool = False
     """Keep expert / MLP weights and the KV cache as block-scaled e4m3."""
+    fused_moe: bool = False
+    """Run each mixture-of-experts layer of a decode step as one kernel."""
 
 
 def main(argv: list[str] | None = None) -> int:
@@ -49,7 +51,7 @@ def main(argv: list[str] | None = None) -> int:
     from lyra_b200.variants import model_variant
 
     settings = InferenceConfig(weights=args.weights or default_weights(args.variant), max_new_tokens=args.max_new_tokens,
-                               max_cache_length=args.max_cache_length, temperature=args.temperature, top_k=args.top_k, fp8=args.fp8)
+                               max_cache_length=args.max_cache_length, temperature=args.temperature, top_k=args.top_k, fp8=args.fp8, fused_moe=args.fused_moe)
     config = apply_inference_overrides(model_variant(args.variant), settings)
     where = join_tensor_parallel(place(args.device), config)
     terminal = {}
