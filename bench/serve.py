@@ -55,6 +55,7 @@ def main() -> None:
     ap.add_argument("--new", type=int, default=128)
     ap.add_argument("--layers", type=int, default=0, help="truncate the model to this many layers (0 = all)")
     ap.add_argument("--fp8", action="store_true", help="block-scaled e4m3 expert weights and an e4m3 KV cache")
+    ap.add_argument("--fused-moe", action="store_true", help="each MoE layer of a decode step in one kernel")
     ap.add_argument("--no-graph", action="store_true")
     ap.add_argument("--profile-decode", action="store_true",
                     help="bracket the timed decode with cudaProfilerStart / Stop, so that a profiler started with "
@@ -85,6 +86,8 @@ def main() -> None:
         mcfg = replace(mcfg, n_layers=args.layers, mlp_map=mcfg.mlp_map[: args.layers])
     if args.fp8:
         mcfg = replace(mcfg, quantize_mlp=True, quantize_cache=True, gemm_dtype=torch.float8_e4m3fn, quant_block=(64, 64))
+    if args.fused_moe:
+        mcfg = replace(mcfg, fused_moe_decode=True)
     rt = None
     tp = world > 1 and args.tensor_parallel
     if tp:          # tensor parallel: every rank holds a slice of every layer and all ranks serve the same batch
