@@ -31,10 +31,12 @@ constexpr int MAX_TOP = 32;
 constexpr int CAP = 1024;            // candidate buffer; more candidates than this (long runs of equal logits) take the slow selection
 constexpr int MAX_RUNS = 10240;      // run maxima kept per CTA (40 KB)
 constexpr float L2E = 1.4426950408889634f;
-// Distances below the maximum are cut off here: e^{-1000} is 0 in fp32 as well, and 0 * y stays 0 for logits of -inf and for
-// masks of the type's lowest value, whose distance would overflow. The maximum itself is kept in the logits' own unit, so a row
-// that holds nothing but the lowest value is a uniform distribution.
+// Distances below a maximum (in log2 units) are cut off here: 2^-1000 is 0 in fp32 as well, and 0 * y stays 0.
 constexpr float FLOOR = -1000.f;
+// Logits are read as at least -BIG (a mask of -inf or of the type's lowest value is a token of probability 0 either way, and stays clear
+// of inf * 0). Slices whose own maximum lies outside of -BIG .. BIG - nothing but such masks, as a rule - are scanned once more with
+// distances formed in the logits' own unit: a row of the type's lowest value is a uniform distribution.
+constexpr float BIG = 1e30f;
 
 struct Fwd {
   const void* x;
@@ -64,6 +66,24 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   return r;
 }
 
+// Two fp32 operations per instruction.
+__device__ __forceinline__ uint64_t pair2(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void split2(uint64_t v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
 template <typename T>
 struct Vec;
 template <>
@@ -74,6 +94,11 @@ struct Vec<float> {
   }
   __device__ static uint4 pack(const float (&f)[4]) {
     return make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
+  }
+  // the four logits as two pairs, at least -BIG
+  __device__ static void pairs(const uint4& v, uint64_t (&x)[2]) {
+    x[0] = pair2(fmaxf(__uint_as_float(v.x), -BIG), fmaxf(__uint_as_float(v.y), -BIG));
+    x[1] = pair2(fmaxf(__uint_as_float(v.z), -BIG), fmaxf(__uint_as_float(v.w), -BIG));
   }
   __device__ static float load(const float* p) { return *p; }
   __device__ static float largest(const uint4& v) {
@@ -100,6 +125,15 @@ struct Vec<__nv_bfloat16> {
       w[i] = *reinterpret_cast<uint32_t*>(&t);
     }
     return make_uint4(w[0], w[1], w[2], w[3]);
+  }
+  __device__ static void pairs(const uint4& v, uint64_t (&x)[4]) {
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      uint32_t c;
+      asm("max.bf16x2 %0, %1, %2;" : "=r"(c) : "r"(w[i]), "r"(0xf149f149u));          // -1e30 in bf16, twice
+      x[i] = pair2(__uint_as_float(c << 16), __uint_as_float(c & 0xffff0000u));
+    }
   }
   __device__ static float load(const __nv_bfloat16* p) { return __bfloat162float(*p); }
   __device__ static uint32_t max2(uint32_t a, uint32_t b) {
@@ -146,15 +180,15 @@ struct Row {
   }
 };
 
-struct Stat {      // running maximum (NaN once a NaN was seen), s = sum e^{x - m}, u = sum e^{x - m} (x - m)
+struct Stat {      // maximum m (NaN once a NaN was seen), s = sum 2^y, u = sum 2^y y with y = (x - m) log2 e
   float m, s, u;
 };
 __device__ __forceinline__ Stat merge(const Stat& a, const Stat& b) {
   Stat r;
   r.m = max_nan(a.m, b.m);
   // an empty side has m = -inf, s = u = 0: its distance must not become inf * 0
-  const float da = a.m == -INFINITY ? 0.f : fmaxf(a.m - r.m, FLOOR), db = b.m == -INFINITY ? 0.f : fmaxf(b.m - r.m, FLOOR);
-  const float ea = exp2f(da * L2E), eb = exp2f(db * L2E);
+  const float da = a.m == -INFINITY ? 0.f : fmaxf((a.m - r.m) * L2E, FLOOR), db = b.m == -INFINITY ? 0.f : fmaxf((b.m - r.m) * L2E, FLOOR);
+  const float ea = exp2f(da), eb = exp2f(db);
   r.s = a.s * ea + b.s * eb;
   r.u = ea * (a.u + da * a.s) + eb * (b.u + db * b.s);
   return r;
@@ -202,8 +236,10 @@ __global__ void __launch_bounds__(THREADS, 2) token_logprobs_kernel(const Fwd p)
   constexpr int STEP = THREADS * UNROLL;
   const int n_chunks = (v1 - v0 + STEP - 1) / STEP;
 
-  // ---- the pass over the slice
-  Stat st{-INFINITY, 0.f, 0.f};
+  // ---- the pass over the slice: y' = x log2e - ml with ml = m log2e as it is rounded, 4.5 operations a logit
+  float m = -INFINITY, ml = 0.f;
+  uint64_t s2 = pair2(0.f, 0.f), u2 = s2;
+  const uint64_t l2e2 = pair2(L2E, L2E);
   uint32_t best_key = 0, this_run = 0;
   int in_run = 0, run = 0;
   for (int c = 0; c < n_chunks; ++c) {
@@ -226,31 +262,46 @@ __global__ void __launch_bounds__(THREADS, 2) token_logprobs_kernel(const Fwd p)
         in_run = 0;
       }
     }
-    const float m2 = max_nan(st.m, g);
-    if (!(m2 <= st.m)) {                            // moved up (or NaN)
-      if (st.m != -INFINITY) {
-        const float d = fmaxf(st.m - m2, FLOOR), e = exp2f(d * L2E);
-        st.u = e * (st.u + d * st.s);
-        st.s *= e;
+    g = max_nan(m, g);
+    if (!(g <= m)) {                                // moved up (or NaN)
+      const float to = fabsf(g) <= BIG ? g * L2E : 0.f;      // out of range: nothing is added up (masks), or scanned once more
+      if (fabsf(m) <= BIG) {
+        const float d = fmaxf(ml - to, FLOOR), e = exp2f(d);
+        const uint64_t e2 = pair2(e, e), d2 = pair2(d, d), zero = pair2(0.f, 0.f);
+        u2 = fma2(fma2(d2, s2, u2), e2, zero);
+        s2 = fma2(s2, e2, zero);
       }
-      st.m = m2;
+      m = g;
+      ml = to;
     }
+    const uint64_t off = pair2(-ml, -ml);
 #pragma unroll
     for (int j = 0; j < UNROLL; ++j) {
-      float f[VE];
-      Vec<T>::unpack(v[j], f);
+      uint64_t x[VE / 2];
+      Vec<T>::pairs(v[j], x);
 #pragma unroll
-      for (int i = 0; i < VE; ++i) {
-        const float y = fmaxf(f[i] - st.m, FLOOR);
-        const float e = exp2f(y * L2E);
-        st.s += e;
-        st.u = fmaf(e, y, st.u);
+      for (int i = 0; i < VE / 2; ++i) {
+        const uint64_t y = fma2(x[i], l2e2, off);
+        float a, b;
+        split2(y, a, b);
+        const uint64_t e = pair2(exp2f(a), exp2f(b));
+        s2 = add2(s2, e);
+        u2 = fma2(e, y, u2);
       }
     }
   }
   if (p.k && in_run) {
     run_key[run++ * THREADS + tid] = this_run;
     best_key = max(best_key, this_run);
+  }
+  Stat st;
+  {
+    float sa, sb, ua, ub;
+    split2(s2, sa, sb);
+    split2(u2, ua, ub);
+    // from ml to m log2e: the rounding of ml, exactly (a product's error in one fma)
+    const float d = fabsf(m) <= BIG ? -fmaf(m, L2E, -ml) : 0.f, e = exp2f(d);
+    st = Stat{m, m == -INFINITY ? 0.f : (sa + sb) * e, m == -INFINITY ? 0.f : ((ua + ub) + d * (sa + sb)) * e};
   }
 
   // ---- statistics of the CTA, then of the cluster
@@ -265,6 +316,28 @@ __global__ void __launch_bounds__(THREADS, 2) token_logprobs_kernel(const Fwd p)
 #pragma unroll
     for (int o = 8; o > 0; o >>= 1) t = merge(t, shfl_stat(t, o));
     if (lane == 0) sh.total = t;
+  }
+  __syncthreads();
+  if (const float top = sh.total.m; fabsf(top) > BIG && fabsf(top) < INFINITY) {      // masks only (or logits beyond any use): see BIG
+    Stat t{top, 0.f, 0.f};
+    for (int i = v0 + tid; i < v1; i += THREADS) {
+      float f[VE];
+      Vec<T>::unpack(row.vec(i), f);
+#pragma unroll
+      for (int x = 0; x < VE; ++x) {
+        const float y = fmaxf((f[x] - top) * L2E, FLOOR), e = exp2f(y);
+        t.s += e;
+        t.u = fmaf(e, y, t.u);
+      }
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) t = merge(t, shfl_stat(t, o));
+    if (lane == 0) sh.part[warp] = t;
+    __syncthreads();
+    if (tid == 0) {
+      for (int w = 1; w < THREADS / 32; ++w) t = merge(t, sh.part[w]);
+      sh.total = t;
+    }
   }
 
   if (p.k) {
@@ -382,7 +455,7 @@ __global__ void __launch_bounds__(THREADS, 2) token_logprobs_kernel(const Fwd p)
     if (tg < 0) lp = 0.f;
     else if (tg < p.V && !bad) lp = logp(Vec<T>::load(rowp + tg));
     p.logprob[row_id] = lp;
-    p.entropy[row_id] = bad ? nan : float(log_s - double(t.u) / double(t.s));
+    p.entropy[row_id] = bad ? nan : float(log_s - double(t.u) / double(t.s) * 0.69314718055994530942);
     if (p.norm) {
       p.norm[row_id] = bad ? nan : t.m;
       p.norm[p.N + row_id] = bad ? nan : float(log_s);
