@@ -10,6 +10,10 @@
 // is a bound that at least k elements reach and few exceed, and only the runs that reach it are read again (a few hundred
 // bytes, still in L2). The candidates are ranked by (value, lowest id), so the order in which they were found does not matter.
 //
+// Two CTAs per SM walk the rows. A producer warp streams them through a ring of bulk copies in shared memory (64 KB), eight warps add up
+// and note run maxima, and a ninth finishes a row - joins the sums, picks the alternatives, writes - while the eight are in the next
+// one: with the same warps doing both, finishing took as long as half a row (2048 rows of 201088 bf16 logits: 256 us, now XX).
+//
 // Few rows are split over a cluster of up to eight CTAs (each SM streams a slice; partial results meet in the first CTA through
 // distributed shared memory): one row of 201088 fp32 logits would otherwise be read by one SM.
 #include <cooperative_groups.h>
@@ -18,6 +22,7 @@
 #include <math.h>
 #include <stdint.h>
 
+#include "../common/sm100.cuh"
 #include "../common/tmap.h"
 
 namespace lyra {
@@ -25,11 +30,13 @@ namespace tlp {
 
 namespace cg = cooperative_groups;
 
-constexpr int THREADS = 512;
-constexpr int UNROLL = 4;            // 16-byte loads in flight per thread
+constexpr int THREADS = 256, ALL = THREADS + 64;            // warps 0..7 add up, warp 8 finishes rows, warp 9 copies
+constexpr int UNROLL = 4;            // 16-byte vectors per thread and chunk
+constexpr int CHUNK = THREADS * UNROLL * 16, STAGES = 4;   // bytes of a chunk; chunks in flight or in use
 constexpr int MAX_TOP = 32;
-constexpr int CAP = 1024;            // candidate buffer; more candidates than this (long runs of equal logits) take the slow selection
-constexpr int MAX_RUNS = 10240;      // run maxima kept per CTA (40 KB)
+constexpr int CAP = 1024;            // candidates kept; more (long runs of equal logits) take the slower selection
+constexpr int MAX_HITS = 256;        // runs looked at again
+constexpr int MAX_RUNS = 3584;       // run maxima kept per row (14 KB, twice: two CTAs fit an SM)
 constexpr float L2E = 1.4426950408889634f;
 // Distances below a maximum (in log2 units) are cut off here: 2^-1000 is 0 in fp32 as well, and 0 * y stays 0.
 constexpr float FLOOR = -1000.f;
@@ -47,7 +54,8 @@ struct Fwd {
   float* top_lp;                     // [N, k]
   long long* top_id;                 // [N, k]
   long long stride;                  // elements between rows
-  int N, V, k, chunks_per_run;
+  int* status;
+  int N, V, k, chunks_per_run, runs;
 };
 
 // Order of the alternatives: larger value first (NaN above +inf, as a sort in torch has it; -0 equals 0), then lower id.
@@ -198,262 +206,167 @@ __device__ __forceinline__ Stat shfl_stat(const Stat& a, int o) {
 }
 
 struct Shared {
-  Stat part[THREADS / 32];
-  Stat total;
-  uint32_t tmax[THREADS];
-  uint32_t bound;
-  int n_cand;
+  uint64_t full[STAGES], empty[STAGES];             // the ring
+  uint64_t ready[2], finished[2];                   // sums and run maxima of a row (by parity): complete; no longer needed
+  int abort;
+  Stat part[2][THREADS / 32];
+  uint32_t tmax[2][THREADS];
+  int n_hits, n_cand;
+  int hits[MAX_HITS];
+  Stat total;                                       // clusters: read by the first CTA
   unsigned long long cand[CAP];                     // (key << 32) | ~id : one unsigned comparison is the whole order
-  unsigned long long best[8 * MAX_TOP];             // the CTA's (then the cluster's) k best
-  unsigned long long red[THREADS / 32];
+  unsigned long long best[MAX_TOP];
 };
 
 __device__ __forceinline__ unsigned long long entry(uint32_t key, int id) { return ((unsigned long long)key << 32) | (uint32_t)(~id); }
 
-// k best of list[0..n) into out[0..k): entries are distinct (their ids are), so an entry's rank is the number of larger ones.
+// k best of list[0..n) into out[0..k), by one warp: entries are distinct (their ids are), so an entry's rank is the number of larger ones.
 __device__ __forceinline__ void rank_select(const unsigned long long* list, int n, int k, unsigned long long* out) {
-  for (int i = threadIdx.x; i < n; i += THREADS) {
+  for (int i = threadIdx.x & 31; i < n; i += 32) {
     const unsigned long long mine = list[i];
     int rank = 0;
     for (int j = 0; j < n; ++j) rank += list[j] > mine;
     if (rank < k) out[rank] = mine;
   }
+  __syncwarp();
 }
 
+// A CTA's slice of a row: vectors [v0, v1), of which [w0, w1) lie wholly inside the row.
 template <typename T>
-__global__ void __launch_bounds__(THREADS, 2) token_logprobs_kernel(const Fwd p) {
-  constexpr int VE = Vec<T>::N;
-  extern __shared__ __align__(16) uint8_t dyn[];
-  Shared& sh = *reinterpret_cast<Shared*>(dyn);
-  uint32_t* run_key = reinterpret_cast<uint32_t*>(dyn + sizeof(Shared));
-  cg::cluster_group cluster = cg::this_cluster();
-  const int cs = int(cluster.num_blocks()), cr = int(cluster.block_rank());
-  const int row_id = int(blockIdx.x) / cs;
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const T* rowp = reinterpret_cast<const T*>(p.x) + (long long)row_id * p.stride;
-  const Row<T> row(rowp, p.V);
-  const int v0 = int((long long)row.n_vec * cr / cs), v1 = int((long long)row.n_vec * (cr + 1) / cs);
-  constexpr int STEP = THREADS * UNROLL;
-  const int n_chunks = (v1 - v0 + STEP - 1) / STEP;
+struct Slice {
+  Row<T> row;
+  int v0, v1, w0, w1, n_chunks;
+  __device__ Slice(const Fwd& p, int row_id, int cr, int lg)
+      : row(reinterpret_cast<const T*>(p.x) + (long long)row_id * p.stride, p.V) {
+    v0 = int((long long)row.n_vec * cr >> lg);
+    v1 = int((long long)row.n_vec * (cr + 1) >> lg);
+    w0 = row.lead > 0 ? 1 : 0;
+    w1 = int(((long long)p.V + row.lead) / Vec<T>::N);
+    n_chunks = (v1 - v0 + THREADS * UNROLL - 1) / (THREADS * UNROLL);
+  }
+};
 
-  // ---- the pass over the slice: y' = x log2e - ml with ml = m log2e as it is rounded, 4.5 operations a logit
-  float m = -INFINITY, ml = 0.f;
-  uint64_t s2 = pair2(0.f, 0.f), u2 = s2;
-  const uint64_t l2e2 = pair2(L2E, L2E);
-  uint32_t best_key = 0, this_run = 0;
-  int in_run = 0, run = 0;
-  for (int c = 0; c < n_chunks; ++c) {
-    uint4 v[UNROLL];
-    const int first = v0 + c * STEP + tid;
+// The k largest entries of a slice into sh.best (unfilled places 0), by one warp, from its run maxima. Returns nothing on purpose: a
+// slice with fewer than k logits leaves places at 0.
+template <typename T>
+__device__ void pick(const Fwd& p, const Slice<T>& slice, Shared& sh, const uint32_t* run_key, const uint32_t* tmax) {
+  constexpr int VE = Vec<T>::N, STEP = THREADS * UNROLL;
+  const int lane = threadIdx.x & 31, k = p.k;
+  const Row<T>& row = slice.row;
+  auto elements = [&](int i, auto&& use) {            // (key, id) of the elements of vector i
+    const int e0 = i * VE - row.lead;
+    float f[VE];
+    Vec<T>::unpack(row.vec(i), f);
 #pragma unroll
-    for (int j = 0; j < UNROLL; ++j) {
-      const int i = first + j * THREADS;
-      v[j] = i < v1 ? row.vec(i) : make_uint4(Vec<T>::MINUS_INF, Vec<T>::MINUS_INF, Vec<T>::MINUS_INF, Vec<T>::MINUS_INF);
-    }
-    float g = Vec<T>::largest(v[0]);
+    for (int x = 0; x < VE; ++x)
+      if (e0 + x >= 0 && e0 + x < p.V) use(order_key(f[x]), e0 + x);
+  };
+  auto push = [&](uint32_t key, int id) {
+    const int at = atomicAdd(&sh.n_cand, 1);
+    if (at < CAP) sh.cand[at] = entry(key, id);
+  };
+  // a bound that at least k elements reach: the k-th largest of 64 disjoint subset maxima (a subset without elements has key 0)
+  uint32_t a = 0, b = 0;
 #pragma unroll
-    for (int j = 1; j < UNROLL; ++j) g = max_nan(g, Vec<T>::largest(v[j]));
-    if (p.k) {
-      if (first < v1) this_run = max(this_run, order_key(g));
-      if (++in_run == p.chunks_per_run) {
-        run_key[run++ * THREADS + tid] = this_run;
-        best_key = max(best_key, this_run);
-        this_run = 0;
-        in_run = 0;
-      }
-    }
-    g = max_nan(m, g);
-    if (!(g <= m)) {                                // moved up (or NaN)
-      const float to = fabsf(g) <= BIG ? g * L2E : 0.f;      // out of range: nothing is added up (masks), or scanned once more
-      if (fabsf(m) <= BIG) {
-        const float d = fmaxf(ml - to, FLOOR), e = exp2f(d);
-        const uint64_t e2 = pair2(e, e), d2 = pair2(d, d), zero = pair2(0.f, 0.f);
-        u2 = fma2(fma2(d2, s2, u2), e2, zero);
-        s2 = fma2(s2, e2, zero);
-      }
-      m = g;
-      ml = to;
-    }
-    const uint64_t off = pair2(-ml, -ml);
-#pragma unroll
-    for (int j = 0; j < UNROLL; ++j) {
-      uint64_t x[VE / 2];
-      Vec<T>::pairs(v[j], x);
-#pragma unroll
-      for (int i = 0; i < VE / 2; ++i) {
-        const uint64_t y = fma2(x[i], l2e2, off);
-        float a, b;
-        split2(y, a, b);
-        const uint64_t e = pair2(exp2f(a), exp2f(b));
-        s2 = add2(s2, e);
-        u2 = fma2(e, y, u2);
-      }
-    }
+  for (int j = 0; j < THREADS / 64; ++j) {
+    a = max(a, tmax[j * 64 + lane]);
+    b = max(b, tmax[j * 64 + 32 + lane]);
   }
-  if (p.k && in_run) {
-    run_key[run++ * THREADS + tid] = this_run;
-    best_key = max(best_key, this_run);
+  int ra = 0, rb = 0;
+#pragma unroll 4
+  for (int s = 0; s < 32; ++s) {
+    const uint32_t oa = __shfl_sync(0xffffffffu, a, s), ob = __shfl_sync(0xffffffffu, b, s);
+    ra += (oa > a || (oa == a && s < lane)) + (ob > a);
+    rb += (oa >= b) + (ob > b || (ob == b && s < lane));
   }
-  Stat st;
-  {
-    float sa, sb, ua, ub;
-    split2(s2, sa, sb);
-    split2(u2, ua, ub);
-    // from ml to m log2e: the rounding of ml, exactly (a product's error in one fma)
-    const float d = fabsf(m) <= BIG ? -fmaf(m, L2E, -ml) : 0.f, e = exp2f(d);
-    st = Stat{m, m == -INFINITY ? 0.f : (sa + sb) * e, m == -INFINITY ? 0.f : ((ua + ub) + d * (sa + sb)) * e};
-  }
-
-  // ---- statistics of the CTA, then of the cluster
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) st = merge(st, shfl_stat(st, o));
-  if (lane == 0) sh.part[warp] = st;
-  sh.tmax[tid] = best_key;
-  if (tid == 0) sh.n_cand = 0;
-  __syncthreads();
-  if (warp == 0) {
-    Stat t = lane < THREADS / 32 ? sh.part[lane] : Stat{-INFINITY, 0.f, 0.f};
-#pragma unroll
-    for (int o = 8; o > 0; o >>= 1) t = merge(t, shfl_stat(t, o));
-    if (lane == 0) sh.total = t;
-  }
-  __syncthreads();
-  if (const float top = sh.total.m; fabsf(top) > BIG && fabsf(top) < INFINITY) {      // masks only (or logits beyond any use): see BIG
-    Stat t{top, 0.f, 0.f};
-    for (int i = v0 + tid; i < v1; i += THREADS) {
-      float f[VE];
-      Vec<T>::unpack(row.vec(i), f);
-#pragma unroll
-      for (int x = 0; x < VE; ++x) {
-        const float y = fmaxf((f[x] - top) * L2E, FLOOR), e = exp2f(y);
-        t.s += e;
-        t.u = fmaf(e, y, t.u);
-      }
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) t = merge(t, shfl_stat(t, o));
-    if (lane == 0) sh.part[warp] = t;
-    __syncthreads();
-    if (tid == 0) {
-      for (int w = 1; w < THREADS / 32; ++w) t = merge(t, sh.part[w]);
-      sh.total = t;
-    }
-  }
-
-  if (p.k) {
-    // ---- a bound that at least k elements reach: the k-th largest of 64 disjoint subset maxima
-    if (warp == 1) {
-      uint32_t a = 0, b = 0;
-#pragma unroll
-      for (int j = 0; j < THREADS / 64; ++j) {
-        a = max(a, sh.tmax[j * 64 + lane]);
-        b = max(b, sh.tmax[j * 64 + 32 + lane]);
-      }
-      int ra = 0, rb = 0;
+  const uint32_t hit_a = __ballot_sync(0xffffffffu, ra == k - 1), hit_b = __ballot_sync(0xffffffffu, rb == k - 1);    // ranks 0..63 are all taken once
+  uint32_t bound = hit_a ? __shfl_sync(0xffffffffu, a, __ffs(hit_a) - 1) : __shfl_sync(0xffffffffu, b, __ffs(hit_b) - 1);
+  bound = max(bound, 1u);                           // every real key is larger than 0 (-inf has 0x007fffff)
+  if (lane < k) sh.best[lane] = 0;
+  if (lane == 0) sh.n_hits = sh.n_cand = 0;
+  __syncwarp();
+  // runs that reach it
+  const int n_runs = (slice.n_chunks + p.chunks_per_run - 1) / p.chunks_per_run * THREADS;
 #pragma unroll 8
-      for (int s = 0; s < 32; ++s) {
-        const uint32_t oa = __shfl_sync(0xffffffffu, a, s), ob = __shfl_sync(0xffffffffu, b, s);
-        ra += (oa > a || (oa == a && s < lane)) + (ob > a);
-        rb += (oa >= b) + (ob > b || (ob == b && s < lane));
-      }
-      if (ra == p.k - 1) sh.bound = a;              // ranks 0..63 are all taken once; a subset without elements has key 0
-      if (rb == p.k - 1) sh.bound = b;
+  for (int e = lane; e < n_runs; e += 32)
+    if (run_key[e] >= bound) {
+      const int at = atomicAdd(&sh.n_hits, 1);
+      if (at < MAX_HITS) sh.hits[at] = e;
     }
-    __syncthreads();
-    const uint32_t bound = max(sh.bound, 1u);       // key 0 marks "no element": every real key is larger (-inf has 0x007fffff)
-    for (int r = 0; r < run; ++r) {
-      if (run_key[r * THREADS + tid] < bound) continue;
-      for (int c = r * p.chunks_per_run; c < min((r + 1) * p.chunks_per_run, n_chunks); ++c) {
-        for (int j = 0; j < UNROLL; ++j) {
-          const int i = v0 + c * STEP + tid + j * THREADS;
-          if (i >= v1) continue;
-          const int e0 = i * VE - row.lead;
-          float f[VE];
-          Vec<T>::unpack(row.vec(i), f);
-#pragma unroll
-          for (int x = 0; x < VE; ++x) {
-            const uint32_t key = order_key(f[x]);
-            if (e0 + x >= 0 && e0 + x < p.V && key >= bound) {
-              const int at = atomicAdd(&sh.n_cand, 1);
-              if (at < CAP) sh.cand[at] = entry(key, e0 + x);
-            }
-          }
-        }
-      }
+  __syncwarp();
+  const int n_hits = *reinterpret_cast<volatile int*>(&sh.n_hits);
+  if (n_hits <= MAX_HITS) {
+    const int per = UNROLL * p.chunks_per_run;      // vectors of a run
+    for (int w = lane; w < n_hits * per; w += 32) {
+      const int e = sh.hits[w / per], x = w % per, c = e / THREADS * p.chunks_per_run + x / UNROLL;
+      const int i = slice.v0 + c * STEP + (x % UNROLL) * THREADS + e % THREADS;
+      if (c < slice.n_chunks && i < slice.v1) elements(i, [&](uint32_t key, int id) { if (key >= bound) push(key, id); });
     }
-    for (int i = tid; i < p.k; i += THREADS) sh.best[i] = 0;
-    __syncthreads();
-    if (sh.n_cand <= CAP) {
-      rank_select(sh.cand, sh.n_cand, p.k, sh.best);
-    } else {
-      // more than CAP elements reach the bound (long runs of equal logits): k passes, each takes the largest entry below the last
-      unsigned long long last = ~0ull;
-      for (int q = 0; q < p.k; ++q) {
-        unsigned long long mine = 0;
-        for (int i = v0 + tid; i < v1; i += THREADS) {
-          const int e0 = i * VE - row.lead;
-          float f[VE];
-          Vec<T>::unpack(row.vec(i), f);
+    __syncwarp();
+    const int n = *reinterpret_cast<volatile int*>(&sh.n_cand);
+    if (n <= CAP) {
+      rank_select(sh.cand, n, k, sh.best);
+      return;
+    }
+    __syncwarp();
+    if (lane == 0) sh.n_cand = 0;
+    __syncwarp();
+  }
+  // Long runs of equal logits: what exceeds the bound, and of what equals it the k lowest ids, in one sweep in the order of the ids.
+  int equal = 0;
+  for (int i0 = slice.v0; i0 < slice.v1; i0 += 32) {
+    int mine = 0;
+    if (i0 + lane < slice.v1) elements(i0 + lane, [&](uint32_t key, int id) { mine += key == bound; if (key > bound) push(key, id); });
+    if (equal < k) {
+      int before = mine;
 #pragma unroll
-          for (int x = 0; x < VE; ++x) {
-            if (e0 + x < 0 || e0 + x >= p.V) continue;
-            const unsigned long long en = entry(order_key(f[x]), e0 + x);
-            if (en < last && en > mine) mine = en;
-          }
-        }
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) mine = max(mine, __shfl_xor_sync(0xffffffffu, mine, o));
-        if (lane == 0) sh.red[warp] = mine;
-        __syncthreads();
-        mine = sh.red[0];
-        for (int w = 1; w < THREADS / 32; ++w) mine = max(mine, sh.red[w]);
-        if (tid == 0) sh.best[q] = mine;
-        last = mine;
-        __syncthreads();
+      for (int o = 1; o < 32; o <<= 1) {
+        const int v = __shfl_up_sync(0xffffffffu, before, o);
+        if (lane >= o) before += v;
       }
+      const int all = __shfl_sync(0xffffffffu, before, 31);
+      int at = equal + before - mine;
+      if (mine && at < k) elements(i0 + lane, [&](uint32_t key, int id) { if (key == bound && at++ < k) push(key, id); });
+      equal += all;
     }
   }
-  __syncthreads();
-  if (cs > 1) {
-    cluster.sync();
-    if (cr == 0) {
-      if (tid == 0) {
-        Stat t = sh.total;
-        for (int r = 1; r < cs; ++r) t = merge(t, cluster.map_shared_rank(&sh, r)->total);
-        sh.total = t;
-      }
-      for (int i = tid; i < cs * p.k; i += THREADS) sh.cand[i] = cluster.map_shared_rank(&sh, i / p.k)->best[i % p.k];
-      __syncthreads();
-      // unfilled slots of small slices are 0: below every entry, but equal to one another, so they are dropped before ranking
-      if (p.k) {
-        for (int i = tid; i < cs * p.k; i += THREADS) {
-          const unsigned long long mine = sh.cand[i];
-          if (!mine) continue;
-          int rank = 0;
-          for (int j = 0; j < cs * p.k; ++j) rank += sh.cand[j] > mine;
-          if (rank < p.k) sh.best[MAX_TOP + rank] = mine;
-        }
-        __syncthreads();
-        for (int i = tid; i < p.k; i += THREADS) sh.best[i] = sh.best[MAX_TOP + i];
-      }
-      __syncthreads();
-    }
-    cluster.sync();                                 // no CTA leaves while its shared memory is read
-    if (cr != 0) return;
+  __syncwarp();
+  const int n = *reinterpret_cast<volatile int*>(&sh.n_cand);
+  if (n <= CAP) {
+    rank_select(sh.cand, n, k, sh.best);
+    return;
   }
+  // One of the 64 subsets holds more than CAP logits above all others' maxima: k sweeps, each takes the largest entry below the last.
+  unsigned long long last = ~0ull;
+  for (int q = 0; q < k; ++q) {
+    unsigned long long mine = 0;
+    for (int i = slice.v0 + lane; i < slice.v1; i += 32)
+      elements(i, [&](uint32_t key, int id) {
+        const unsigned long long en = entry(key, id);
+        if (en < last && en > mine) mine = en;
+      });
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) mine = max(mine, __shfl_xor_sync(0xffffffffu, mine, o));
+    if (lane == 0) sh.best[q] = mine;
+    last = mine;
+  }
+  __syncwarp();
+}
 
-  // ---- results
-  const Stat t = sh.total;
+// Results of a row from its sums and (lane i of the warp) its i-th best entry.
+template <typename T>
+__device__ void finish_row(const Fwd& p, const Slice<T>& slice, int row_id, const Stat& t, unsigned long long b) {
+  const int lane = threadIdx.x & 31;
   const bool bad = !(fabsf(t.m) < INFINITY);        // a NaN, a +inf, or nothing but -inf: no distribution
   const float nan = __uint_as_float(0x7fc00000u);
   const double log_s = log(double(t.s));
   // (x - m) - log s, never x - lse: in a row of the type's lowest value m + log s would swallow log s
   auto logp = [&](float x) { return float((double(x) - double(t.m)) - log_s); };
-  if (tid == 0) {
+  if (lane == 0) {
     const long long tg = p.target[row_id];
     float lp = nan;
     if (tg < 0) lp = 0.f;
-    else if (tg < p.V && !bad) lp = logp(Vec<T>::load(rowp + tg));
+    else if (tg < p.V && !bad) lp = logp(Vec<T>::load(slice.row.p + tg));
     p.logprob[row_id] = lp;
     p.entropy[row_id] = bad ? nan : float(log_s - double(t.u) / double(t.s) * 0.69314718055994530942);
     if (p.norm) {
@@ -461,11 +374,215 @@ __global__ void __launch_bounds__(THREADS, 2) token_logprobs_kernel(const Fwd p)
       p.norm[p.N + row_id] = bad ? nan : float(log_s);
     }
   }
-  for (int i = tid; i < p.k; i += THREADS) {
-    const unsigned long long b = sh.best[i];
-    p.top_id[(long long)row_id * p.k + i] = (long long)(uint32_t)~(uint32_t)b;
-    p.top_lp[(long long)row_id * p.k + i] = bad ? nan : logp(key_value(uint32_t(b >> 32)));
+  if (lane < p.k) {
+    p.top_id[(long long)row_id * p.k + lane] = (long long)(uint32_t)~(uint32_t)b;
+    p.top_lp[(long long)row_id * p.k + lane] = bad ? nan : logp(key_value(uint32_t(b >> 32)));
   }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(ALL, 2) token_logprobs_kernel(const Fwd p) {
+  constexpr int VE = Vec<T>::N, STEP = THREADS * UNROLL;
+  extern __shared__ __align__(128) uint8_t dyn[];
+  uint8_t* ring = dyn;
+  Shared& sh = *reinterpret_cast<Shared*>(dyn + STAGES * CHUNK);
+  uint32_t* run_keys = reinterpret_cast<uint32_t*>(dyn + STAGES * CHUNK + sizeof(Shared));      // [2][p.runs][THREADS]
+  cg::cluster_group cluster = cg::this_cluster();
+  const int cs = int(cluster.num_blocks()), cr = int(cluster.block_rank()), lg = 31 - __clz(cs);
+  const int row0 = int(blockIdx.x) >> lg, row_step = int(gridDim.x) >> lg;      // in a cluster of several CTAs: one row each
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+
+  if (tid == 0) {
+    for (int i = 0; i < STAGES; ++i) {
+      mbar_init(smem_u32(&sh.full[i]), 1);
+      mbar_init(smem_u32(&sh.empty[i]), THREADS / 32);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(smem_u32(&sh.ready[i]), THREADS / 32);
+      mbar_init(smem_u32(&sh.finished[i]), 1);
+    }
+    sh.abort = 0;
+    fence_mbar_init();
+  }
+  __syncthreads();
+  volatile int* abortp = &sh.abort;
+  auto wait = [&](uint64_t& bar, uint32_t parity) {
+    if (!mbar_wait(smem_u32(&bar), parity & 1, abortp)) {
+      *abortp = 1;                                  // every later wait gives up at once; the results are void, the status word says so
+      atomicCAS(p.status, 0, STATUS_TIMEOUT_FULL);
+    }
+  };
+
+  if (warp == 9) {
+    if (lane == 0) {
+      uint32_t q = 0;
+      for (int row_id = row0; row_id < p.N; row_id += row_step) {
+        const Slice<T> slice(p, row_id, cr, lg);
+        for (int c = 0; c < slice.n_chunks; ++c, ++q) {
+          const uint32_t s = q % STAGES, bar = smem_u32(&sh.full[s]);
+          wait(sh.empty[s], q / STAGES + 1);
+          if (*abortp) continue;
+          // the chunk's whole vectors; the one or two that reach over the row's ends are gathered by the threads that own them
+          const int at = slice.v0 + c * STEP, a = max(at, slice.w0), b = min(min(at + STEP, slice.v1), slice.w1), n = max(b - a, 0) * 16;
+          mbar_expect_tx(bar, n);
+          if (n)
+            asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(ring + s * CHUNK + (a - at) * 16)),
+                         "l"(slice.row.p + (long long)a * VE - slice.row.lead), "r"(n), "r"(bar)
+                         : "memory");
+        }
+      }
+    }
+    __syncwarp();
+  } else if (warp < 8) {
+    uint32_t q = 0, it = 0;                         // chunks, rows so far
+    const uint64_t l2e2 = pair2(L2E, L2E);
+    for (int row_id = row0; row_id < p.N; row_id += row_step, ++it) {
+      const Slice<T> slice(p, row_id, cr, lg);
+      const int v0 = slice.v0, v1 = slice.v1;
+      uint32_t* run_key = run_keys + (it & 1) * p.runs * THREADS;
+      wait(sh.finished[it & 1], (it >> 1) + 1);     // the row before the last has been finished: its places are free
+      // y' = x log2e - ml with ml = m log2e as it is rounded
+      float m = -INFINITY, ml = 0.f;
+      uint64_t s2 = pair2(0.f, 0.f), u2 = s2;
+      uint32_t best_key = 0, this_run = 0;
+      int in_run = 0, run = 0;
+      for (int c = 0; c < slice.n_chunks; ++c, ++q) {
+        const uint32_t s = q % STAGES;
+        wait(sh.full[s], q / STAGES);
+        uint4 v[UNROLL];
+        const int first = v0 + c * STEP + tid;
+        const uint8_t* stage = ring + s * CHUNK;
+        if (v0 + c * STEP >= slice.w0 && v0 + (c + 1) * STEP <= min(v1, slice.w1)) {
+#pragma unroll
+          for (int j = 0; j < UNROLL; ++j) v[j] = *reinterpret_cast<const uint4*>(stage + (j * THREADS + tid) * 16);
+        } else {
+#pragma unroll
+          for (int j = 0; j < UNROLL; ++j) {
+            const int i = first + j * THREADS;
+            if (i >= v1) v[j] = make_uint4(Vec<T>::MINUS_INF, Vec<T>::MINUS_INF, Vec<T>::MINUS_INF, Vec<T>::MINUS_INF);
+            else if (i >= slice.w0 && i < slice.w1) v[j] = *reinterpret_cast<const uint4*>(stage + (j * THREADS + tid) * 16);
+            else v[j] = slice.row.vec(i);
+          }
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&sh.empty[s]));
+        float g = Vec<T>::largest(v[0]);
+#pragma unroll
+        for (int j = 1; j < UNROLL; ++j) g = max_nan(g, Vec<T>::largest(v[j]));
+        if (p.k) {
+          if (first < v1) this_run = max(this_run, order_key(g));
+          if (++in_run == p.chunks_per_run) {
+            run_key[run++ * THREADS + tid] = this_run;
+            best_key = max(best_key, this_run);
+            this_run = 0;
+            in_run = 0;
+          }
+        }
+        g = max_nan(m, g);
+        if (!(g <= m)) {                            // moved up (or NaN)
+          const float to = fabsf(g) <= BIG ? g * L2E : 0.f;      // out of range: nothing is added up (masks), or scanned once more
+          if (fabsf(m) <= BIG) {
+            const float d = fmaxf(ml - to, FLOOR), e = exp2f(d);
+            const uint64_t e2 = pair2(e, e), d2 = pair2(d, d), zero = pair2(0.f, 0.f);
+            u2 = fma2(fma2(d2, s2, u2), e2, zero);
+            s2 = fma2(s2, e2, zero);
+          }
+          m = g;
+          ml = to;
+        }
+        const uint64_t off = pair2(-ml, -ml);
+#pragma unroll
+        for (int j = 0; j < UNROLL; ++j) {
+          uint64_t x[VE / 2];
+          Vec<T>::pairs(v[j], x);
+#pragma unroll
+          for (int i = 0; i < VE / 2; ++i) {
+            const uint64_t y = fma2(x[i], l2e2, off);
+            float a, b;
+            split2(y, a, b);
+            const uint64_t e = pair2(exp2f(a), exp2f(b));
+            s2 = add2(s2, e);
+            u2 = fma2(e, y, u2);
+          }
+        }
+      }
+      if (p.k) {
+        if (in_run) {
+          run_key[run++ * THREADS + tid] = this_run;
+          best_key = max(best_key, this_run);
+        }
+        sh.tmax[it & 1][tid] = best_key;
+      }
+      float sa, sb, ua, ub;
+      split2(s2, sa, sb);
+      split2(u2, ua, ub);
+      // from ml to m log2e: the rounding of ml, exactly (a product's error in one fma)
+      const float d = fabsf(m) <= BIG ? -fmaf(m, L2E, -ml) : 0.f, e = exp2f(d);
+      Stat st{m, m == -INFINITY ? 0.f : (sa + sb) * e, m == -INFINITY ? 0.f : ((ua + ub) + d * (sa + sb)) * e};
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) st = merge(st, shfl_stat(st, o));
+      if (lane == 0) sh.part[it & 1][warp] = st;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(&sh.ready[it & 1]));
+    }
+  } else {
+    // ---- the finishing warp
+    uint32_t it = 0;
+    for (int row_id = row0; row_id < p.N; row_id += row_step, ++it) {
+      const Slice<T> slice(p, row_id, cr, lg);
+      wait(sh.ready[it & 1], it >> 1);
+      Stat t = lane < THREADS / 32 ? sh.part[it & 1][lane] : Stat{-INFINITY, 0.f, 0.f};
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) t = merge(t, shfl_stat(t, o));
+      if (const float top = t.m; fabsf(top) > BIG && fabsf(top) < INFINITY) {      // masks only (or logits beyond any use): see BIG
+        t = Stat{top, 0.f, 0.f};
+        for (int i = slice.v0 + lane; i < slice.v1; i += 32) {
+          float f[VE];
+          Vec<T>::unpack(slice.row.vec(i), f);
+#pragma unroll
+          for (int x = 0; x < VE; ++x) {
+            const float y = fmaxf((f[x] - top) * L2E, FLOOR), e = exp2f(y);
+            t.s += e;
+            t.u = fmaf(e, y, t.u);
+          }
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) t = merge(t, shfl_stat(t, o));
+      }
+      if (p.k) pick(p, slice, sh, run_keys + (it & 1) * p.runs * THREADS, sh.tmax[it & 1]);
+      if (lane == 0) mbar_arrive(smem_u32(&sh.finished[it & 1]));
+      if (cs > 1) {
+        if (lane == 0) sh.total = t;
+      } else {
+        finish_row<T>(p, slice, row_id, t, lane < p.k ? sh.best[lane] : 0ull);
+        __syncwarp();
+      }
+    }
+  }
+  if (cs > 1) {                                     // one row per cluster: its first CTA joins the slices
+    cluster.sync();
+    if (cr == 0 && warp == 8) {
+      Stat t = lane < cs ? cluster.map_shared_rank(&sh, lane)->total : Stat{-INFINITY, 0.f, 0.f};
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) t = merge(t, shfl_stat(t, o));
+      // unfilled places of small slices are 0: below every entry, but equal to one another, so they are dropped
+      for (int i = lane; i < cs * p.k; i += 32) sh.cand[i] = cluster.map_shared_rank(&sh, i / p.k)->best[i % p.k];
+      __syncwarp();
+      unsigned long long* out = sh.cand + 8 * MAX_TOP;
+      for (int i = lane; i < cs * p.k; i += 32) {
+        const unsigned long long mine = sh.cand[i];
+        if (!mine) continue;
+        int rank = 0;
+        for (int j = 0; j < cs * p.k; ++j) rank += sh.cand[j] > mine;
+        if (rank < p.k) out[rank] = mine;
+      }
+      __syncwarp();
+      finish_row<T>(p, Slice<T>(p, row0, cr, lg), row0, t, lane < p.k ? out[lane] : 0ull);
+    }
+    cluster.sync();                                 // no CTA leaves while its shared memory is read
+  }
+  if (*abortp)
+    for (int i = 0; i < 64; ++i) __nanosleep(1000);  // copies still in flight land before the shared memory is given back
 }
 
 // ------------------------------------------------------------------------------------------------ gradient
@@ -542,8 +659,8 @@ int launch_fwd(Fwd p, cudaStream_t stream) {
   const long long n_vec = ((long long)p.V + 2 * Vec<T>::N) / Vec<T>::N + 1;
   const long long chunks = (n_vec / cs + 1 + THREADS * UNROLL - 1) / (THREADS * UNROLL) + 1;
   p.chunks_per_run = int((chunks * THREADS + MAX_RUNS - 1) / MAX_RUNS);
-  const long long runs = (chunks + p.chunks_per_run - 1) / p.chunks_per_run + 1;
-  const size_t smem = sizeof(Shared) + (p.k ? size_t(runs) * THREADS * 4 : 0);
+  p.runs = int((chunks + p.chunks_per_run - 1) / p.chunks_per_run);
+  const size_t smem = STAGES * CHUNK + sizeof(Shared) + (p.k ? size_t(2) * p.runs * THREADS * 4 : 0);
   static std::mutex lock;
   static size_t configured[64] = {};
   int dev = 0;
@@ -556,8 +673,9 @@ int launch_fwd(Fwd p, cudaStream_t stream) {
     }
   }
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(unsigned(p.N) * cs);
-  cfg.blockDim = dim3(THREADS);
+  const long long groups = 2LL * sm_count() / cs;               // two CTAs per SM, each walks rows
+  cfg.gridDim = dim3(unsigned(p.N < groups ? p.N : groups) * cs);
+  cfg.blockDim = dim3(ALL);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
@@ -590,11 +708,11 @@ int launch_bwd(Bwd p, cudaStream_t stream) {
 
 // x [N, *] (rows `stride` elements apart, columns 0 .. V - 1 are used), bf16 or fp32; target int64 [N].
 extern "C" int lyra_token_logprobs(const void* x, int is_bf16, const long long* target, float* logprob, float* entropy, float* norm, float* top_lp,
-                                   long long* top_id, int N, int V, int k, long long stride, cudaStream_t stream) {
+                                   long long* top_id, int N, int V, int k, long long stride, int* status, cudaStream_t stream) {
   using namespace lyra::tlp;
   if (N < 1 || N > (1 << 28) || V < 1 || V > (1 << 30) || k < 0 || k > MAX_TOP || k > V || stride < V) return -90;
   if (reinterpret_cast<uintptr_t>(x) % (is_bf16 ? 2 : 4)) return -90;
-  Fwd p{x, target, logprob, entropy, norm, top_lp, top_id, stride, N, V, k, 1};
+  Fwd p{x, target, logprob, entropy, norm, top_lp, top_id, stride, status, N, V, k, 1, 1};
   return is_bf16 ? launch_fwd<__nv_bfloat16>(p, stream) : launch_fwd<float>(p, stream);
 }
 

@@ -42,10 +42,10 @@ def _forward(logits, targets, k: int, vocab: int, norm: torch.Tensor | None):
     logprob, entropy = torch.empty(N, dtype=torch.float32, device=dev), torch.empty(N, dtype=torch.float32, device=dev)
     top_lp, top_id = torch.empty(N, k, dtype=torch.float32, device=dev), torch.empty(N, k, dtype=torch.int64, device=dev)
     if N:
-        fn = native.function("lyra_token_logprobs", "pippppppiiilp")
+        fn = native.function("lyra_token_logprobs", "pippppppiiilpp")
         native.check(fn(logits.data_ptr(), logits.dtype == torch.bfloat16, targets.data_ptr(), logprob.data_ptr(), entropy.data_ptr(),
                         norm.data_ptr() if norm is not None else None, top_lp.data_ptr(), top_id.data_ptr(), N, vocab, k, logits.stride(0),
-                        native.stream_address()), "lyra_token_logprobs")
+                        native.status_word().data_ptr(), native.stream_address()), "lyra_token_logprobs")
         native.count_launch()
     return logprob, entropy, top_lp, top_id
 
