@@ -225,6 +225,7 @@ __device__ __forceinline__ void rank_select(const unsigned long long* list, int 
   for (int i = threadIdx.x & 31; i < n; i += 32) {
     const unsigned long long mine = list[i];
     int rank = 0;
+#pragma unroll 8
     for (int j = 0; j < n; ++j) rank += list[j] > mine;
     if (rank < k) out[rank] = mine;
   }
@@ -561,23 +562,26 @@ __global__ void __launch_bounds__(ALL, 2) token_logprobs_kernel(const Fwd p) {
   }
   if (cs > 1) {                                     // one row per cluster: its first CTA joins the slices
     cluster.sync();
-    if (cr == 0 && warp == 8) {
-      Stat t = lane < cs ? cluster.map_shared_rank(&sh, lane)->total : Stat{-INFINITY, 0.f, 0.f};
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) t = merge(t, shfl_stat(t, o));
+    if (cr == 0) {
       // unfilled places of small slices are 0: below every entry, but equal to one another, so they are dropped
-      for (int i = lane; i < cs * p.k; i += 32) sh.cand[i] = cluster.map_shared_rank(&sh, i / p.k)->best[i % p.k];
-      __syncwarp();
+      const int n = cs * p.k;                       // at most 256
       unsigned long long* out = sh.cand + 8 * MAX_TOP;
-      for (int i = lane; i < cs * p.k; i += 32) {
-        const unsigned long long mine = sh.cand[i];
-        if (!mine) continue;
+      if (tid < n) sh.cand[tid] = cluster.map_shared_rank(&sh, tid / p.k)->best[tid % p.k];
+      __syncthreads();
+      if (tid < n && sh.cand[tid]) {
+        const unsigned long long mine = sh.cand[tid];
         int rank = 0;
-        for (int j = 0; j < cs * p.k; ++j) rank += sh.cand[j] > mine;
+#pragma unroll 8
+        for (int j = 0; j < n; ++j) rank += sh.cand[j] > mine;
         if (rank < p.k) out[rank] = mine;
       }
-      __syncwarp();
-      finish_row<T>(p, Slice<T>(p, row0, cr, lg), row0, t, lane < p.k ? out[lane] : 0ull);
+      __syncthreads();
+      if (warp == 8) {
+        Stat t = lane < cs ? cluster.map_shared_rank(&sh, lane)->total : Stat{-INFINITY, 0.f, 0.f};
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) t = merge(t, shfl_stat(t, o));
+        finish_row<T>(p, Slice<T>(p, row0, cr, lg), row0, t, lane < p.k ? out[lane] : 0ull);
+      }
     }
     cluster.sync();                                 // no CTA leaves while its shared memory is read
   }
@@ -599,6 +603,8 @@ constexpr int B_THREADS = 256, B_UNROLL = 4;
 
 // Bound by memory: every logit is read once and every gradient written once, in 16-byte pieces aligned to the gradient's row
 // (which a row of logits with the same distance from a 16-byte boundary shares; otherwise its elements are loaded one by one).
+// With d = x - m:  p = 2^{d log2e - log2 s},  g = -p (g_H d + c),  c = g_l + g_H (H - log s): 5.5 operations a logit, the target's
+// term is added to the one vector that holds it. A row without a distribution has NaN for m, d is cut off and p is 0, but c is NaN.
 template <typename T>
 __global__ void __launch_bounds__(B_THREADS) token_logprobs_bwd_kernel(const Bwd p) {
   constexpr int VE = Vec<T>::N;
@@ -609,44 +615,53 @@ __global__ void __launch_bounds__(B_THREADS) token_logprobs_bwd_kernel(const Bwd
   const int lead = int((reinterpret_cast<uintptr_t>(dx) & 15) / sizeof(T));
   const bool same = ((reinterpret_cast<uintptr_t>(x) ^ reinterpret_cast<uintptr_t>(dx)) & 15) == 0;
   const int n_vec = int(((long long)p.W + lead + VE - 1) / VE);
-  const long long tg = p.target[r];
-  float gl = p.g_lp && tg >= 0 ? p.g_lp[r] : 0.f;
-  if (tg >= p.V) gl = __uint_as_float(0x7fc00000u);
-  const float gh = p.g_h ? p.g_h[r] : 0.f, m = p.norm[r], log_s = p.norm[p.N + r], H = p.entropy[r];
-  const float base = gl + gh * H;
-  uint4 v[B_UNROLL];
   const int first = blk * B_THREADS * B_UNROLL + threadIdx.x;
+  uint4 v[B_UNROLL];
 #pragma unroll
   for (int j = 0; j < B_UNROLL; ++j) {
     const int i = first + j * B_THREADS, e0 = i * VE - lead;
     if (i < n_vec && same && e0 >= 0 && e0 + VE <= p.V) v[j] = __ldg(reinterpret_cast<const uint4*>(x + e0));
   }
+  const long long tg = p.target[r];
+  float gl = p.g_lp && tg >= 0 ? p.g_lp[r] : 0.f;
+  if (tg >= p.V) gl = __uint_as_float(0x7fc00000u);
+  const float gh = p.g_h ? p.g_h[r] : 0.f, m = p.norm[r], log_s = p.norm[p.N + r], H = p.entropy[r];
+  const float c = m != m ? m : fmaf(gh, H - log_s, gl), shift = -log_s * L2E;
+  // whatever the target's place, as a vector index; -1 for none
+  const int hot = tg >= 0 && tg < p.V ? int((tg + lead) / VE) : -1;
 #pragma unroll
   for (int j = 0; j < B_UNROLL; ++j) {
     const int i = first + j * B_THREADS, e0 = i * VE - lead;
     if (i >= n_vec) continue;
-    const bool whole = e0 >= 0 && e0 + VE <= p.W;
+    const bool inside = e0 >= 0 && e0 + VE <= p.V;
     float f[VE];
-    if (same && e0 >= 0 && e0 + VE <= p.V) {
+    if (same && inside) {
       Vec<T>::unpack(v[j], f);
     } else {
 #pragma unroll
       for (int q = 0; q < VE; ++q) f[q] = (e0 + q >= 0 && e0 + q < p.V) ? Vec<T>::load(x + e0 + q) : -INFINITY;
     }
 #pragma unroll
-    for (int q = 0; q < VE; ++q) {
-      const float lp = fmaxf((f[q] - m) - log_s, FLOOR);        // a probability of 0 contributes 0, not 0 * inf
-      const float pr = exp2f(lp * L2E);
-      float g = -pr * fmaf(gh, lp, base);
-      if (e0 + q == tg) g += gl;
-      f[q] = e0 + q < p.V ? (m != m ? m : g) : 0.f;       // fmaxf drops a NaN: a row without a distribution has no gradient
+    for (int q = 0; q < VE; q += 2) {
+      const float d0 = fmaxf(f[q] - m, FLOOR), d1 = fmaxf(f[q + 1] - m, FLOOR);      // a probability of 0 contributes 0, not 0 * inf
+      const uint64_t d = pair2(d0, d1);
+      float y0, y1, w0, w1;
+      split2(fma2(d, pair2(L2E, L2E), pair2(shift, shift)), y0, y1);
+      split2(fma2(d, pair2(gh, gh), pair2(c, c)), w0, w1);
+      f[q] = -exp2f(y0) * w0;
+      f[q + 1] = -exp2f(y1) * w1;
     }
-    if (whole) {
+    if (i == hot) {
+#pragma unroll
+      for (int q = 0; q < VE; ++q)
+        if (e0 + q == tg) f[q] += gl;
+    }
+    if (inside) {
       *reinterpret_cast<uint4*>(dx + e0) = Vec<T>::pack(f);
     } else {
 #pragma unroll
       for (int q = 0; q < VE; ++q)
-        if (e0 + q >= 0 && e0 + q < p.W) dx[e0 + q] = T(f[q]);
+        if (e0 + q >= 0 && e0 + q < p.W) dx[e0 + q] = T(e0 + q < p.V ? f[q] : 0.f);
     }
   }
 }
