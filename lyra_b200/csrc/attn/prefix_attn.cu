@@ -13,10 +13,12 @@
 //
 // Prefix kernel, per item (row tile, kv head, key split), one persistent CTA per SM:
 //   warp 0        TMA producer: K and V tiles of 128 keys (bf16: straight into the operand tiles; e4m3: into a raw ring)
-//   warp 1        tcgen05 issuer:  S_g = Q K_j^T  and  O_g += P_g V_j   (g = j mod 2)
+//   warp 1        tcgen05 issuer:  S = Q K_j^T  and, e4m3, O_g += P V_j   (g = j mod 2)
+//   warp 10       bf16: issuer of O_g += P V_j, so that neither product's barriers hold up the other's instructions
 //   warps 2..9    two softmax groups of four warps, alternate key tiles, one row per thread; each has its own scores, maximum, sum and
 //                 accumulator, merged once per item. P replaces S in TMEM as packed bf16 and is the MMA's TMEM operand.
-//   warps 10, 11  gather the query rows (any strides) into the operand tile; e4m3: also turn raw K / V tiles into bf16 operand tiles.
+//   warp 11, e4m3: 10 and 11   gather the query rows (any strides) into the operand tile; e4m3: also turn raw K / V tiles into bf16
+//                 operand tiles.
 //                 That conversion is exact; a key's scale multiplies its score, a value's scale its probability, both in fp32.
 #include <cooperative_groups.h>
 #include <cuda_fp8.h>
@@ -30,7 +32,7 @@ namespace prefix {
 namespace cg = cooperative_groups;
 
 constexpr float L2E = 1.4426950408889634f;
-constexpr int THREADS = 384, LOADERS = 64;      // warps 0, 1 | 2..9 | 10, 11
+constexpr int THREADS = 384;                    // warps 0, 1 | 2..9 | 10, 11
 constexpr int BM = 128, BN = 128;               // rows and keys of a tile
 constexpr int MAX_SPLITS = 32;
 constexpr int POLY_AT = 6;                      // place in a run of eight scores of the pair that is exponentiated by polynomial
@@ -59,8 +61,10 @@ struct Item {
 __device__ __forceinline__ void cp16(uint32_t dst, const void* src, int nbytes) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(nbytes) : "memory");
 }
-// Barrier of the two loader warps that also tells both whether both are well: they leave together or not at all.
+// Barrier of the loader warps that also tells all whether all are well: they leave together or not at all.
+template <int LOADERS>
 __device__ __forceinline__ bool loaders_agree(bool ok) {
+  if (LOADERS == 32) return __all_sync(0xffffffffu, ok);
   uint32_t all;
   asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbar.red.and.pred q, 2, 64, p;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(all) : "r"(uint32_t(ok)) : "memory");
   return all != 0;
@@ -113,6 +117,7 @@ struct Smem {
   // Score buffers in TMEM and stages of the K and V rings. Head dim 64: two accumulators leave room for a third score buffer, so the
   // scores of a group's next tile are ready when it finishes one; with two it waits for P V and Q K^T in between.
   static constexpr int NS = D == 64 ? 3 : 2;
+  static constexpr int LOADERS = FP8 ? 64 : 32;
   static constexpr int BYTES = (1 + 2 * NS) * TILE + (FP8 ? RAW * RAW_TILE : 0) + 1024;
 };
 
@@ -125,7 +130,7 @@ __device__ __forceinline__ uint32_t e4m3x2_to_bf16x2(uint16_t two) {      // exa
 template <int D, bool FP8>
 __global__ void __launch_bounds__(THREADS, 1)
 prefix_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv, const Params p) {
-  constexpr int TILE = Smem<D, FP8>::TILE, RAW_TILE = Smem<D, FP8>::RAW_TILE, RAW = Smem<D, FP8>::RAW, NS = Smem<D, FP8>::NS;
+  constexpr int TILE = Smem<D, FP8>::TILE, RAW_TILE = Smem<D, FP8>::RAW_TILE, RAW = Smem<D, FP8>::RAW, NS = Smem<D, FP8>::NS, LOADERS = Smem<D, FP8>::LOADERS;
   constexpr int HALF = 128 * 128;               // bytes of one 64-column block of an operand tile
   constexpr uint32_t TMEM_COLS = 512, S_COL = 0, O_COL = NS * 128, O_COLS = NS == 3 ? 64 : 128;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");         // own_kernel may start wherever there is room
@@ -134,7 +139,7 @@ prefix_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CU
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t *sQ = smem, *sK = sQ + TILE, *sV = sK + NS * TILE, *sR = sV + NS * TILE;
-  __shared__ uint64_t q_full, q_empty, k_full[NS], v_full[NS], v_empty[NS], s_full[NS], p_full[NS], o_full, o_empty, l_full;
+  __shared__ uint64_t q_full, q_empty, k_full[NS], v_empty[NS], s_full[NS], p_full[NS], o_full, o_empty, l_full;   // p_full: P and V are there
   __shared__ uint64_t raw_full[RAW], raw_empty[RAW], sc_full[SLOTS];
   __shared__ float xm[2][2][BM], xl[2][2][BM];  // [item parity][group][row]
   __shared__ __align__(16) float ksc[FP8 ? SLOTS : 1][BN], vsc[FP8 ? SLOTS : 1][BN];   // scales of the key tiles in flight
@@ -166,10 +171,9 @@ prefix_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CU
     mbar_init(smem_u32(&q_empty), 1);
     for (int s = 0; s < NS; ++s) {
       mbar_init(smem_u32(&k_full[s]), FP8 ? LOADERS : 1);
-      mbar_init(smem_u32(&v_full[s]), FP8 ? LOADERS : 1);
       mbar_init(smem_u32(&v_empty[s]), 1);
       mbar_init(smem_u32(&s_full[s]), 1);
-      mbar_init(smem_u32(&p_full[s]), 128);
+      mbar_init(smem_u32(&p_full[s]), 128 + (FP8 ? LOADERS : 1));
     }
     for (int s = 0; s < RAW; ++s) {
       mbar_init(smem_u32(&raw_full[s]), 1);
@@ -219,8 +223,8 @@ prefix_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CU
             mbar_expect_tx(smem_u32(&k_full[s]), TILE);
             for (int c = 0; c < D / 64; ++c) tma_load_3d(smem_u32(sK + s * TILE + c * HALF), &tk, smem_u32(&k_full[s]), c * 64, k0, w.h);
             if (!mbar_wait(smem_u32(&v_empty[s]), ph ^ 1, abortp)) { ok = false; break; }
-            mbar_expect_tx(smem_u32(&v_full[s]), TILE);
-            for (int c = 0; c < D / 64; ++c) tma_load_3d(smem_u32(sV + s * TILE + c * HALF), &tv, smem_u32(&v_full[s]), c * 64, k0, w.h);
+            mbar_expect_tx(smem_u32(&p_full[s]), TILE);
+            for (int c = 0; c < D / 64; ++c) tma_load_3d(smem_u32(sV + s * TILE + c * HALF), &tv, smem_u32(&p_full[s]), c * 64, k0, w.h);
           }
         }
       }
@@ -229,53 +233,59 @@ prefix_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CU
         abort_flag = 1;
       }
     }
-  } else if (warp == 1) {
-    // The whole warp walks the tiles and one elected lane issues: the loop's values are then the same in all lanes for the compiler
+  } else if (warp == 1 || (!FP8 && warp == 10)) {
+    // A whole warp walks the tiles and one elected lane issues: the loop's values are then the same in all lanes for the compiler
     // too and live in uniform registers, from which the MMA takes its descriptors. (With the loop itself inside `lane == 0`, moving
     // them there took most of 2000 clk per tile; the tensor core needs about 600 for it.)
-    // MMAs of one thread retire in issue order: the scores of tile j + NS, issued after P(j) V_j, cannot overwrite P(j) before it
-    // was read.
+    const bool scores = warp == 1, outputs = FP8 || warp == 10;
     uint32_t n = 0, ks = 0, kph = 0, vs = 0, vph = 0;       // stage and parity of the next K tile (scores) and of the next V tile
     bool ok = true;
     const uint64_t dq0 = make_smem_desc(smem_u32(sQ), 16, 1024), dk0 = make_smem_desc(smem_u32(sK), 16, 1024);
     const uint64_t dv0 = make_smem_desc(smem_u32(sV), HALF, 1024);
-    for (int round = 0; ok && item_at(round, w); ++round) {
-      auto issue_s = [&](bool last) -> bool {
-        if (!mbar_wait(smem_u32(&k_full[ks]), kph, abortp)) return false;
-        tc_fence_after();
-        if (elect_one()) {
-          const uint64_t dk = desc_advance(dk0, ks * TILE);
+    auto issue_s = [&](bool last) -> bool {
+      if (!mbar_wait(smem_u32(&k_full[ks]), kph, abortp)) return false;
+      if (!outputs && !mbar_wait(smem_u32(&v_empty[ks]), kph ^ 1, abortp)) return false;   // the buffer's P has been read (own MMAs retire in order)
+      tc_fence_after();
+      if (elect_one()) {
+        const uint64_t dk = desc_advance(dk0, ks * TILE);
 #pragma unroll
-          for (int k = 0; k < D / 16; ++k)
-            tc_mma_ss(tmem + S_COL + ks * 128, desc_advance(dq0, (k / 4) * HALF + (k % 4) * 32), desc_advance(dk, (k / 4) * HALF + (k % 4) * 32), IDESC_S, k > 0);
-          tc_commit(smem_u32(&s_full[ks]));
-          if (last) tc_commit(smem_u32(&q_empty));
-        }
-        __syncwarp();
-        if (++ks == NS) { ks = 0; kph ^= 1; }
-        return true;
-      };
-      ok = mbar_wait(smem_u32(&q_full), n & 1, abortp);
-      for (int j = 0; ok && j < NS && j < w.tiles; ++j) ok = issue_s(j == w.tiles - 1);
+        for (int k = 0; k < D / 16; ++k)
+          tc_mma_ss(tmem + S_COL + ks * 128, desc_advance(dq0, (k / 4) * HALF + (k % 4) * 32), desc_advance(dk, (k / 4) * HALF + (k % 4) * 32), IDESC_S, k > 0);
+        tc_commit(smem_u32(&s_full[ks]));
+        if (last) tc_commit(smem_u32(&q_empty));
+      }
+      __syncwarp();
+      if (++ks == NS) { ks = 0; kph ^= 1; }
+      return true;
+    };
+    auto issue_o = [&](int j, bool last) -> bool {
+      if (!mbar_wait(smem_u32(&p_full[vs]), vph, abortp)) return false;
+      tc_fence_after();
+      if (elect_one()) {
+        const uint64_t dv = desc_advance(dv0, vs * TILE);
+#pragma unroll
+        for (int k = 0; k < BN / 16; ++k)
+          tc_mma_ts(tmem + O_COL + (j & 1) * O_COLS, tmem + S_COL + vs * 128 + k * 8, desc_advance(dv, k * 2048), IDESC_O, (j >= 2 || k > 0) ? 1u : 0u);
+        tc_commit(smem_u32(&v_empty[vs]));
+        if (last) tc_commit(smem_u32(&o_full));
+      }
+      __syncwarp();
+      if (++vs == NS) { vs = 0; vph ^= 1; }
+      return true;
+    };
+    for (int round = 0; ok && item_at(round, w); ++round, ++n) {
+      if (scores) ok = mbar_wait(smem_u32(&q_full), n & 1, abortp);
+      if (scores && !outputs) {
+        for (int j = 0; j < w.tiles && ok; ++j) ok = issue_s(j == w.tiles - 1);
+        continue;
+      }
+      if (scores)
+        for (int j = 0; ok && j < NS && j < w.tiles; ++j) ok = issue_s(j == w.tiles - 1);
       if (ok) ok = mbar_wait(smem_u32(&o_empty), (n & 1) ^ 1, abortp);       // the previous item's output has been read
       for (int j = 0; j < w.tiles && ok; ++j) {
-        const int g = j & 1;
-        if (!mbar_wait(smem_u32(&v_full[vs]), vph, abortp)) { ok = false; break; }
-        if (!mbar_wait(smem_u32(&p_full[vs]), vph, abortp)) { ok = false; break; }
-        tc_fence_after();
-        if (elect_one()) {
-          const uint64_t dv = desc_advance(dv0, vs * TILE);
-#pragma unroll
-          for (int k = 0; k < BN / 16; ++k)
-            tc_mma_ts(tmem + O_COL + g * O_COLS, tmem + S_COL + vs * 128 + k * 8, desc_advance(dv, k * 2048), IDESC_O, (j >= 2 || k > 0) ? 1u : 0u);
-          tc_commit(smem_u32(&v_empty[vs]));
-          if (j == w.tiles - 1) tc_commit(smem_u32(&o_full));
-        }
-        __syncwarp();
-        if (++vs == NS) { vs = 0; vph ^= 1; }
-        if (j + NS < w.tiles) ok = issue_s(j + NS == w.tiles - 1);
+        ok = issue_o(j, j == w.tiles - 1);
+        if (scores && ok && j + NS < w.tiles) ok = issue_s(j + NS == w.tiles - 1);
       }
-      ++n;
     }
     if (!ok) {
       if (lane == 0) atomicCAS(p.status, 0, STATUS_TIMEOUT_FULL);
@@ -283,7 +293,7 @@ prefix_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CU
     }
   } else if (warp >= 10) {
     // ------------------------------------------------------------ query rows; e4m3 tiles to bf16
-    const int tid = threadIdx.x - 320;
+    const int tid = threadIdx.x - (THREADS - LOADERS);
     constexpr int CPR = D / 8;                  // 16-byte chunks per query row
     uint32_t t = 0, n = 0;
     bool ok = true;
@@ -293,7 +303,7 @@ prefix_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CU
         const int m = w.m0 + r, bt = m / p.rep, b = bt / p.T;
         q_row[r] = m < M ? b * p.q_sb + (long long)(w.h * p.rep + m - bt * p.rep) * p.q_sn + (long long)(bt - b * p.T) * p.q_st : -1;
       }
-      if (!(ok = loaders_agree(ok))) break;
+      if (!(ok = loaders_agree<LOADERS>(ok))) break;
       if (!mbar_wait(smem_u32(&q_empty), (n & 1) ^ 1, abortp)) ok = false;
       if (ok) {
 #pragma unroll 8
@@ -304,7 +314,7 @@ prefix_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CU
         }
         asm volatile("cp.async.wait_all;" ::: "memory");
       }
-      if (!(ok = loaders_agree(ok))) break;                  // the table is rewritten for the next item after this
+      if (!(ok = loaders_agree<LOADERS>(ok))) break;                  // the table is rewritten for the next item after this
       fence_proxy_async_smem();
       mbar_arrive(smem_u32(&q_full));
       if (FP8) {
@@ -349,7 +359,7 @@ prefix_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CU
             }
             fence_proxy_async_smem();
             mbar_arrive(smem_u32(&raw_empty[rs]));
-            mbar_arrive(smem_u32(which ? &v_full[s] : &k_full[s]));
+            mbar_arrive(smem_u32(which ? &p_full[s] : &k_full[s]));
           }
         }
       }
