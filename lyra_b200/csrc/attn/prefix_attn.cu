@@ -865,25 +865,30 @@ __global__ void __launch_bounds__(OTHREADS, D == 64 ? 4 : 3) own_kernel(const Ow
     const int r = tid / TPR, x = tid % TPR, n_own = ROWS ? 1 : p.cluster, n = n_own + p.splits;
     const int mrow = b * R + row0 + (r < n_rows ? r : 0);      // row of the prefix product
     const float2* prefix_ml = p.part_ml + ((long long)h * p.prefix_tiles + mrow / BM) * p.splits * BM + mrow % BM;
-    float M = -INFINITY, L = 0.f;
     auto ml = [&](int j) -> float2 {
       if (j >= n_own) return __ldcg(prefix_ml + (j - n_own) * BM);
       if (ROWS || p.cluster == 1) return make_float2(comb_m[r], comb_l[r]);
       return make_float2(*cluster.map_shared_rank(&comb_m[r], j), *cluster.map_shared_rank(&comb_l[r], j));
     };
     const float sink = p.sinks && r < n_rows ? __ldg(p.sinks + h * p.rep + (row0 + r) % p.rep) * L2E : -INFINITY;
-    if (r < n_rows)
-      for (int j = x; j < n; j += TPR) M = fmaxf(M, ml(j).x);
+    constexpr int PER = (MAXW + TPR - 1) / TPR;                  // a thread's share, all fetched at once
+    float2 part[PER];
+#pragma unroll
+    for (int i = 0; i < PER; ++i) part[i] = r < n_rows && x + i * TPR < n ? ml(x + i * TPR) : make_float2(-INFINITY, 0.f);
+    float M = -INFINITY, L = 0.f;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) M = fmaxf(M, part[i].x);
 #pragma unroll
     for (int of = TPR / 2; of > 0; of >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, of));
     M = fmaxf(M, sink);
-    if (r < n_rows)
-      for (int j = x; j < n; j += TPR) {
-        const float2 v = ml(j);
-        const float f = v.x == -INFINITY ? 0.f : exp2f(v.x - M);
-        weight[r][j] = f;
-        L += v.y * f;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      if (r < n_rows && x + i * TPR < n) {
+        const float f = part[i].x == -INFINITY ? 0.f : exp2f(part[i].x - M);
+        weight[r][x + i * TPR] = f;
+        L += part[i].y * f;
       }
+    }
 #pragma unroll
     for (int of = TPR / 2; of > 0; of >>= 1) L += __shfl_xor_sync(0xffffffffu, L, of);
     if (sink != -INFINITY) L += exp2f(sink - M);
@@ -891,34 +896,77 @@ __global__ void __launch_bounds__(OTHREADS, D == 64 ? 4 : 3) own_kernel(const Ow
   }
   __syncthreads();
 
-  auto finish = [&](int r, int d, float v) -> float {             // + the prefix's splits, times 1 / L
-    const float inv = weight[r][MAXW];
-    if (inv == 0.f) return 0.f;                                  // nothing visible, or an unused place: whatever the sums hold
-    const int mrow = b * R + row0 + r;
-    const float* po = p.part_o + (((long long)h * p.prefix_tiles + mrow / BM) * p.splits * D + d) * BM + mrow % BM;
-    const float* wp = &weight[r][ROWS ? 1 : p.cluster];
-#pragma unroll 8
-    for (int j = 0; j < p.splits; ++j) v = fmaf(__ldcg(po + (long long)j * D * BM), wp[j], v);
-    return v * inv;
-  };
   // ---- sums, a row's columns dealt to the CTAs of a cluster. Neighbouring threads take neighbouring rows, which lie side by side in
-  // the prefix partials; the results go through shared memory (over this CTA's own partial) and leave row by row.
+  // the prefix partials (four at a time where they start on such a border); the results go through shared memory and leave row by row.
+  // A thread fetches the splits of several places before it adds them up: one place at a time this took up to 15 us, most of it waiting.
   const int dn = D / p.cluster, d0 = rank * dn;                  // this CTA's columns
-  if (ROWS || p.cluster == 1) {
-    for (int i = tid; i < n_rows * D; i += OTHREADS) {
-      const int d = i / n_rows, r = i - d * n_rows;
-      comb[r * PITCH + d] = finish(r, d, comb[r * PITCH + d] * weight[r][0]);
+  const int m0 = b * R + row0, n_own = ROWS ? 1 : p.cluster;
+  float* result = ROWS || p.cluster == 1 ? comb : warp_o;        // in place, unless the cluster's other CTAs still read it
+  const float* part = p.part_o + ((long long)h * p.prefix_tiles + m0 / BM) * p.splits * D * BM + m0 % BM;
+  auto own_part = [&](int r, int d) -> float {
+    if (ROWS || p.cluster == 1) return comb[r * PITCH + d] * weight[r][0];
+    float v = 0.f;
+    for (int j = 0; j < p.cluster; ++j) v += *cluster.map_shared_rank(comb + r * PITCH + d, j) * weight[r][j];
+    return v;
+  };
+  // a tile's rows end at a multiple of 128: row r of this CTA in tile (m0 + r) / 128
+  auto place = [&](int r, int d) { return part + (long long)((m0 % BM + r) / BM) * p.splits * D * BM + d * BM + r - (m0 % BM + r) / BM * BM; };
+  if (n_rows % 4 == 0 && m0 % 4 == 0) {
+    const int nq = n_rows / 4, total = dn * nq;
+    constexpr int E = 2;
+    for (int i0 = tid; i0 < total; i0 += E * OTHREADS) {
+      float4 v[E];
+#pragma unroll
+      for (int e = 0; e < E; ++e) v[e] = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int j0 = 0; j0 < p.splits; j0 += 4) {
+        float4 x[E][4];
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+          const int i = min(i0 + e * OTHREADS, total - 1), d = d0 + i / nq, r = i % nq * 4;
+          const float* at = place(r, d);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) x[e][j] = __ldcg(reinterpret_cast<const float4*>(at + (long long)min(j0 + j, p.splits - 1) * D * BM));
+        }
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+          const int r = min(i0 + e * OTHREADS, total - 1) % nq * 4;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            if (j0 + j < p.splits) {
+              v[e].x = fmaf(x[e][j].x, weight[r][n_own + j0 + j], v[e].x);
+              v[e].y = fmaf(x[e][j].y, weight[r + 1][n_own + j0 + j], v[e].y);
+              v[e].z = fmaf(x[e][j].z, weight[r + 2][n_own + j0 + j], v[e].z);
+              v[e].w = fmaf(x[e][j].w, weight[r + 3][n_own + j0 + j], v[e].w);
+            }
+          }
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        const int i = i0 + e * OTHREADS, d = d0 + i / nq, r = i % nq * 4;
+        if (i < total) {
+          const float add[4] = {v[e].x, v[e].y, v[e].z, v[e].w};
+#pragma unroll
+          for (int y = 0; y < 4; ++y) {
+            const float inv = weight[r + y][MAXW];               // 0: nothing visible, or an unused place - whatever the sums hold
+            result[(r + y) * PITCH + d] = inv == 0.f ? 0.f : (own_part(r + y, d) + add[y]) * inv;
+          }
+        }
+      }
     }
   } else {
     for (int i = tid; i < n_rows * dn; i += OTHREADS) {
       const int d = d0 + i / n_rows, r = i % n_rows;
+      const float inv = weight[r][MAXW];
+      const float* at = place(r, d);
       float v = 0.f;
-      for (int j = 0; j < p.cluster; ++j) v += *cluster.map_shared_rank(comb + r * PITCH + d, j) * weight[r][j];
-      warp_o[r * PITCH + d] = finish(r, d, v);
+#pragma unroll 8
+      for (int j = 0; j < p.splits; ++j) v = fmaf(__ldcg(at + (long long)j * D * BM), weight[r][n_own + j], v);
+      result[r * PITCH + d] = inv == 0.f ? 0.f : (own_part(r, d) + v) * inv;
     }
   }
   __syncthreads();
-  const float* done = ROWS || p.cluster == 1 ? comb : warp_o;
+  const float* done = result;
   for (int i = tid; i < n_rows * (dn / 8); i += OTHREADS) {
     const int r = i / (dn / 8), d = d0 + i % (dn / 8) * 8;
     const float4 x = *reinterpret_cast<const float4*>(done + r * PITCH + d), y = *reinterpret_cast<const float4*>(done + r * PITCH + d + 4);
