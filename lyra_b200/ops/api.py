@@ -17,6 +17,10 @@ import sys
 
 import torch
 
+from lyra_b200.nn.quant import QArray, dequantize
+from lyra_b200.ops import attention as attn_k
+from lyra_b200.ops import decode as decode_k
+from lyra_b200.ops import logprobs as logprobs_k
 from lyra_b200.ops import native
 from lyra_b200.ops import reference as ref
 
@@ -125,9 +129,6 @@ def prefix_attention(q, prefix_k, prefix_v, k_cache, v_cache, sinks, scale: floa
     with ``pos < 0`` is an unused place of the batch: zeros, as for a query that sees nothing without a sink.
 
     On a GPU: head dim 64 or 128; the prefix is read once per 128 query rows of a kv head instead of once per sequence."""
-    from lyra_b200.nn.quant import QArray, dequantize
-    from lyra_b200.ops import attention as attn_k
-
     attn_k.check_prefix_attention(q, prefix_k, prefix_v, k_cache, v_cache, sinks, scale, window, pos)
     if use_kernels(q, implementation):
         return attn_k.prefix_attention(q, prefix_k, prefix_v, k_cache, v_cache, sinks, scale, window, pos)
@@ -176,12 +177,10 @@ def token_logprobs(logits, targets, top_k: int = 0, vocab_size: int | None = Non
     ``logprob`` and ``entropy`` are differentiable with respect to ``logits`` (once); the alternatives are not. A negative target
     marks a position without a token: its log probability is 0 and carries no gradient. A target from ``vocab_size`` on, a row
     with a NaN or +inf, or one of nothing but -inf, has NaN scores and gradients. A logit of -inf is a token of probability 0."""
-    from lyra_b200.ops import logprobs
-
-    vocab = logprobs.check_arguments(logits, targets, top_k, vocab_size)
+    vocab = logprobs_k.check_arguments(logits, targets, top_k, vocab_size)
     if use_kernels(logits, implementation):
-        return logprobs.token_logprobs(logits, targets, top_k, vocab)
-    return logprobs.TokenLogprobs(*ref.token_logprobs(logits, targets, top_k, vocab))
+        return logprobs_k.token_logprobs(logits, targets, top_k, vocab)
+    return logprobs_k.TokenLogprobs(*ref.token_logprobs(logits, targets, top_k, vocab))
 
 
 def embedding(emb, tokens, implementation: str = "auto", presorted: bool = True):
@@ -241,12 +240,9 @@ def moe_block(x, norm_scale, eps: float, router, router_bias, w_up, up_bias, w_d
 
     The router works on the unrounded normalised input in fp32. On a GPU: one kernel for 1..64 tokens of bf16 (``ops.decode.
     moe_block_supported`` names the shapes), which reads the chosen experts' weights once."""
-    from lyra_b200.nn.quant import QArray, dequantize
-    from lyra_b200.ops import decode
-
-    n, C, H = decode.check_moe_block(x, norm_scale, router, router_bias, w_up, up_bias, w_down, down_bias, k, n_shared)
+    n, C, H = decode_k.check_moe_block(x, norm_scale, router, router_bias, w_up, up_bias, w_down, down_bias, k, n_shared)
     if use_kernels(x, implementation):
-        return decode.moe_block(x, norm_scale, eps, router, router_bias, w_up, up_bias, w_down, down_bias, k, n_shared, beta, limit, residual_scale)
+        return decode_k.moe_block(x, norm_scale, eps, router, router_bias, w_up, up_bias, w_down, down_bias, k, n_shared, beta, limit, residual_scale)
 
     def expert(e):
         pick = lambda w: dequantize(QArray(w.qval[e], w.scale[e], w.block), torch.float32) if isinstance(w, QArray) else w[e]

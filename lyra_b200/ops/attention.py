@@ -98,36 +98,39 @@ def check_prefix_attention(q, prefix_k, prefix_v, k_cache, v_cache, sinks, scale
     if q.ndim != 4 or not q.is_floating_point():
         raise ValueError(f"q must be a floating-point [B, Nq, T, D], got {tuple(q.shape)} {q.dtype}")
     B, Nq, T, D = q.shape
-    tensors = [q]
-    for name, kv, lead in (("prefix", (prefix_k, prefix_v), ()), ("own cache", (k_cache, v_cache), (B,))):
-        if isinstance(kv[0], QArray) != isinstance(kv[1], QArray):
+    device, tensors = q.device, [q]
+    for name, keys, values, axes in (("prefix", prefix_k, prefix_v, 3), ("own cache", k_cache, v_cache, 4)):
+        quantised = isinstance(keys, QArray)
+        if quantised != isinstance(values, QArray):
             raise ValueError(f"{name}: keys and values must both be quantised or both not")
-        shape = tuple(kv[0].shape)
-        if tuple(kv[1].shape) != shape or len(shape) != len(lead) + 3 or shape[:-3] != lead or shape[-1] != D or shape[-3] < 1 or Nq % shape[-3]:
-            raise ValueError(f"{name}: keys {shape} and values {tuple(kv[1].shape)} must be {[*lead, 'Nkv', 'positions', D]} with Nkv a divisor of {Nq}")
-        for t in kv:
-            if isinstance(t, QArray):
+        shape = keys.shape
+        if len(shape) != axes or values.shape != shape or shape[-1] != D or shape[-3] < 1 or Nq % shape[-3] or (axes == 4 and shape[0] != B):
+            raise ValueError(f"{name}: keys {tuple(shape)} and values {tuple(values.shape)} must be {['B', 'Nkv', 'positions', D][4 - axes:]} with B {B} and "
+                             f"Nkv a divisor of {Nq}")
+        if quantised:
+            for t in (keys, values):
                 if tuple(t.block) != (1, D) or tuple(t.scale.shape) != (*shape[:-1], 1):
                     raise ValueError(f"{name}: a quantised cache has blocks (1, {D}), got {t.block} with scales {tuple(t.scale.shape)}")
-                tensors += [t.qval, t.scale]
-            else:
-                tensors.append(t)
+                tensors += (t.qval, t.scale)
+        else:
+            tensors += (keys, values)
     if prefix_k.shape[0] != k_cache.shape[1]:
         raise ValueError(f"{prefix_k.shape[0]} kv heads in the prefix, {k_cache.shape[1]} in the caches")
     if sinks is not None:
-        if tuple(sinks.shape) != (Nq,):
+        if sinks.shape != (Nq,):
             raise ValueError(f"sinks {tuple(sinks.shape)} must be [{Nq}]")
         tensors.append(sinks)
     if not scale > 0 or window < 0 or window != int(window):
-        raise ValueError(f"scale {scale} must be positive and window {window} not negative")
+        raise ValueError(f"scale {scale} must be positive and window {window} a number of positions (0: none)")
     if isinstance(pos, torch.Tensor):
         if pos.dtype not in (torch.int32, torch.int64) or pos.numel() not in (1, B):
             raise ValueError(f"pos must hold 1 or {B} integers, got {tuple(pos.shape)} {pos.dtype}")
         tensors.append(pos)
     elif pos + T > k_cache.shape[2]:
         raise ValueError(f"{T} tokens from position {pos} on do not fit a cache of {k_cache.shape[2]}")
-    if any(t.device != q.device for t in tensors):
-        raise ValueError(f"all arguments must be on {q.device}")
+    for t in tensors:
+        if t.device != device:
+            raise ValueError(f"all arguments must be on {device}")
     if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
         raise ValueError("prefix_attention has no backward pass: call it under torch.no_grad()")
 
@@ -166,7 +169,7 @@ def prefix_attention(q, prefix_k, prefix_v, k_cache, v_cache, sinks, scale: floa
     Nkv, P = pk.shape[0], pk.shape[1]
     S = kc.shape[2]
     dev = q.device
-    out = torch.empty(B, T, Nq, D, dtype=torch.bfloat16, device=dev)
+    out = torch.empty((B, T, Nq, D), dtype=torch.bfloat16, device=dev)
     if out.numel() == 0:
         return out.transpose(1, 2).to(q.dtype)
     with native.on_device(q):

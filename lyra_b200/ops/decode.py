@@ -271,17 +271,18 @@ def check_moe_block(x, norm_scale, router, router_bias, w_up, up_bias, w_down, d
         raise ValueError(f"{k} routed choices and {n_shared} shared of {n} experts: k must lie in 1..{E}")
     for name, t, shape in (("norm_scale", norm_scale, (C,)), ("router", router, (C, E)), ("router_bias", router_bias, (E,)),
                            ("up_bias", up_bias, (n, 2, H)), ("down_bias", down_bias, (n, C))):
-        if t is not None and tuple(t.shape) != shape:
+        if t is not None and t.shape != shape:
             raise ValueError(f"{name} {tuple(t.shape)} must be {shape}")
     for w in (w_up, w_down):
         if isinstance(w, QArray):
             r, c = w.qval.shape[-2:]
             if len(w.block) != 2 or r % w.block[0] or c % w.block[1] or tuple(w.scale.shape) != (n, r // w.block[0], c // w.block[1]):
                 raise ValueError(f"quantised weights need 2-D blocks that divide them: block {w.block}, scale {tuple(w.scale.shape)}, values {tuple(w.qval.shape)}")
-    tensors = [t for t in (x, norm_scale, router, router_bias, up, up_bias, down, down_bias) if t is not None]
-    if any(t.device != x.device for t in tensors):
-        raise ValueError(f"all arguments must be on {x.device}")
-    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
+    device, tensors = x.device, (x, norm_scale, router, router_bias, up, up_bias, down, down_bias)
+    for t in tensors:
+        if t is not None and t.device != device:
+            raise ValueError(f"all arguments must be on {device}")
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
         raise ValueError("moe_block has no backward pass: call it under torch.no_grad()")
     return n, C, H
 
