@@ -448,34 +448,30 @@ __device__ __forceinline__ void multiply(Ring& ring, int n_units, int rows_pad, 
         lds128(at + 16, sc[t][4], sc[t][5], sc[t][6], sc[t][7]);
       }
     }
-    uint32_t raw[2][2][2][4];                      // [step parity][tile][k-16 step (bf16)]: one step ahead of the MMAs
-    auto fetch = [&](int st) {
+    auto fetch = [&](int st, uint32_t (&raw)[2][2][4]) {           // [tile][k-16 step (bf16)]
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
         if (FP8) {
-          ldsm4t(raw[st & 1][t][0], w + t * TILE1 + swz128(st * 32 + lane, warp));
+          ldsm4t(raw[t][0], w + t * TILE1 + swz128(st * 32 + lane, warp));
         } else {
 #pragma unroll
           for (int h = 0; h < 2; ++h)
-            ldsm4t(raw[st & 1][t][h], w + t * TILE1 + swz128(st * 32 + h * 16 + ((lane >> 4) << 3) + (lane & 7), (warp & 3) * 2 + ((lane >> 3) & 1)));
+            ldsm4t(raw[t][h], w + t * TILE1 + swz128(st * 32 + h * 16 + ((lane >> 4) << 3) + (lane & 7), (warp & 3) * 2 + ((lane >> 3) & 1)));
         }
       }
     };
-    fetch(0);
-#pragma unroll
-    for (int st = 0; st < STEPS; ++st) {
-      uint32_t b[NT][4];
+    auto fetch_rows = [&](int st, uint32_t (&b)[NT][4]) {
 #pragma unroll
       for (int i = 0; i < NT; ++i) ldsm4(b[i], xa + (st >> 1) * rows_pad * 128 + i * 1024 + swz128(lane & 7, (st & 1) * 4 + (lane >> 3)));
-      if (st + 1 < STEPS) fetch(st + 1);
-      uint32_t a[2][2][4];                         // [tile][k-16 step]
+    };
+    auto operand = [&](const uint32_t (&raw)[2][2][4], uint32_t (&a)[2][2][4]) {       // [tile][k-16 step]
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
         if (FP8) {
           // raw[j]: k = 8j + 2 (lane % 4) in the low half, k + 1 in the high half; columns 2 (lane / 4) and + 1 as the two bytes
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            const uint32_t v = __byte_perm(raw[st & 1][t][0][j], 0, 0x3120);
+            const uint32_t v = __byte_perm(raw[t][0][j], 0, 0x3120);
             a[t][j >> 1][(j & 1) * 2] = e4m3x2_to_f16x2(uint16_t(v & 0xffffu));
             a[t][j >> 1][(j & 1) * 2 + 1] = e4m3x2_to_f16x2(uint16_t(v >> 16));
           }
@@ -483,9 +479,11 @@ __device__ __forceinline__ void multiply(Ring& ring, int n_units, int rows_pad, 
 #pragma unroll
           for (int h = 0; h < 2; ++h)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) a[t][h][j] = raw[st & 1][t][h][j];
+            for (int j = 0; j < 4; ++j) a[t][h][j] = raw[t][h][j];
         }
       }
+    };
+    auto products = [&](int st, const uint32_t (&a)[2][2][4], const uint32_t (&b)[NT][4]) {
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
 #pragma unroll
@@ -503,6 +501,34 @@ __device__ __forceinline__ void multiply(Ring& ring, int n_units, int rows_pad, 
           }
         }
       }
+    };
+    if (FP8 && NT <= 2) {
+      // Few rows: all of the unit goes through the conversion into registers, the stage is given back, then come the products. With
+      // 64 tokens the ring has three stages; held for the whole of a unit, one of them was missing in flight.
+      uint32_t a[STEPS][2][2][4], b[STEPS][NT][4];
+#pragma unroll
+      for (int st = 0; st < STEPS; ++st) {
+        uint32_t raw[2][2][4];
+        fetch(st, raw);
+        fetch_rows(st, b[st]);
+        operand(raw, a[st]);
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(ring.empty + ring.s * 8);         // a release: the loads above come before it
+      ring.next();
+#pragma unroll
+      for (int st = 0; st < STEPS; ++st) products(st, a[st], b[st]);
+      continue;
+    }
+    uint32_t raw[2][2][2][4];                      // the weights one step ahead of the products
+    fetch(0, raw[0]);
+#pragma unroll
+    for (int st = 0; st < STEPS; ++st) {
+      uint32_t a[2][2][4], b[NT][4];
+      fetch_rows(st, b);
+      if (st + 1 < STEPS) fetch(st + 1, raw[(st + 1) & 1]);
+      operand(raw[st & 1], a);
+      products(st, a, b);
     }
     __syncwarp();
     if (lane == 0) mbar_arrive(ring.empty + ring.s * 8);
