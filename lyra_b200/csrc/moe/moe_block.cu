@@ -698,32 +698,43 @@ struct Block {
   __device__ void store_out(long long at, float v) const {
     p.out[at] = __float2bfloat16(fmaf(p.residual_scale, v, __bfloat162float(p.x[at])));
   }
-  // After the last barrier: the outputs of cut panels, summed in team order by all CTAs together (the CTA that happened to come
-  // last took 75 us for it at 64 tokens).
-  __device__ void join() const {
-    const int per = L.n_active * dn_units;
+  struct Join {                                    // four neighbouring outputs of one token and the teams first .. last that share their panel
+    const float* at[2];                            // in the slot of the first team; of a team for which the panel is the first of its run
+    long long out;
+    int first, last;
+    uint2 x;
+  };
+  __device__ bool find(int i, Join& w) const {
+    const int quads = p.C / 4, per = L.n_active * dn_units;      // C is a multiple of 8: four columns at a time stay inside a panel
+    if (i >= p.F * quads) return false;
     const Runs runs = down_runs();
-    const int quads = p.C / 4;                     // C is a multiple of 8: four columns at a time stay inside a panel
-    for (int i = c * THREADS + int(threadIdx.x); i < p.F * quads; i += G * THREADS) {
-      const int t = i / quads, g = (i - t * quads) * 4, q = g / PANEL, group = q / dn_team, q0 = group * per;
-      const int first = runs.owner(q0), last = runs.owner(q0 + per - 1);
-      if (first == last) continue;
-      const int at = t * PANEL + g % PANEL, member = q % dn_team;
-      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    const int t = i / quads, g = (i - t * quads) * 4, q = g / PANEL, group = q / dn_team, q0 = group * per;
+    w.first = runs.owner(q0);
+    w.last = runs.owner(q0 + per - 1);
+    w.out = (long long)t * p.C + g;
+    const int in_slot = t * PANEL + g % PANEL, member = q % dn_team;
+    w.at[0] = slot_of(runs, q0, w.first, dn_team, member) + in_slot;
+    w.at[1] = slot_of(runs, q0, w.first + 1, dn_team, member) + in_slot;       // the following teams begin inside the panel: slot 0 each
+    w.x = *reinterpret_cast<const uint2*>(p.x + w.out);
+    return true;
+  }
+  __device__ void join(const Join& w) const {
+    if (w.first == w.last) return;
+    float4 v = __ldcg(reinterpret_cast<const float4*>(w.at[0]));
+    const long long step = (long long)dn_team * 2 * slot_rows(p.F) * PANEL;
 #pragma unroll 8
-      for (int k = first; k <= last; ++k) {
-        const float4 part = __ldcg(reinterpret_cast<const float4*>(slot_of(runs, q0, k, dn_team, member) + at));
-        v.x += part.x;
-        v.y += part.y;
-        v.z += part.z;
-        v.w += part.w;
-      }
-      const long long o = (long long)t * p.C + g;
-      store_out(o, v.x);
-      store_out(o + 1, v.y);
-      store_out(o + 2, v.z);
-      store_out(o + 3, v.w);
+    for (int k = 0; k < w.last - w.first; ++k) {
+      const float4 part = __ldcg(reinterpret_cast<const float4*>(w.at[1] + k * step));
+      v.x += part.x;
+      v.y += part.y;
+      v.z += part.z;
+      v.w += part.w;
     }
+    const uint32_t in[2] = {w.x.x, w.x.y};
+    uint2 o;
+    o.x = pack_bf16(fmaf(p.residual_scale, v.x, __uint_as_float(in[0] << 16)), fmaf(p.residual_scale, v.y, __uint_as_float(in[0] & 0xffff0000u)));
+    o.y = pack_bf16(fmaf(p.residual_scale, v.z, __uint_as_float(in[1] << 16)), fmaf(p.residual_scale, v.w, __uint_as_float(in[1] & 0xffff0000u)));
+    *reinterpret_cast<uint2*>(p.out + w.out) = o;
   }
 
   // ---- producer side. A cursor walks a run without divisions: a warp that issues a unit every few hundred cycles has no time for
@@ -848,7 +859,7 @@ moe_block_kernel(const __grid_constant__ CUtensorMap up_map, const __grid_consta
     if (FP8) {
       for (int t = G - 1 - c; t < p.F; t += G) operand_row_f16(p, t, buf);     // the CTAs with the fewest router tasks
     } else {
-      for (int i = c * CONSUMERS + threadIdx.x; i < p.F * p.C; i += G * CONSUMERS)
+      for (int i = (G - 1 - c) * CONSUMERS + int(threadIdx.x); i < p.F * p.C; i += G * CONSUMERS)      // from the far end: the first CTAs have the router's tasks
         p.xs[i] = __bfloat16_as_ushort(__float2bfloat16(__bfloat162float(__ldg(p.x + i)) * __ldg(p.norm + i % p.C)));
     }
     const int tasks = (p.E + RE - 1) / RE * ((p.F + RT - 1) / RT) * p.csplit;
@@ -890,8 +901,16 @@ moe_block_kernel(const __grid_constant__ CUtensorMap up_map, const __grid_consta
     blk.consume_down();
   }
   asm volatile("cp.async.wait_all;" ::: "memory");
+  // the outputs of panels that run borders cut, summed in team order by all CTAs together (the CTA that happened to come last took
+  // 75 us for it at 64 tokens); where they lie is found out before the barrier
+  typename Block<FP8>::Join w;
+  int i = c * THREADS + int(threadIdx.x);
+  bool some = blk.find(i, w);
   grid.sync();
-  blk.join();
+  while (some) {
+    blk.join(w);
+    some = blk.find(i += G * THREADS, w);
+  }
   if (L.abort)
     for (int i = 0; i < 64; ++i) __nanosleep(1000);   // copies still in flight land before the shared memory is given back
 }
