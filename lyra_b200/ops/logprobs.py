@@ -98,4 +98,4 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, top_k: int, voca
             out = _TokenLogprobs.apply(rows, flat, top_k, vocab)
         else:
             out = _forward(rows, flat, top_k, vocab, None)
-    return TokenLogprobs(*out) if logits.ndim == 2 else TokenLogprobs(*(t.reshape(*lead, *t.shape[1:]) for t in out))
+    return TokenLogprobs(*out) if logits.ndim == 2 else TokenLogprobs(*(t.reshape((*lead, *t.shape[1:])) for t in out))

@@ -226,6 +226,27 @@ def test_layouts_gpu():
         ops.token_logprobs(x, targets.cpu())
 
 
+def check_one_row_without_leading_dimensions(device):
+    torch.manual_seed(8)
+    logits, target = torch.randn(301, device=device, requires_grad=True), torch.tensor(17, device=device)
+    r = ops.token_logprobs(logits, target, 3)
+    want = exact(logits.detach()[None], target[None], 3, 301)
+    assert r.logprob.shape == () and r.entropy.shape == () and r.top_logprobs.shape == (3,) and torch.equal(r.top_ids, want[3][0])
+    assert abs(float(r.logprob) - float(want[0])) < 3.2e-5 and abs(float(r.entropy) - float(want[1])) < 6.1e-4
+    (g,) = torch.autograd.grad(r.logprob, logits)
+    one = torch.ones(1, device=device)
+    assert g.shape == logits.shape and (g - exact_gradient(logits.detach()[None], target[None], 301, one, 0 * one)[0]).abs().max() < 1e-5
+
+
+def test_one_row_without_leading_dimensions_cpu():
+    check_one_row_without_leading_dimensions("cpu")
+
+
+@pytest.mark.gpu
+def test_one_row_without_leading_dimensions_gpu():
+    check_one_row_without_leading_dimensions("cuda")
+
+
 @pytest.mark.gpu
 def test_replay_in_a_graph_gpu():
     x = torch.randn(9, 5000, device="cuda").requires_grad_()
