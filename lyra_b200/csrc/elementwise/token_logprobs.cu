@@ -36,6 +36,8 @@ constexpr int CHUNK = THREADS * UNROLL * 16, STAGES = 4;   // bytes of a chunk; 
 constexpr int MAX_TOP = 32;
 constexpr int CAP = 1024;            // candidates kept; more (long runs of equal logits) take the slower selection
 constexpr int MAX_HITS = 256;        // runs looked at again
+constexpr int MAX_VOCAB = 1 << 22;   // one warp sweeps a row of ties up to 33 times (a vector of 16 bytes per lane in about 800 cycles): 0.9e9
+                                     // cycles, while the other warps' waits run out after 4e9
 constexpr int MAX_RUNS = 3584;       // run maxima kept per row (14 KB, twice: two CTAs fit an SM)
 constexpr float L2E = 1.4426950408889634f;
 // Distances below a maximum (in log2 units) are cut off here: 2^-1000 is 0 in fp32 as well, and 0 * y stays 0.
@@ -725,7 +727,7 @@ int launch_bwd(Bwd p, cudaStream_t stream) {
 extern "C" int lyra_token_logprobs(const void* x, int is_bf16, const long long* target, float* logprob, float* entropy, float* norm, float* top_lp,
                                    long long* top_id, int N, int V, int k, long long stride, int* status, cudaStream_t stream) {
   using namespace lyra::tlp;
-  if (N < 1 || N > (1 << 28) || V < 1 || V > (1 << 30) || k < 0 || k > MAX_TOP || k > V || stride < V) return -90;
+  if (N < 1 || N > (1 << 28) || V < 1 || V > MAX_VOCAB || k < 0 || k > MAX_TOP || k > V || stride < V) return -90;
   if (reinterpret_cast<uintptr_t>(x) % (is_bf16 ? 2 : 4)) return -90;
   Fwd p{x, target, logprob, entropy, norm, top_lp, top_id, stride, status, N, V, k, 1, 1};
   return is_bf16 ? launch_fwd<__nv_bfloat16>(p, stream) : launch_fwd<float>(p, stream);

@@ -176,7 +176,7 @@ def token_logprobs(logits, targets, top_k: int = 0, vocab_size: int | None = Non
 
     ``logprob`` and ``entropy`` are differentiable with respect to ``logits`` (once); the alternatives are not. A negative target
     marks a position without a token: its log probability is 0 and carries no gradient. A target from ``vocab_size`` on, a row
-    with a NaN or +inf, or one of nothing but -inf, has NaN scores and gradients. A logit of -inf is a token of probability 0."""
+    with a NaN or +inf, or one of nothing but -inf, has NaN scores and gradients. A logit of -inf is a token of probability 0. On a GPU: at most 2^22 columns."""
     vocab = logprobs_k.check_arguments(logits, targets, top_k, vocab_size)
     if use_kernels(logits, implementation):
         return logprobs_k.token_logprobs(logits, targets, top_k, vocab)

@@ -10,6 +10,7 @@ import torch
 from lyra_b200.ops import native
 
 MAX_TOP_K = 32
+MAX_VOCAB = 1 << 22      # on a GPU: a single warp may have to sweep a row of nothing but ties, in less time than a wait is given
 
 
 class TokenLogprobs(NamedTuple):
@@ -85,6 +86,8 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, top_k: int, voca
     """CUDA path; the arguments have passed :func:`check_arguments`. Rows may be strided, elements of a row may not."""
     if logits.dtype not in (torch.float32, torch.bfloat16):
         raise ValueError(f"logits must be fp32 or bf16 on a GPU, got {logits.dtype}")
+    if vocab > MAX_VOCAB:
+        raise ValueError(f"token_logprobs takes at most {MAX_VOCAB} columns on a GPU, got {vocab}")
     lead = logits.shape[:-1]
     rows, flat = logits, targets
     if logits.ndim != 2:
