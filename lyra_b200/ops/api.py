@@ -126,7 +126,8 @@ def prefix_attention(q, prefix_k, prefix_v, k_cache, v_cache, sinks, scale: floa
     ``pos`` is the number of own positions before the new tokens: an int, or an int32 tensor on the device with one value or one per
     sequence (then the call can be captured and replayed). Query ``t`` stands at absolute position ``P + pos + t``; it sees every key at
     or before it, with ``window > 0`` the last ``window`` of them. ``sinks [Nq]`` (or None) adds ``exp(sink)`` to the denominator. A sequence
-    with ``pos < 0`` is an unused place of the batch: zeros, as for a query that sees nothing without a sink.
+    with ``pos < 0`` is an unused place of the batch: zeros, as for a query that sees nothing without a sink. Places that no query of a
+    call sees may hold anything; a NaN or an infinity in a place that one query sees may reach the call's other queries.
 
     On a GPU: head dim 64 or 128; the prefix is read once per 128 query rows of a kv head instead of once per sequence."""
     attn_k.check_prefix_attention(q, prefix_k, prefix_v, k_cache, v_cache, sinks, scale, window, pos)

@@ -126,6 +126,8 @@ def check_prefix_attention(q, prefix_k, prefix_v, k_cache, v_cache, sinks, scale
         if pos.dtype not in (torch.int32, torch.int64) or pos.numel() not in (1, B):
             raise ValueError(f"pos must hold 1 or {B} integers, got {tuple(pos.shape)} {pos.dtype}")
         tensors.append(pos)
+    elif not hasattr(pos, "__index__"):
+        raise ValueError(f"pos must be an int or a tensor of integers, got {type(pos).__name__}")
     elif pos + T > k_cache.shape[2]:
         raise ValueError(f"{T} tokens from position {pos} on do not fit a cache of {k_cache.shape[2]}")
     for t in tensors:
@@ -169,6 +171,7 @@ def prefix_attention(q, prefix_k, prefix_v, k_cache, v_cache, sinks, scale: floa
     Nkv, P = pk.shape[0], pk.shape[1]
     S = kc.shape[2]
     dev = q.device
+    window = 0 if window >= P + S else int(window)            # a window of everything is none
     out = torch.empty((B, T, Nq, D), dtype=torch.bfloat16, device=dev)
     if out.numel() == 0:
         return out.transpose(1, 2).to(q.dtype)
@@ -195,7 +198,7 @@ def prefix_attention(q, prefix_k, prefix_v, k_cache, v_cache, sinks, scale: floa
         qs, ps, vs_ = qb.stride(), _steps(pk), _steps(pv)
         rc = fn(qb.data_ptr(), qs[0], qs[1], qs[2], pk.data_ptr(), ps[0], ps[1], pv.data_ptr(), vs_[0], vs_[1], address(pks), pks_step, address(pvs), pvs_step,
                 quant, kc.data_ptr(), vc.data_ptr(), address(ks), address(vs), own_quant, address(sk), address(at), at.numel() if at is not None else 0,
-                int(pos) if at is None else 0, out.data_ptr(), ws.data_ptr(), need, B, T, P, S, Nq, Nkv, D, scale, window, native.status_word().data_ptr(),
+                max(int(pos), -1) if at is None else 0, out.data_ptr(), ws.data_ptr(), need, B, T, P, S, Nq, Nkv, D, scale, window, native.status_word().data_ptr(),
                 native.stream_address())
     native.check(rc, "lyra_prefix_attention")
     native.count_launch(2 if P else 1)

@@ -132,7 +132,28 @@ def test_refusals():
         call(a, 0, implementation="b200")
 
 
+def check_numbers_of_other_types(device):
+    """A window beyond any 32-bit number or written as a float, a position far below zero; a position that is no integer is refused."""
+    a = make(2, 2, 1, 1, 40, 30, 64, device=device)
+    everything = call(a, 3, 0)
+    assert torch.equal(call(a, 3, 2**32 + 5), everything) and torch.equal(call(a, 3, 70.0), everything)
+    assert torch.equal(call(a, 3, 9.0), call(a, 3, 9)) and not torch.equal(call(a, 3, 9), everything)
+    assert call(a, -2**32, 0).abs().max() == 0
+    for pos in (1.0, 2.5, None):
+        with pytest.raises(ValueError):
+            call(a, pos)
+
+
+def test_numbers_of_other_types_cpu():
+    check_numbers_of_other_types("cpu")
+
+
 # --------------------------------------------------------------------------- GPU
+@pytest.mark.gpu
+def test_numbers_of_other_types_gpu():
+    check_numbers_of_other_types("cuda")
+
+
 def check(a, pos, window=0, scale=None):
     from lyra_b200.ops import native
 
