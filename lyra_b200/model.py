@@ -167,6 +167,8 @@ class ModelCache:
         P = prefix.pos
         if prefix.prefix_len:
             raise ValueError("a cache that continues a shared prefix cannot itself be one")
+        if any(len(l.k.shape) != 4 or l.k.shape[0] != 1 for l in prefix.layers):
+            raise ValueError("a shared prefix is the cache of one sequence")
         cut = lambda a: QArray(a.qval[0, :, :P], a.scale[0, :, :P], a.block) if isinstance(a, QArray) else a[0, :, :P]
         own = ModelCache.create(config, batch, capacity, device, n_kv_local)
         layers = tuple(replace(o, prefix_k=cut(l.k), prefix_v=cut(l.v)) for o, l in zip(own.layers, prefix.layers))

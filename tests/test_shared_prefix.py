@@ -54,6 +54,12 @@ def test_model_behind_a_prefix_equals_the_joined_sequence(fp8):
         ModelCache.share(cache, cfg, 2, 4, "cpu")
 
 
+def test_a_batch_is_no_shared_prefix():
+    c = small_config()
+    with pytest.raises(ValueError):
+        ModelCache.share(init_cache(c, 8, "cpu", 2), c, 3, 4, "cpu")
+
+
 def test_batched_generation_behind_a_prefix():
     c = small_config(compute_dtype=torch.float32, sample_temperature=0.0, seq_len=64)
     w = ModelWeights.init(0, c)
