@@ -206,6 +206,9 @@ class BatchedGenerator:
         start = self.cache.pos
         if start + n - 1 > self.capacity:
             raise ValueError(f"cache capacity {self.capacity} too small for {start} + {n - 1} positions")
+        behind, longest = self.cache.prefix_len, int(self.decode_cfg.seq_len * self.decode_cfg.rope_scale)
+        if behind and behind + start + n - 1 > longest:       # a replay reads its RoPE row by an index on the device, which nothing checks there
+            raise ValueError(f"{behind} + {start} + {n - 1} positions do not fit the model's {longest}")
         if self._graph is None:
             self._static_tok = torch.zeros(self.batch, dtype=torch.long, device=self.device)
             self.cache.pos_dev = torch.zeros(1, dtype=torch.int32, device=self.device)

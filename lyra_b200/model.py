@@ -686,6 +686,8 @@ def model_apply(tokens, model: ModelWeights, cache: ModelCache | None, config: M
             freq_cis = (cos.index_select(0, at)[None, :, None, :], sin.index_select(0, at)[None, :, None, :])
         else:
             first = behind + start_pos
+            if behind and first + T > cos.shape[0]:
+                raise ValueError(f"{T} tokens behind {first} positions do not fit the model's {cos.shape[0]}")
             freq_cis = (cos[first:first + T][None, :, None, :], sin[first:first + T][None, :, None, :])
 
         aux_loss = torch.zeros((), dtype=torch.float32, device=h.device)

@@ -77,6 +77,21 @@ def test_batched_generation_behind_a_prefix():
             gen.prefill(prompts, bad)
 
 
+def test_generation_behind_a_prefix_ends_with_the_model_s_positions():
+    """A cache may be larger than what the model's positions leave behind the prefix: the last token that fits is generated, one more is
+    refused, in steps and (before anything runs) in a recorded sequence of steps."""
+    c = small_config(compute_dtype=torch.float32, sample_temperature=0.0, seq_len=32, rope_scale=1.0)
+    w = ModelWeights.init(0, c)
+    gen = BatchedGenerator(w, c, batch=2, capacity=30, device="cpu")
+    prefix, prompts = torch.arange(20), torch.arange(10).view(2, 5)
+    first = gen.prefill(prompts, prefix)
+    assert gen.decode(first, 8).shape == (2, 8)                # 20 + 5 + 7 positions
+    for run in (gen.decode, gen._decode_graph):
+        first = gen.prefill(prompts, prefix)
+        with pytest.raises(ValueError, match="32"):
+            run(first, 9)
+
+
 def test_fused_moe_decode_is_opt_in_and_follows_the_step_by_step_path():
     c = small_config(compute_dtype=torch.float32, sample_temperature=0.0)
     assert not c.fused_moe_decode
