@@ -24,7 +24,8 @@
 // the output is rounded once at the end. The router sees neither rounding. The operand type is bf16 for bf16 weights. For e4m3
 // weights it is fp16, into which e4m3 converts in one instruction per pair (by way of bf16 it is four, and the conversions then set
 // the pace: 3.8 instead of XX TB/s); fp16 has three more bits of mantissa and a smaller range, so each token's x * norm is scaled by
-// a power of two that puts its largest value below 2^10, and the SwiGLU result by one that makes its bound (limit + 1) * limit fit.
+// a power of two that puts its largest value below 2^10, and the SwiGLU result by one that makes its bound fit: g sigmoid(beta g) lies in
+// [-0.2785 / beta, limit] for beta > 0, |l + 1| in 0 .. limit + 1.
 #include <cooperative_groups.h>
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
@@ -1014,7 +1015,7 @@ extern "C" int lyra_moe_block(const void* x, const float* norm, float eps, const
   using namespace lyra::moeblk;
   const long long need = lyra_moe_block_workspace(F, C, H, E, shared, k, fp8);
   if (need < 0 || workspace_bytes < need) return -100;
-  if (fp8 && !(limit >= 0.f && limit <= 1e4f)) return -100;   // the fp16 operand's range is fitted to it
+  if (fp8 && !(limit >= 0.f && limit <= 1e4f && beta >= 2.8e-5f)) return -100;      // the fp16 operand's range is fitted to them
   if (fp8 && (!up_scale || !down_scale || up_bk % 16 || up_bn % 16 || dn_bk % 16 || dn_bn % 16 || up_bk < 16 || up_bn < 16 || dn_bk < 16 || dn_bn < 16 ||
               C % up_bk || (2 * H) % up_bn || H % dn_bk || C % dn_bn))
     return -100;
@@ -1059,8 +1060,9 @@ extern "C" int lyra_moe_block(const void* x, const float* norm, float eps, const
   p.csplit = q.csplit; p.stages = q.stages; p.x_stage = q.x_stage; p.up_team = q.up_team; p.dn_team = q.dn_team;
   p.up_bk = up_bk; p.up_bn = up_bn; p.dn_bk = dn_bk; p.dn_bn = dn_bn;
   p.eps = eps; p.beta = beta; p.limit = limit; p.residual_scale = residual_scale;
-  int halvings = 0;                                            // that bring (limit + 1) * limit below fp16's 65504
-  while (fp8 && double(limit + 1.f) * limit > 60000.0 * exp2(halvings)) ++halvings;
+  int halvings = 0;                                            // that bring the SwiGLU result's bound below fp16's 65504
+  const double gate = limit * double(beta) > 0.279 ? limit : 0.279 / double(beta);
+  while (fp8 && double(limit + 1.f) * gate > 60000.0 * exp2(halvings)) ++halvings;
   p.act_scale = float(exp2(-halvings));
   p.act_gain = float(exp2(halvings));
   return fp8 ? launch<true>(um, dm, p, q.grid, q.smem, stream) : launch<false>(um, dm, p, q.grid, q.smem, stream);

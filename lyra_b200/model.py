@@ -466,7 +466,7 @@ def _takes_moe_block(x, w: MoEWeights, config: ModelConfig, probe: Probe, rt) ->
     from lyra_b200.ops import decode
 
     return x.dtype == torch.bfloat16 and decode.moe_block_supported(x.shape[0] * x.shape[1], c.n_embd, c.expert_hidden, c.n_routed_experts,
-                                                                    c.n_shared_experts, c.n_active_routed_experts, w.mlp_up, w.mlp_down)
+                                                                    c.n_shared_experts, c.n_active_routed_experts, w.mlp_up, w.mlp_down, c.swiglu_beta, c.swiglu_limit)
 
 
 def moe_apply(x, w: MoEWeights, config: ModelConfig, *, probe: Probe = NO_PROBE, rt=None):

@@ -287,14 +287,16 @@ def check_moe_block(x, norm_scale, router, router_bias, w_up, up_bias, w_down, d
     return n, C, H
 
 
-def moe_block_supported(F_: int, C: int, H: int, E: int, n_shared: int, k: int, w_up, w_down) -> bool:
+def moe_block_supported(F_: int, C: int, H: int, E: int, n_shared: int, k: int, w_up, w_down, beta: float = 1.0, limit: float = 7.0) -> bool:
     """Shapes of the one-kernel block: 1..64 tokens, up to 256 experts, at most 8 experts per token (shared ones included); bf16 (or
     fp32 masters, through their bf16 copies) with widths that are multiples of 8, or e4m3 for both matrices with widths and blocks
-    that are multiples of 16."""
+    that are multiples of 16, a SwiGLU limit in 0..1e4 and a beta of at least 2.8e-5 (they bound the hidden units, which are fp16 then)."""
     quant = isinstance(w_up, QArray)
     if quant != isinstance(w_down, QArray):
         return False
     if quant and any(w.qval.dtype != torch.float8_e4m3fn or w.block[0] % 16 or w.block[1] % 16 for w in (w_up, w_down)):
+        return False
+    if quant and not (0.0 <= limit <= 1e4 and beta >= 2.8e-5):
         return False
     return F_ >= 1 and _moe_block_workspace(F_, C, H, E, n_shared, k, quant) >= 0
 
@@ -318,12 +320,10 @@ def moe_block(x, norm_scale, eps, router, router_bias, w_up, up_bias, w_down, do
         return torch.empty_like(x), scores, idx
     if x.dtype != BF16:
         raise ValueError(f"moe_block takes bf16 tokens on a GPU, got {x.dtype}")
-    if not moe_block_supported(F_, C, H, E, n_shared, k, w_up, w_down):
+    if not moe_block_supported(F_, C, H, E, n_shared, k, w_up, w_down, beta, limit):
         raise ValueError(f"moe_block does not take {F_} tokens, C {C}, H {H}, {E} + {n_shared} experts, k {k}, weights "
-                         f"{type(w_up).__name__} / {type(w_down).__name__} on a GPU (ops.decode.moe_block_supported)")
+                         f"{type(w_up).__name__} / {type(w_down).__name__}, SwiGLU beta {beta} and limit {limit} on a GPU (ops.decode.moe_block_supported)")
     quant = isinstance(w_up, QArray)
-    if quant and not 0.0 <= limit <= 1e4:
-        raise ValueError(f"moe_block with e4m3 weights takes a SwiGLU limit in 0..1e4, got {limit}")
     with native.on_device(x):
         if quant:
             wu, wd = _aligned(w_up.qval), _aligned(w_down.qval)

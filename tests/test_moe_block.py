@@ -261,6 +261,49 @@ def test_every_e4m3_code_gpu():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("beta,limit", [(1e-4, 1000.0), (2.8e-5, 7.0), (1.702, 0.0)])
+def test_hidden_units_of_any_size_with_e4m3_weights_gpu(beta, limit):
+    """Gates far below zero under a small beta make hidden units of up to 0.2785 (limit + 1) / beta, beyond fp16 unless they are scaled.
+    The weights copy hidden units to the output one by one. Tolerance: the gate and the linear half carry the rounding of x * norm to fp16
+    (2^-11, as do both products with their sums of one term) and the hidden unit, fp16 after a power of two, 2^-11 of itself or half a step
+    of the smallest size, 2^-25 times that power (bound / 60000, rounded up); the output 2^-8 of itself. |d(g sigmoid(b g)) / dg| <= 1.1."""
+    C, H = 16, 16
+    a = make(1, C, H, 1, 1, 0, False, False, "cuda")
+    x = torch.linspace(-2.0, 2.0, C, device="cuda").to(torch.bfloat16)[None]
+    eye = torch.eye(C, device="cuda")
+    up = torch.cat([eye, eye], 1)[None].to(E4M3)
+    for gate_scale in (1.0, 1 / beta):
+        for linear_scale in (1.0, max(limit, 1.0)):
+            scale = torch.tensor([[[gate_scale, linear_scale]]], device="cuda")
+            w_up = QArray(up, scale, (16, 16))
+            w_down = QArray(eye[None].to(E4M3), torch.ones(1, 1, 1, device="cuda"), (16, 16))
+            with torch.no_grad():
+                out = ops.moe_block(x, a["norm"], EPS, a["router"], None, w_up, None, w_down, None, 1, 0, beta, limit, 1.0)[0]
+            xd = x.double()
+            xn = xd / torch.sqrt((xd * xd).mean() + EPS) * a["norm"].double()
+            g, l = (xn * gate_scale).clamp(max=limit), (xn * linear_scale).clamp(-limit, limit)
+            s = g * torch.sigmoid(beta * g)
+            act = (l + 1) * s
+            step = 2.0**-11 * 1.05
+            err = (step * (xn * linear_scale).abs()) * s.abs() + 1.1 * step * (xn * gate_scale).abs() * ((l + 1).abs() * 1.001 + 1e-3)
+            top = (limit + 1) * max(limit, 0.279 / beta)
+            err = err + step * act.abs() + 2.0**-25 * max(1.0, 2 * top / 60000)
+            err = err + 2.0**-8 * ((xd + act).abs() + err)
+            assert ((out.double() - (xd + act)).abs() <= err).all(), ((out.double() - (xd + act)).abs() / err).max()
+
+
+@pytest.mark.gpu
+def test_sizes_of_hidden_units_that_are_refused_gpu():
+    from lyra_b200.ops import decode
+
+    a = make(2, 64, 48, 6, 2, 1, True, True, "cuda")
+    for beta, limit in ((0.0, 7.0), (-1.0, 7.0), (1e-6, 7.0), (1.702, 2e4), (1.702, -1.0), (float("nan"), 7.0)):
+        with pytest.raises(ValueError), torch.no_grad():
+            ops.moe_block(a["x"], a["norm"], EPS, a["router"], a["router_bias"], a["up"], a["up_bias"], a["down"], a["down_bias"], 2, 1, beta, limit, 1.0)
+        assert not decode.moe_block_supported(2, 64, 48, 6, 1, 2, a["up"], a["down"], beta, limit)
+
+
+@pytest.mark.gpu
 def test_refusals_and_layouts_gpu():
     from lyra_b200.ops import decode
 
