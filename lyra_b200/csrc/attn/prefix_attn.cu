@@ -306,7 +306,7 @@ prefix_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CU
       if (!(ok = loaders_agree<LOADERS>(ok))) break;
       if (!mbar_wait(smem_u32(&q_empty), (n & 1) ^ 1, abortp)) ok = false;
       if (ok) {
-#pragma unroll 8
+#pragma unroll 4
         for (int i = tid; i < BM * CPR; i += LOADERS) {
           const int r = i / CPR, c = i % CPR;
           const long long at = q_row[r];
@@ -323,6 +323,7 @@ prefix_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CU
           const int k0 = w.key + j * BN;
           // slot t % 8 is free: the stage of tile t is, so the scores of tile t - NS are done; they were asked for after the
           // probabilities of tile t - 2 NS, and those came after the group was through with tile t - 8
+#pragma unroll 1
           for (int which = 0; which < 2; ++which) {
             const uint32_t i = 2 * t + which, rs = i % RAW;
             if (!mbar_wait(smem_u32(which ? &v_empty[s] : &s_full[s]), ph ^ 1, abortp) || !mbar_wait(smem_u32(&raw_full[rs]), (i / RAW) & 1, abortp)) {
@@ -332,7 +333,7 @@ prefix_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CU
             const uint8_t* from = sR + rs * RAW_TILE;
             uint8_t* to = (which ? sV : sK) + s * TILE;
             constexpr int RC = D / 16;          // 16-byte chunks per raw row
-#pragma unroll 4
+#pragma unroll 2
             for (int x = tid; x < BN * RC; x += LOADERS) {
               const int r = x / RC, c = x % RC;
               const uint4 v = *reinterpret_cast<const uint4*>(from + x * 16);
@@ -408,11 +409,11 @@ prefix_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CU
               }
             }
             if (need_mask) {
+              const int from = lo - (k0 + c * 32), to = p.P - (k0 + c * 32);        // places [from, to) of the 32 are visible
+              const uint32_t seen = (to >= 32 ? ~0u : to > 0 ? (1u << to) - 1u : 0u) & (from <= 0 ? ~0u : from < 32 ? ~0u << from : 0u);
 #pragma unroll
-              for (int i = 0; i < 32; ++i) {
-                const int kk = k0 + c * 32 + i;
-                if (kk >= p.P || kk < lo) r[i] = 0xff800000u;
-              }
+              for (int i = 0; i < 32; ++i)
+                if (!(seen >> i & 1u)) r[i] = 0xff800000u;
             }
           };
           const float s2 = FP8 ? 1.f : sc;      // e4m3: the softmax scale came in with the key's
@@ -473,9 +474,11 @@ prefix_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CU
               }
             }
           };
-          pass();
-          const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * s2;
-          if (__any_sync(0xffffffffu, mx > ref + 8.f)) {
+#pragma unroll 1                                 // one copy of the pass in the program (see the merge in own_kernel)
+          for (int again = 0;; ++again) {
+            pass();
+            const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * s2;
+            if (again || !__any_sync(0xffffffffu, mx > ref + 8.f)) break;
             float factor = 1.f;
             if (mx > ref + 8.f) {
               factor = exp2f(ref - mx);
@@ -495,7 +498,6 @@ prefix_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CU
                 tmem_st32(o_addr + c * 32, o);
               }
             }
-            pass();
           }
           tmem_st32(s_addr, pk[0]);
           tmem_st32(s_addr + 32, pk[1]);
@@ -899,6 +901,8 @@ __global__ void __launch_bounds__(OTHREADS, D == 64 ? 4 : 3) own_kernel(const Ow
   // ---- sums, a row's columns dealt to the CTAs of a cluster. Neighbouring threads take neighbouring rows, which lie side by side in
   // the prefix partials (four at a time where they start on such a border); the results go through shared memory and leave row by row.
   // A thread fetches the splits of several places before it adds them up: one place at a time this took up to 15 us, most of it waiting.
+  // The program is kept short on purpose, here and in the softmax: in a decode step a kernel's instructions come from memory as often as
+  // not, and with twice the unrolling a call of 4 x 16 heads took 24 us instead of 18, one of 32 x 32 heads over e4m3 49 instead of 39.
   const int dn = D / p.cluster, d0 = rank * dn;                  // this CTA's columns
   const int m0 = b * R + row0, n_own = ROWS ? 1 : p.cluster;
   float* result = ROWS || p.cluster == 1 ? comb : warp_o;        // in place, unless the cluster's other CTAs still read it
@@ -913,25 +917,25 @@ __global__ void __launch_bounds__(OTHREADS, D == 64 ? 4 : 3) own_kernel(const Ow
   auto place = [&](int r, int d) { return part + (long long)((m0 % BM + r) / BM) * p.splits * D * BM + d * BM + r - (m0 % BM + r) / BM * BM; };
   if (n_rows % 4 == 0 && m0 % 4 == 0) {
     const int nq = n_rows / 4, total = dn * nq;
-    constexpr int E = 2;
+    constexpr int E = ROWS ? 2 : 1, J = ROWS ? 4 : 8;            // places and splits in flight per thread (few rows: 128 places or fewer)
     for (int i0 = tid; i0 < total; i0 += E * OTHREADS) {
       float4 v[E];
 #pragma unroll
       for (int e = 0; e < E; ++e) v[e] = make_float4(0.f, 0.f, 0.f, 0.f);
-      for (int j0 = 0; j0 < p.splits; j0 += 4) {
-        float4 x[E][4];
+      for (int j0 = 0; j0 < p.splits; j0 += J) {
+        float4 x[E][J];
 #pragma unroll
         for (int e = 0; e < E; ++e) {
           const int i = min(i0 + e * OTHREADS, total - 1), d = d0 + i / nq, r = i % nq * 4;
           const float* at = place(r, d);
 #pragma unroll
-          for (int j = 0; j < 4; ++j) x[e][j] = __ldcg(reinterpret_cast<const float4*>(at + (long long)min(j0 + j, p.splits - 1) * D * BM));
+          for (int j = 0; j < J; ++j) x[e][j] = __ldcg(reinterpret_cast<const float4*>(at + (long long)min(j0 + j, p.splits - 1) * D * BM));
         }
 #pragma unroll
         for (int e = 0; e < E; ++e) {
           const int r = min(i0 + e * OTHREADS, total - 1) % nq * 4;
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
+          for (int j = 0; j < J; ++j) {
             if (j0 + j < p.splits) {
               v[e].x = fmaf(x[e][j].x, weight[r][n_own + j0 + j], v[e].x);
               v[e].y = fmaf(x[e][j].y, weight[r + 1][n_own + j0 + j], v[e].y);
@@ -945,11 +949,11 @@ __global__ void __launch_bounds__(OTHREADS, D == 64 ? 4 : 3) own_kernel(const Ow
       for (int e = 0; e < E; ++e) {
         const int i = i0 + e * OTHREADS, d = d0 + i / nq, r = i % nq * 4;
         if (i < total) {
-          const float add[4] = {v[e].x, v[e].y, v[e].z, v[e].w};
-#pragma unroll
+#pragma unroll 1
           for (int y = 0; y < 4; ++y) {
+            const float add = y == 0 ? v[e].x : y == 1 ? v[e].y : y == 2 ? v[e].z : v[e].w;
             const float inv = weight[r + y][MAXW];               // 0: nothing visible, or an unused place - whatever the sums hold
-            result[(r + y) * PITCH + d] = inv == 0.f ? 0.f : (own_part(r + y, d) + add[y]) * inv;
+            result[(r + y) * PITCH + d] = inv == 0.f ? 0.f : (own_part(r + y, d) + add) * inv;
           }
         }
       }
@@ -960,7 +964,7 @@ __global__ void __launch_bounds__(OTHREADS, D == 64 ? 4 : 3) own_kernel(const Ow
       const float inv = weight[r][MAXW];
       const float* at = place(r, d);
       float v = 0.f;
-#pragma unroll 8
+#pragma unroll 2
       for (int j = 0; j < p.splits; ++j) v = fmaf(__ldcg(at + (long long)j * D * BM), weight[r][n_own + j], v);
       result[r * PITCH + d] = inv == 0.f ? 0.f : (own_part(r, d) + v) * inv;
     }
@@ -1086,7 +1090,7 @@ extern "C" int lyra_prefix_attention(const void* q, long long q_sb, long long q_
                                      const void* pv, long long pv_sh, long long pv_sp, const float* pk_scale, long long pks_sh, const float* pv_scale,
                                      long long pvs_sh, int prefix_fp8, const void* k, const void* v, const float* k_scale, const float* v_scale, int own_fp8,
                                      const float* sinks, const int* pos, int pos_n, int pos_host, void* out, void* workspace, long long workspace_bytes,
-                                     int B, int T, int P, int S,                                     int Nq, int Nkv, int D, float scale, int window, int* status, cudaStream_t stream) {
+                                     int B, int T, int P, int S, int Nq, int Nkv, int D, float scale, int window, int* status, cudaStream_t stream) {
   using namespace lyra;
   using namespace lyra::prefix;
   const long long need = lyra_prefix_attention_workspace(B, T, P, Nq, Nkv, D, window);

@@ -1010,7 +1010,7 @@ extern "C" long long lyra_moe_block_workspace(int F, int C, int H, int E, int sh
 extern "C" int lyra_moe_block(const void* x, const float* norm, float eps, const float* router, const float* router_bias, const void* up, const float* up_scale,
                               int up_bk, int up_bn, const float* up_bias, const void* down, const float* down_scale, int dn_bk, int dn_bn,
                               const float* down_bias, void* out, float* scores, long long* idx, void* workspace, long long workspace_bytes, int F, int C, int H, int E,
-                              int shared,                              int k, int fp8, float beta, float limit, float residual_scale, int* status, cudaStream_t stream) {
+                              int shared, int k, int fp8, float beta, float limit, float residual_scale, int* status, cudaStream_t stream) {
   using namespace lyra;
   using namespace lyra::moeblk;
   const long long need = lyra_moe_block_workspace(F, C, H, E, shared, k, fp8);
