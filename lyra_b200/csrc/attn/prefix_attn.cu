@@ -11,6 +11,10 @@
 //   own_kernel     each sequence against its own cache: no reuse beyond the rep heads, bound by reading the cache, so warp MMAs with
 //                  many bytes in flight. Its last step merges the prefix partials, its own and the sink, and rounds once.
 //
+// 64 query heads of 64 over 8 kv heads, bf16: 256 sequences behind 32768 shared positions with up to 1024 own ones 272 us, of which the
+// prefix kernel has 218: the softmax (its exponentials and their issue, about 1450 clk per 128 x 128 tile and SM) bounds it, the tensor
+// cores need 600 of them; the rest is the own caches at 4 TB/s. 64 sequences behind 8192 positions with up to 512: 40 us.
+//
 // Prefix kernel, per item (row tile, kv head, key split), one persistent CTA per SM:
 //   warp 0        TMA producer: K and V tiles of 128 keys (bf16: straight into the operand tiles; e4m3: into a raw ring)
 //   warp 1        tcgen05 issuer:  S = Q K_j^T  and, e4m3, O_g += P V_j   (g = j mod 2)
