@@ -3,6 +3,8 @@ heads-first views (``x.transpose(1, 2)``) of such tensors are accepted without a
 
 from __future__ import annotations
 
+import functools
+
 import torch
 
 from lyra_b200.nn.quant import QArray
@@ -149,12 +151,15 @@ def _rows16(t: torch.Tensor) -> torch.Tensor:
 
 
 def _scales(t: QArray, contiguous: bool) -> torch.Tensor:
-    """fp32 ``[..., positions]`` of a cache's scales."""
+    """fp32 ``[..., positions, 1]`` of a cache's scales, neighbouring positions side by side."""
     s = t.scale if t.scale.dtype == torch.float32 else t.scale.float()
-    if contiguous:
-        return s if s.is_contiguous() else s.contiguous()
-    s = s[..., 0]
-    return s if s.stride(-1) == 1 or s.shape[-1] <= 1 else s.contiguous()
+    ready = s.is_contiguous() or (not contiguous and (s.stride(-2) == 1 or s.shape[-2] <= 1))
+    return s if ready else s.contiguous()
+
+
+@functools.lru_cache(maxsize=256)
+def _prefix_workspace(*shape: int) -> int:
+    return native.function("lyra_prefix_attention_workspace", "iiiiiii", c_ll)(*shape)
 
 
 def prefix_attention(q, prefix_k, prefix_v, k_cache, v_cache, sinks, scale: float, window: int, pos):
@@ -176,7 +181,7 @@ def prefix_attention(q, prefix_k, prefix_v, k_cache, v_cache, sinks, scale: floa
     if out.numel() == 0:
         return out.transpose(1, 2).to(q.dtype)
     with native.on_device(q):
-        need = native.function("lyra_prefix_attention_workspace", "iiiiiii", c_ll)(B, T, P, Nq, Nkv, D, window)
+        need = _prefix_workspace(B, T, P, Nq, Nkv, D, window)
         if need < 0:
             raise ValueError(f"prefix_attention does not take B {B}, T {T}, {Nq} / {Nkv} heads on a GPU")
         ws = torch.empty(need, dtype=torch.uint8, device=dev)

@@ -79,18 +79,21 @@ def ptr(t: torch.Tensor | None) -> c_void_p:
 
 
 def stream_address() -> int:
-    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
+    return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
 
 
 def stream_ptr() -> c_void_p:
     return c_void_p(torch._C._cuda_getCurrentRawStream(torch.cuda.current_device()))
 
 
+_NOTHING = contextlib.nullcontext()
+
+
 def on_device(t: torch.Tensor):
     """Context in which ``t``'s GPU is the current one: a launch goes to the current device's stream, which for a tensor of
     another GPU would be the wrong stream. Free of cost where the device is current already."""
-    if t.device.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
+    if t.device.index == torch._C._cuda_getDevice():
+        return _NOTHING
     return torch.cuda.device(t.device)
 
 
