@@ -7,6 +7,8 @@ fp8 caches carry one fp32 scale per (sequence, kv head, position) and are dequan
 
 from __future__ import annotations
 
+import functools
+
 import torch
 
 from lyra_b200.nn.quant import QArray, dequantize
@@ -301,6 +303,7 @@ def moe_block_supported(F_: int, C: int, H: int, E: int, n_shared: int, k: int, 
     return F_ >= 1 and _moe_block_workspace(F_, C, H, E, n_shared, k, quant) >= 0
 
 
+@functools.lru_cache(maxsize=256)
 def _moe_block_workspace(F_, C, H, E, n_shared, k, quant) -> int:
     return native.function("lyra_moe_block_workspace", "iiiiiii", c_ll)(F_, C, H, E, n_shared, k, quant)
 
